@@ -55,7 +55,7 @@ template <> struct VecOf<bf16_t> { typedef bf16_t type __attribute__((ext_vector
 
 __device__ __forceinline__ float silu_f(float x) { return x / (1.0f + __expf(-x)); }
 __device__ __forceinline__ float gelu_erf_f(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f)); }
-// val * GELU(gate) for the GEGLU epilogues.  16-bit outputs: two values per instruction on the packed fp32 pipe,
+// val * GELU(gate) for the GEGLU epilogues.  16-bit outputs, two values at a time:
 // erf(g / sqrt 2) = g P(g^2) / Q(g^2) with cubic P and Q (fitted on |g| <= 3.3 sqrt 2, where erf has reached
 // 1 - 3e-6; |error| <= 2.7e-6, the result stays inside (-1, 1)): one reciprocal and no exponential per value, about
 // two thirds of the vector instructions of the series form with an exponential (Abramowitz & Stegun 7.1.26) that it
