@@ -310,6 +310,54 @@ int sdmi_conv2d_splits(int m, int n, int k, int dtype);
  * per workgroup; its results equal the general kernel's bit for bit.) */
 int sdmi_attention(const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, void* out, int ldo,
                    int batch, int heads, int nq, int nk, int d, float scale, int dtype, int impl, void* stream);
+/* ------------------------------------------------------------------------------------------
+ * Layers with dropout and gradients, for tuning the denoiser: what ResBlock (GroupNorm, SiLU, Dropout
+ * ahead of its second convolution, :3130-3234), CrossAttention (to_out: Linear, Dropout, :2776-2797) and
+ * FeedForward (:2697-2724) hold between their convolutions and attentions.
+ *
+ * The dropout mask is a function of (seed, offset, row, column) and is never stored: Philox4x32-10 with key =
+ * seed and counter = (column / 8, row, row >> 32, offset) gives eight 16-bit numbers, one per column of the
+ * group, low halves first; an element is kept if its number is at least round(p 65536) and scaled by the
+ * reciprocal of the probability so used.  Dropped elements are 0 whatever they held.  Rows and columns are
+ * those of the result ([rows][cols]; a pixel is a row), so the same (seed, offset) drops the same elements in
+ * sdmi_dropout and in the fused calls.  seed_dev: NULL, or 8 bytes of device memory the seed is read from
+ * instead (a replayed graph then draws anew when they change).  offset: 0 .. 2^32 - 1, one per layer or call.
+ * p in [0, 1].  act: 0 none, 1 SiLU, 2 GELU (erf), 3 z sigmoid(1.702 z).
+ *
+ * Workspaces are device memory of *_workspace_bytes(...) bytes (0: NULL will do) that a call reads only what
+ * it wrote itself: nothing to clear, but calls that overlap in time need one each.  Pointers need the
+ * alignment of their elements only (16-byte rows are faster).  Empty tensors are fine (their sums are 0).
+ * ------------------------------------------------------------------------------------------ */
+/* out[r][c] = [resid +] dropout(x)[r][c]; the gradient of x is the same call on the gradient (resid NULL).  ldx,
+ * ldr: elements from row to row; out is dense. */
+int sdmi_dropout(const void* x, int64_t ldx, const void* resid, int64_t ldr, void* out, int64_t rows, int cols, double p,
+                 int64_t seed, const int64_t* seed_dev, int64_t offset, int dtype, void* stream);
+/* z = x W^T + bias; out = [resid +] dropout(act(z)).  x [rows][ldx], w [n][ldw], resid [rows][ldr], out
+ * [rows][n] in dtype; bias fp32 or NULL.  preact: NULL, or fp32 [rows][n] that receives z for the backward
+ * call (an activation's derivative taken at a z of 16 bits would show in the fp32 bias gradient). */
+int64_t sdmi_linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype);
+int sdmi_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* resid,
+                    int64_t ldr, void* out, float* preact, int64_t rows, int k, int n, int act, double p, int64_t seed,
+                    const int64_t* seed_dev, int64_t offset, void* workspace, int dtype, void* stream);
+/* dz = dropout(dy) act'(z); dx = dz W [rows][k], dw = dz^T x [n][k] in dtype, db = column sums of dz, fp32; each may
+ * be NULL.  want of the workspace: 1 dx + 2 dw + 4 db.  preact is needed with an activation only.  resid's gradient
+ * is dy. */
+int64_t sdmi_linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype);
+int sdmi_linear_act_backward(const void* dy, int64_t lddy, const float* preact, const void* x, int64_t ldx, const void* w,
+                             int64_t ldw, void* dx, void* dw, float* db, int64_t rows, int k, int n, int act, double p,
+                             int64_t seed, const int64_t* seed_dev, int64_t offset, void* workspace, int dtype,
+                             void* stream);
+/* out = dropout(act(GroupNorm(x0 | x1))), channels last; x1 NULL with c1 = 0.  Any channel count up to 8192 that
+ * `groups` divides, any hw.  stats: fp32 [batch][groups][2], receives (mean, 1 / sqrt(var + eps)). */
+int64_t sdmi_groupnorm_act_workspace_bytes(int batch, int64_t hw, int c0, int c1, int groups, int dtype, int backward);
+int sdmi_groupnorm_act(const void* x0, int c0, const void* x1, int c1, int batch, int64_t hw, int groups, float eps,
+                       const float* gamma, const float* beta, int act, double p, int64_t seed, const int64_t* seed_dev,
+                       int64_t offset, void* out, float* stats, void* workspace, int dtype, void* stream);
+/* dx0 / dx1 in dtype, dgamma / dbeta fp32; each may be NULL (dx0 and dx1 together). */
+int sdmi_groupnorm_act_backward(const void* dy, const void* x0, int c0, const void* x1, int c1, int batch, int64_t hw,
+                                int groups, const float* gamma, const float* beta, const float* stats, int act, double p,
+                                int64_t seed, const int64_t* seed_dev, int64_t offset, void* dx0, void* dx1,
+                                float* dgamma, float* dbeta, void* workspace, int dtype, void* stream);
 /* timestep_embedding :2212-2232 (fp32 out [batch][dim]) */
 int sdmi_timestep_embedding(const int64_t* t, float* out, int batch, int dim, float max_period, void* stream);
 /* y = act_out(act_in(x) W^T + b), fp32, small M (time_embed :3317-3322, emb_layers :3180-3183) */

@@ -13,6 +13,7 @@ CSRC = os.path.join(_HERE, "csrc")
 
 c_void_p, c_int, c_float, c_int64, c_char_p = (ctypes.c_void_p, ctypes.c_int, ctypes.c_float,
                                                 ctypes.c_int64, ctypes.c_char_p)
+c_double = ctypes.c_double
 P = ctypes.POINTER
 
 F32, F16, BF16 = 0, 1, 2
@@ -111,6 +112,23 @@ SIGNATURES = {
     "sdmi_conv2d_splits": (c_int, [c_int, c_int, c_int, c_int]),
     "sdmi_attention": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                                c_int, c_int, c_int, c_float, c_int, c_int, c_void_p]),
+    "sdmi_dropout": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_double, c_int64, c_void_p,
+                             c_int64, c_int, c_void_p]),
+    "sdmi_linear_act_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int]),
+    "sdmi_linear_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                                c_int64, c_int, c_int, c_int, c_double, c_int64, c_void_p, c_int64, c_void_p, c_int,
+                                c_void_p]),
+    "sdmi_linear_act_backward_workspace_bytes": (c_int64, [c_int64, c_int, c_int, c_int, c_double, c_int, c_int]),
+    "sdmi_linear_act_backward": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                         c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_double, c_int64, c_void_p,
+                                         c_int64, c_void_p, c_int, c_void_p]),
+    "sdmi_groupnorm_act_workspace_bytes": (c_int64, [c_int, c_int64, c_int, c_int, c_int, c_int, c_int]),
+    "sdmi_groupnorm_act": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int, c_float, c_void_p, c_void_p,
+                                   c_int, c_double, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                   c_void_p]),
+    "sdmi_groupnorm_act_backward": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int64, c_int, c_void_p,
+                                            c_void_p, c_void_p, c_int, c_double, c_int64, c_void_p, c_int64, c_void_p,
+                                            c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "sdmi_timestep_embedding": (c_int, [c_void_p, c_void_p, c_int, c_int, c_float, c_void_p]),
     "sdmi_small_linear": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                   c_void_p]),

@@ -290,6 +290,64 @@ int sdmi_attention(const void* q, int ldq, const void* k, int ldk, const void* v
   return attention(a, (hipStream_t)stream);
 }
 
+int sdmi_dropout(const void* x, int64_t ldx, const void* resid, int64_t ldr, void* out, int64_t rows, int cols, double p,
+                 int64_t seed, const int64_t* seed_dev, int64_t offset, int dtype, void* stream) {
+  DropoutArgs a;
+  a.x = x; a.ldx = ldx; a.resid = resid; a.ldr = ldr; a.out = out; a.rows = rows; a.cols = cols; a.p = p;
+  a.seed = seed; a.seed_dev = seed_dev; a.offset = offset; a.dtype = dtype;
+  return dropout(a, (hipStream_t)stream);
+}
+
+int64_t sdmi_linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype) {
+  return linear_act_workspace_bytes(rows, k, n, dtype);
+}
+int sdmi_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, const void* resid,
+                    int64_t ldr, void* out, float* preact, int64_t rows, int k, int n, int act, double p, int64_t seed,
+                    const int64_t* seed_dev, int64_t offset, void* workspace, int dtype, void* stream) {
+  LinearActArgs a;
+  a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw; a.bias = bias; a.resid = resid; a.ldr = ldr; a.out = out; a.preact = preact;
+  a.rows = rows; a.k = k; a.n = n; a.act = act; a.p = p; a.seed = seed; a.seed_dev = seed_dev; a.offset = offset;
+  a.workspace = workspace; a.dtype = dtype;
+  return linear_act(a, (hipStream_t)stream);
+}
+int64_t sdmi_linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype) {
+  return linear_act_backward_workspace_bytes(rows, k, n, act, p, want, dtype);
+}
+int sdmi_linear_act_backward(const void* dy, int64_t lddy, const float* preact, const void* x, int64_t ldx, const void* w,
+                             int64_t ldw, void* dx, void* dw, float* db, int64_t rows, int k, int n, int act, double p,
+                             int64_t seed, const int64_t* seed_dev, int64_t offset, void* workspace, int dtype,
+                             void* stream) {
+  LinearActArgs a;
+  a.dy = dy; a.lddy = lddy; a.preact = const_cast<float*>(preact); a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
+  a.dx = dx; a.dw = dw; a.db = db; a.rows = rows; a.k = k; a.n = n; a.act = act; a.p = p; a.seed = seed;
+  a.seed_dev = seed_dev; a.offset = offset; a.workspace = workspace; a.dtype = dtype;
+  return linear_act_backward(a, (hipStream_t)stream);
+}
+
+int64_t sdmi_groupnorm_act_workspace_bytes(int batch, int64_t hw, int c0, int c1, int groups, int dtype, int backward) {
+  return groupnorm_act_workspace_bytes(batch, hw, c0, c1, groups, dtype, backward);
+}
+int sdmi_groupnorm_act(const void* x0, int c0, const void* x1, int c1, int batch, int64_t hw, int groups, float eps,
+                       const float* gamma, const float* beta, int act, double p, int64_t seed, const int64_t* seed_dev,
+                       int64_t offset, void* out, float* stats, void* workspace, int dtype, void* stream) {
+  GroupNormActArgs a;
+  a.x0 = x0; a.c0 = c0; a.x1 = x1; a.c1 = c1; a.B = batch; a.HW = hw; a.groups = groups; a.eps = eps; a.gamma = gamma;
+  a.beta = beta; a.act = act; a.p = p; a.seed = seed; a.seed_dev = seed_dev; a.offset = offset; a.out = out;
+  a.stats = stats; a.workspace = workspace; a.dtype = dtype;
+  return groupnorm_act(a, (hipStream_t)stream);
+}
+int sdmi_groupnorm_act_backward(const void* dy, const void* x0, int c0, const void* x1, int c1, int batch, int64_t hw,
+                                int groups, const float* gamma, const float* beta, const float* stats, int act, double p,
+                                int64_t seed, const int64_t* seed_dev, int64_t offset, void* dx0, void* dx1,
+                                float* dgamma, float* dbeta, void* workspace, int dtype, void* stream) {
+  GroupNormActArgs a;
+  a.dy = dy; a.x0 = x0; a.c0 = c0; a.x1 = x1; a.c1 = c1; a.B = batch; a.HW = hw; a.groups = groups; a.gamma = gamma;
+  a.beta = beta; a.stats = const_cast<float*>(stats); a.act = act; a.p = p; a.seed = seed; a.seed_dev = seed_dev;
+  a.offset = offset; a.dx0 = dx0; a.dx1 = dx1; a.dgamma = dgamma; a.dbeta = dbeta; a.workspace = workspace;
+  a.dtype = dtype;
+  return groupnorm_act_backward(a, (hipStream_t)stream);
+}
+
 int sdmi_timestep_embedding(const int64_t* t, float* out, int batch, int dim, float max_period, void* stream) {
   return timestep_embedding(t, out, batch, dim, max_period, (hipStream_t)stream);
 }

@@ -1,0 +1,719 @@
+// GroupNorm with activation and dropout, channels last, and its gradients:
+//   xh = (x - mean_g) rstd_g      u = gamma xh + beta        y = drop(act(u))
+//   du = drop(dy) act'(u)         dgamma = sum du xh         dbeta = sum du        h = gamma du
+//   dx = rstd_g (h - mean_g(h) - xh mean_g(h xh))            (means over the sample's group)
+// The input may be the channel concatenation of two tensors; any channel count per group, any image size.
+//
+// A (sample, group) slice that fits LDS is one workgroup's work: read once, normalised from LDS, one launch (the
+// weight gradients of several samples take a second one).  Larger slices take two launches over strips of pixels:
+// the first leaves per-strip sums, the second folds them in double and finishes the strip.  Every sum is taken in a
+// fixed order.  Statistics are taken about a value of the group (its first one), so that a common offset does not
+// cancel in E[x^2] - E[x]^2.
+#include "act_drop.h"
+#include "ops.h"
+#include <stdio.h>
+
+namespace {
+
+constexpr int GNA_MAX_C = 8192;               // channel sums of a strip fit LDS
+
+struct GnaParams {
+  const void* x0; const void* x1; const void* dy;
+  void* out0; void* out1;                     // forward: out0 = y [B][HW][C]; backward: dx of x0, x1
+  int c0, c1, C, G, cpg, B;
+  int64_t HW;
+  FastDiv div_cpg;
+  float eps;
+  const float* gamma; const float* beta;
+  int act;
+  DropArgs drop;
+  float* stats;                               // [B][G][2]: mean, rstd
+  int strips; int64_t px_per_strip;
+  float* part;                                // [B][strips][G][2] sums of a strip's groups
+  float* cpart;                               // backward: [B][strips][2][C] sums of a strip's channels
+  float* dgamma; float* dbeta;
+  int apply_blocks;                           // backward: blockIdx.x beyond fold dgamma / dbeta
+};
+
+// columns c .. c + W - 1 (of C) of pixel row `row` of the two-source tensor
+template <typename T, int W>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[W]) {
+  if constexpr (W == 8) load8<T>(p, 8, v);
+  else {
+    typedef T V __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    if constexpr (W == 1) v[0] = to_f32<T>(*p);
+    else {
+      const V r = *reinterpret_cast<const V*>(p);
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = to_f32<T>(r[e]);
+    }
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_n(T* p, const float (&v)[W]) {
+  if constexpr (W == 8) store8<T>(p, 8, v);
+  else if constexpr (W == 1) *p = from_f32<T>(v[0]);
+  else {
+    typedef T V __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    V r;
+#pragma unroll
+    for (int e = 0; e < W; ++e) r[e] = from_f32<T>(v[e]);
+    *reinterpret_cast<V*>(p) = r;
+  }
+}
+// eight columns that may be short (the row's last) or straddle the two sources
+template <typename T>
+__device__ __forceinline__ void load_cols(const void* x0, const void* x1, int c0, int c1, int64_t row, int c, float (&v)[8]) {
+  if (!x1) load8<T>((const T*)x0 + row * c0 + c, c0 - c, v);
+  else if (c + 8 <= c0) load8<T>((const T*)x0 + row * c0 + c, 8, v);
+  else if (c >= c0) load8<T>((const T*)x1 + row * c1 + (c - c0), c1 - (c - c0), v);
+  else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e;
+      v[e] = ce < c0 ? to_f32<T>(((const T*)x0)[row * c0 + ce])
+                     : (ce < c0 + c1 ? to_f32<T>(((const T*)x1)[row * c1 + (ce - c0)]) : 0.f);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(void* x0, void* x1, int c0, int c1, int64_t row, int c, const float (&v)[8]) {
+  if (!x1) store8<T>((T*)x0 + row * c0 + c, c0 - c, v);
+  else if (c + 8 <= c0) store8<T>((T*)x0 + row * c0 + c, 8, v);
+  else if (c >= c0) store8<T>((T*)x1 + row * c1 + (c - c0), c1 - (c - c0), v);
+  else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e;
+      if (ce < c0) ((T*)x0)[row * c0 + ce] = from_f32<T>(v[e]);
+      else if (ce < c0 + c1) ((T*)x1)[row * c1 + (ce - c0)] = from_f32<T>(v[e]);
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ float first_of(const GnaParams& p, int b, int c) {
+  const int64_t row = (int64_t)b * p.HW;
+  return c < p.c0 ? to_f32<T>(((const T*)p.x0)[row * p.c0 + c]) : to_f32<T>(((const T*)p.x1)[row * p.c1 + (c - p.c0)]);
+}
+
+// ---- one workgroup per (sample, group) ---------------------------------------------------------------
+__device__ __forceinline__ float block_sum(float v, float* red) {       // red: 16 floats; same value on every thread
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (unsigned w = 0; w < blockDim.x >> 6; ++w) t += red[w];
+  return t;
+}
+__device__ __forceinline__ void slice_of_block(const GnaParams& p, int& b, int& g) {
+  // neighbouring groups of a sample share 128-byte lines: a contiguous run of slices per XCD
+  const unsigned total = (unsigned)p.B * (unsigned)p.G, xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
+  const unsigned id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+  b = (int)(id / (unsigned)p.G); g = (int)(id - (unsigned)b * (unsigned)p.G);
+}
+
+template <typename T, int W>
+__global__ __launch_bounds__(1024) void gna_slice_fwd_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[16];
+  T* xs = reinterpret_cast<T*>(smem);
+  int b, g;
+  slice_of_block(p, b, g);
+  const int cbase = g * p.cpg, vpp = p.cpg / W, nv = (int)p.HW * vpp;
+  float s = 0.f;
+  for (int i = threadIdx.x; i < nv; i += blockDim.x) {
+    const int px = (int)div_by((unsigned)i, p.div_cpg), c = cbase + (i - px * vpp) * W;
+    const int64_t row = (int64_t)b * p.HW + px;
+    float v[W];
+    if (c < p.c0) load_n<T, W>((const T*)p.x0 + row * p.c0 + c, v);
+    else load_n<T, W>((const T*)p.x1 + row * p.c1 + (c - p.c0), v);
+    store_n<T, W>(xs + i * W, v);
+#pragma unroll
+    for (int e = 0; e < W; ++e) s += v[e];
+  }
+  const float inv_n = 1.f / ((float)p.HW * (float)p.cpg);
+  const float m0 = block_sum(s, red) * inv_n;
+  float q = 0.f, d = 0.f;
+  for (int i = threadIdx.x; i < nv; i += blockDim.x) {      // a thread reads back what it wrote
+    float v[W];
+    load_n<T, W>(xs + i * W, v);
+#pragma unroll
+    for (int e = 0; e < W; ++e) { const float t = v[e] - m0; d += t; q = fmaf(t, t, q); }
+  }
+  d = block_sum(d, red) * inv_n;                            // what the first sum's rounding left over
+  const float var = fmaxf(block_sum(q, red) * inv_n - d * d, 0.f);
+  const float mean = m0 + d, rstd = 1.f / sqrtf(var + p.eps);
+  if (threadIdx.x == 0) {
+    p.stats[((size_t)b * p.G + g) * 2] = mean;
+    p.stats[((size_t)b * p.G + g) * 2 + 1] = rstd;
+  }
+  unsigned k0 = 0, k1 = 0;
+  if (p.drop.thr) drop_key(p.drop, k0, k1);
+  for (int i = threadIdx.x; i < nv; i += blockDim.x) {
+    const int px = (int)div_by((unsigned)i, p.div_cpg), c = cbase + (i - px * vpp) * W;
+    const int64_t row = (int64_t)b * p.HW + px;
+    float v[W];
+    load_n<T, W>(xs + i * W, v);
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = act_f<T>(fmaf(v[e] - mean, rstd * p.gamma[c + e], p.beta[c + e]), p.act);
+    if (p.drop.thr) {
+      const Keep8 k = philox8(k0, k1, (unsigned)c >> 3, (uint64_t)row, p.drop.offset);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const int ce = (c + e) & 7;
+        const unsigned wd = ce < 4 ? (ce < 2 ? k.w[0] : k.w[1]) : (ce < 6 ? k.w[2] : k.w[3]);
+        v[e] = ((ce & 1) ? wd >> 16 : wd & 0xFFFFu) >= p.drop.thr ? v[e] * p.drop.scale : 0.f;
+      }
+    }
+    store_n<T, W>((T*)p.out0 + row * p.C + c, v);
+  }
+}
+
+// du of W columns from x and dy
+template <typename T, int W>
+__device__ __forceinline__ void grad_u(const GnaParams& p, unsigned k0, unsigned k1, int64_t row, int c, float mean, float rstd,
+                                       const float (&x)[W], const float (&dy)[W], float (&xh)[W], float (&du)[W]) {
+  unsigned num[W];
+  if (p.drop.thr) {
+    const Keep8 k = philox8(k0, k1, (unsigned)c >> 3, (uint64_t)row, p.drop.offset);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int ce = (c + e) & 7;
+      const unsigned wd = ce < 4 ? (ce < 2 ? k.w[0] : k.w[1]) : (ce < 6 ? k.w[2] : k.w[3]);
+      num[e] = (ce & 1) ? wd >> 16 : wd & 0xFFFFu;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    xh[e] = (x[e] - mean) * rstd;
+    float t = dy[e];
+    if (p.drop.thr) t = num[e] >= p.drop.thr ? t * p.drop.scale : 0.f;
+    du[e] = t * act_grad<T>(fmaf(xh[e], p.gamma[c + e], p.beta[c + e]), p.act);
+  }
+}
+
+// Backward of a slice: x and du in LDS.  Channel sums: a thread keeps one vector column (blockDim is a multiple of
+// the vectors per pixel, or the channels are walked one after the other), folded over the pixel lanes in LDS.
+template <typename T, int W>
+__global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float red[16];
+  int b, g;
+  slice_of_block(p, b, g);
+  const int cbase = g * p.cpg, vpp = p.cpg / W, nv = (int)p.HW * vpp;
+  float* dus = reinterpret_cast<float*>(smem);                     // [HW][cpg] fp32
+  T* xs = reinterpret_cast<T*>(smem + (size_t)p.HW * p.cpg * 4);   // [HW][cpg]
+  const float mean = p.stats[((size_t)b * p.G + g) * 2], rstd = p.stats[((size_t)b * p.G + g) * 2 + 1];
+  unsigned k0 = 0, k1 = 0;
+  if (p.drop.thr) drop_key(p.drop, k0, k1);
+  float a1 = 0.f, a2 = 0.f;
+  for (int i = threadIdx.x; i < nv; i += blockDim.x) {
+    const int px = (int)div_by((unsigned)i, p.div_cpg), c = cbase + (i - px * vpp) * W;
+    const int64_t row = (int64_t)b * p.HW + px;
+    float x[W], dy[W], xh[W], du[W];
+    if (c < p.c0) load_n<T, W>((const T*)p.x0 + row * p.c0 + c, x);
+    else load_n<T, W>((const T*)p.x1 + row * p.c1 + (c - p.c0), x);
+    load_n<T, W>((const T*)p.dy + row * p.C + c, dy);
+    grad_u<T, W>(p, k0, k1, row, c, mean, rstd, x, dy, xh, du);
+    store_n<T, W>(xs + i * W, x);
+    store_n<float, W>(dus + i * W, du);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const float h = du[e] * p.gamma[c + e];
+      a1 += h;
+      a2 = fmaf(h, xh[e], a2);
+    }
+  }
+  const float inv_n = 1.f / ((float)p.HW * (float)p.cpg);
+  a1 = block_sum(a1, red) * inv_n;
+  a2 = block_sum(a2, red) * inv_n;                                 // (its barriers also make xs and dus visible)
+  if (p.out0 || p.out1) {
+    for (int i = threadIdx.x; i < nv; i += blockDim.x) {
+      const int px = (int)div_by((unsigned)i, p.div_cpg), c = cbase + (i - px * vpp) * W;
+      const int64_t row = (int64_t)b * p.HW + px;
+      float x[W], du[W];
+      load_n<T, W>(xs + i * W, x);
+      load_n<float, W>(dus + i * W, du);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float xh = (x[e] - mean) * rstd;
+        x[e] = rstd * (du[e] * p.gamma[c + e] - a1 - xh * a2);
+      }
+      if (c < p.c0) { if (p.out0) store_n<T, W>((T*)p.out0 + row * p.c0 + c, x); }
+      else if (p.out1) store_n<T, W>((T*)p.out1 + row * p.c1 + (c - p.c0), x);
+    }
+  }
+  if (!p.dgamma && !p.dbeta) return;
+  // channel sums over the pixels: the block's threads as pl pixel lanes x channels, a lane's sums folded by shuffles
+  // where a group of lanes is whole, else through red: one wave per channel
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  for (int c = wave; c < p.cpg; c += nw) {
+    float s1 = 0.f, s2 = 0.f;
+    for (int px = lane; px < (int)p.HW; px += 64) {
+      const float du = dus[px * p.cpg + c];
+      s1 += du;
+      s2 = fmaf(du, (to_f32<T>(xs[px * p.cpg + c]) - mean) * rstd, s2);
+    }
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (lane == 0) {
+      if (p.B == 1) {
+        if (p.dbeta) p.dbeta[cbase + c] = s1;
+        if (p.dgamma) p.dgamma[cbase + c] = s2;
+      } else {
+        p.cpart[((size_t)b * 2) * p.C + cbase + c] = s1;
+        p.cpart[((size_t)b * 2 + 1) * p.C + cbase + c] = s2;
+      }
+    }
+  }
+}
+
+// ---- strips ------------------------------------------------------------------------------------------
+// A thread owns one group of eight columns and walks every lanes-th pixel of its strip; tensors of more than 2048
+// channels make a thread take several column groups, one after the other.
+struct Walk { int ncg, lanes, pl, cg0, cgs; int64_t pb, pe; };
+__device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip) {
+  Walk w;
+  w.ncg = (p.C + 7) >> 3;
+  const bool fits = w.ncg <= 256;
+  w.lanes = fits ? 256 / w.ncg : 1;
+  w.pl = fits ? (int)threadIdx.x / w.ncg : 0;
+  w.cg0 = fits ? (int)threadIdx.x - w.pl * w.ncg : (int)threadIdx.x;
+  w.cgs = 256;
+  if (w.pl >= w.lanes) w.cg0 = w.ncg;                    // threads left over
+  w.pb = (int64_t)strip * p.px_per_strip;
+  w.pe = w.pb + p.px_per_strip < p.HW ? w.pb + p.px_per_strip : p.HW;
+  return w;
+}
+// threads per group for folds over the groups: a power of two, at most a wave
+__device__ __forceinline__ int threads_per_group(int G) {
+  int t = 64;
+  while (t > 1 && t * G > 256) t >>= 1;
+  return t;
+}
+template <typename F> __device__ __forceinline__ F fold_lanes(F v, int tpg) {
+  for (int o = tpg >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// the strip's channel sums in LDS ([lanes][ncg * 8], two arrays) -> lane 0's row holds the totals
+__device__ __forceinline__ void fold_pixel_lanes(float* s1, float* s2, int lanes, int width) {
+  __syncthreads();
+  for (int c = threadIdx.x; c < width; c += 256) {
+    float a = s1[c], q = s2[c];
+    for (int l = 1; l < lanes; ++l) { a += s1[l * width + c]; q += s2[l * width + c]; }
+    s1[c] = a; s2[c] = q;
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  const int strip = blockIdx.x, b = blockIdx.y;
+  const Walk w = walk_of(p, strip);
+  const int width = w.ncg * 8;
+  float* s1 = reinterpret_cast<float*>(smem);
+  float* s2 = s1 + w.lanes * width;
+  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+    const int c = cg * 8;
+    float sh[8], s[8], q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e < p.C ? c + e : p.C - 1;
+      sh[e] = first_of<T>(p, b, (int)div_by((unsigned)ce, p.div_cpg) * p.cpg);
+      s[e] = 0.f; q[e] = 0.f;
+    }
+    int64_t px = w.pb + w.pl;
+    for (; px + 3 * w.lanes < w.pe; px += 4 * w.lanes) {       // four independent loads in flight
+      float v[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px + u * w.lanes, c, v[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { const float t = v[u][e] - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
+    }
+    for (; px < w.pe; px += w.lanes) {
+      float v[8];
+      load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px, c, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { const float t = v[e] - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
+  }
+  fold_pixel_lanes(s1, s2, w.lanes, width);
+  const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
+  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {                // every lane goes round equally often (shuffles)
+    const int g = g0 + (int)threadIdx.x / tpg;
+    float a = 0.f, q = 0.f;
+    if (g < p.G)
+      for (int c = j; c < p.cpg; c += tpg) { a += s1[g * p.cpg + c]; q += s2[g * p.cpg + c]; }
+    a = fold_lanes(a, tpg);
+    q = fold_lanes(q, tpg);
+    if (g < p.G && j == 0) {
+      float* dst = p.part + (((size_t)b * p.strips + strip) * p.G + g) * 2;
+      dst[0] = a; dst[1] = q;
+    }
+  }
+}
+
+// sums over the strips of sample b, per group, in double: fin(g, first sum, second sum) on one thread per group
+template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaParams& p, int b, Fn fin) {
+  const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
+  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {
+    const int g = g0 + (int)threadIdx.x / tpg;
+    double a = 0.0, q = 0.0;
+    if (g < p.G) {
+      const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.strips * p.G + g;
+      for (int s = j; s < p.strips; s += tpg) { const float2 v = src[(size_t)s * p.G]; a += (double)v.x; q += (double)v.y; }
+    }
+    a = fold_lanes(a, tpg);
+    q = fold_lanes(q, tpg);
+    if (g < p.G && j == 0) fin(g, a, q);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gna_apply_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  float* s_mean = reinterpret_cast<float*>(smem);
+  float* s_rstd = s_mean + p.G;
+  const int strip = blockIdx.x, b = blockIdx.y;
+  fold_strips(p, b, [&](int g, double a, double q) {
+    const double n = (double)p.HW * (double)p.cpg, m = a / n;
+    double var = q / n - m * m;
+    if (var < 0.0) var = 0.0;
+    const float mean = (float)((double)first_of<T>(p, b, g * p.cpg) + m), rstd = (float)(1.0 / sqrt(var + (double)p.eps));
+    s_mean[g] = mean; s_rstd[g] = rstd;
+    if (strip == 0) {
+      p.stats[((size_t)b * p.G + g) * 2] = mean;
+      p.stats[((size_t)b * p.G + g) * 2 + 1] = rstd;
+    }
+  });
+  __syncthreads();
+  const Walk w = walk_of(p, strip);
+  unsigned k0 = 0, k1 = 0;
+  if (p.drop.thr) drop_key(p.drop, k0, k1);
+  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+    const int c = cg * 8;
+    float mn[8], sc[8], bt[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
+      mn[e] = s_mean[g]; sc[e] = s_rstd[g] * p.gamma[ce]; bt[e] = p.beta[ce];
+    }
+    auto put = [&](int64_t row, float (&v)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = act_f<T>(fmaf(v[e] - mn[e], sc[e], bt[e]), p.act);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+      store8<T>((T*)p.out0 + row * p.C + c, p.C - c, v);
+    };
+    int64_t px = w.pb + w.pl;
+    for (; px + 3 * w.lanes < w.pe; px += 4 * w.lanes) {
+      float v[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px + u * w.lanes, c, v[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) put((int64_t)b * p.HW + px + u * w.lanes, v[u]);
+    }
+    for (; px < w.pe; px += w.lanes) {
+      float v[8];
+      load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px, c, v);
+      put((int64_t)b * p.HW + px, v);
+    }
+  }
+}
+
+// backward, first launch: channel sums of du and du xh over the strip, and the group sums of gamma times them
+template <typename T>
+__global__ __launch_bounds__(256) void gna_grad_sums_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  const int strip = blockIdx.x, b = blockIdx.y;
+  const Walk w = walk_of(p, strip);
+  const int width = w.ncg * 8;
+  float* s1 = reinterpret_cast<float*>(smem);
+  float* s2 = s1 + w.lanes * width;
+  unsigned k0 = 0, k1 = 0;
+  if (p.drop.thr) drop_key(p.drop, k0, k1);
+  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+    const int c = cg * 8;
+    float mn[8], rs[8], ga[8], bt[8], s[8], q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
+      const float* st = p.stats + ((size_t)b * p.G + g) * 2;
+      mn[e] = st[0]; rs[e] = st[1]; ga[e] = p.gamma[ce]; bt[e] = p.beta[ce];
+      s[e] = 0.f; q[e] = 0.f;
+    }
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += w.lanes) {
+      const int64_t row = (int64_t)b * p.HW + px;
+      float x[8], v[8];
+      load_cols<T>(p.x0, p.x1, p.c0, p.c1, row, c, x);
+      load8<T>((const T*)p.dy + row * p.C + c, p.C - c, v);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xh = (x[e] - mn[e]) * rs[e];
+        const float du = v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
+        s[e] += du;
+        q[e] = fmaf(du, xh, q[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
+  }
+  fold_pixel_lanes(s1, s2, w.lanes, width);
+  if (p.dgamma || p.dbeta) {
+    float* cp = p.cpart + ((size_t)b * p.strips + strip) * 2 * p.C;
+    for (int c = threadIdx.x; c < p.C; c += 256) { cp[c] = s1[c]; cp[p.C + c] = s2[c]; }
+  }
+  const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
+  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {
+    const int g = g0 + (int)threadIdx.x / tpg;
+    float a = 0.f, q = 0.f;
+    if (g < p.G)
+      for (int c = j; c < p.cpg; c += tpg) {
+        const float ga = p.gamma[g * p.cpg + c];
+        a = fmaf(ga, s1[g * p.cpg + c], a);
+        q = fmaf(ga, s2[g * p.cpg + c], q);
+      }
+    a = fold_lanes(a, tpg);
+    q = fold_lanes(q, tpg);
+    if (g < p.G && j == 0) {
+      float* dst = p.part + (((size_t)b * p.strips + strip) * p.G + g) * 2;
+      dst[0] = a; dst[1] = q;
+    }
+  }
+}
+
+// dgamma / dbeta: sum of `rows` rows [2][C] of channel sums; a block takes 16 channels x 16 row lanes
+__device__ __forceinline__ void fold_channels(const GnaParams& p, int block, int64_t rows, float* red) {
+  const int cl = threadIdx.x & 15, rl = (threadIdx.x >> 4) & 15, c = block * 16 + cl;
+  float a = 0.f, q = 0.f;
+  if (threadIdx.x < 256 && c < p.C)
+    for (int64_t r = rl; r < rows; r += 16) { a += p.cpart[r * 2 * p.C + c]; q += p.cpart[r * 2 * p.C + p.C + c]; }
+  if (threadIdx.x < 256) { red[rl * 16 + cl] = a; red[256 + rl * 16 + cl] = q; }
+  __syncthreads();
+  if (threadIdx.x < 16 && c < p.C) {
+    a = 0.f; q = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { a += red[r * 16 + cl]; q += red[256 + r * 16 + cl]; }
+    if (p.dbeta) p.dbeta[c] = a;
+    if (p.dgamma) p.dgamma[c] = q;
+  }
+}
+__global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int64_t rows) {
+  __shared__ float red[512];
+  fold_channels(p, (int)blockIdx.x, rows, red);
+}
+
+// backward, second launch: dx; the blocks behind the strips' fold dgamma and dbeta
+template <typename T>
+__global__ __launch_bounds__(256) void gna_grad_apply_kernel(GnaParams p) {
+  extern __shared__ __align__(16) char smem[];
+  if ((int)blockIdx.x >= p.apply_blocks) {
+    if (blockIdx.y == 0)
+      fold_channels(p, (int)blockIdx.x - p.apply_blocks, (int64_t)p.B * p.strips, reinterpret_cast<float*>(smem));
+    return;
+  }
+  float* s_a = reinterpret_cast<float*>(smem);
+  float* s_q = s_a + p.G;
+  const int strip = blockIdx.x, b = blockIdx.y;
+  fold_strips(p, b, [&](int g, double a, double q) {
+    const double n = (double)p.HW * (double)p.cpg;
+    s_a[g] = (float)(a / n); s_q[g] = (float)(q / n);
+  });
+  __syncthreads();
+  const Walk w = walk_of(p, strip);
+  unsigned k0 = 0, k1 = 0;
+  if (p.drop.thr) drop_key(p.drop, k0, k1);
+  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+    const int c = cg * 8;
+    float mn[8], rs[8], ga[8], bt[8], ma[8], mq[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
+      const float* st = p.stats + ((size_t)b * p.G + g) * 2;
+      mn[e] = st[0]; rs[e] = st[1]; ga[e] = p.gamma[ce]; bt[e] = p.beta[ce];
+      ma[e] = s_a[g]; mq[e] = s_q[g];
+    }
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += w.lanes) {
+      const int64_t row = (int64_t)b * p.HW + px;
+      float x[8], v[8];
+      load_cols<T>(p.x0, p.x1, p.c0, p.c1, row, c, x);
+      load8<T>((const T*)p.dy + row * p.C + c, p.C - c, v);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float xh = (x[e] - mn[e]) * rs[e];
+        const float h = ga[e] * v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
+        x[e] = rs[e] * (h - ma[e] - xh * mq[e]);
+      }
+      store_cols<T>(p.out0, p.out1, p.c0, p.c1, row, c, x);
+    }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------
+struct GnaPlan {
+  int slice;                    // 1: one workgroup per (sample, group)
+  int w;                        // ... columns per access
+  int lds;
+  int strips; int64_t px_per_strip;
+  size_t part, cpart, total;    // workspace offsets
+};
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backward) {
+  GnaPlan pl = {};
+  const int C = c0 + c1, cpg = C / G;
+  const size_t esz = sdmi_dtype_size(dtype);
+  const size_t per = backward ? esz + 4 : esz;
+  pl.w = 1;
+  for (int w = 8; w > 1; w >>= 1)
+    if (cpg % w == 0 && c0 % w == 0) { pl.w = w; break; }
+  if (HW <= (1 << 20) && (size_t)HW * cpg * per <= 60 * 1024) {
+    pl.slice = 1;
+    pl.lds = (int)((size_t)HW * cpg * per);
+    pl.cpart = 0;
+    pl.total = backward && B > 1 ? up256((size_t)B * 2 * C * 4) : 0;
+    return pl;
+  }
+  const int ncg = (C + 7) / 8, lanes = ncg <= 256 ? 256 / ncg : 1;
+  // about four workgroups per CU, every pixel lane at least four pixels, and no more strips than a fold likes to read
+  int64_t strips = (1024 + B - 1) / B;
+  const int64_t by_work = (HW + 4 * lanes - 1) / (4 * lanes);
+  if (strips > by_work) strips = by_work;
+  if (strips > 256) strips = 256;
+  if (strips < 1) strips = 1;
+  pl.px_per_strip = (HW + strips - 1) / strips;
+  pl.strips = (int)((HW + pl.px_per_strip - 1) / pl.px_per_strip);
+  pl.lds = 2 * lanes * ncg * 8 * 4;
+  pl.part = 0;
+  pl.cpart = up256((size_t)B * pl.strips * G * 2 * 4);
+  pl.total = pl.cpart + (backward ? up256((size_t)B * pl.strips * 2 * C * 4) : 0);
+  return pl;
+}
+
+int gna_check(const GroupNormActArgs& a, const char* who) {
+  SDMI_REQUIRE(a.dtype >= 0 && a.dtype <= 2, "%s: bad dtype %d", who, a.dtype);
+  SDMI_REQUIRE(a.B >= 0 && a.HW >= 0 && a.c0 > 0 && a.c1 >= 0, "%s: bad size", who);
+  const int64_t C = (int64_t)a.c0 + a.c1;
+  SDMI_REQUIRE(C <= GNA_MAX_C, "%s: %lld channels, at most %d are supported", who, (long long)C, GNA_MAX_C);
+  SDMI_REQUIRE(a.groups > 0 && C % a.groups == 0, "%s: %lld channels do not split into %d groups", who, (long long)C, a.groups);
+  SDMI_REQUIRE(a.eps >= 0.f, "%s: negative eps", who);
+  SDMI_REQUIRE(a.act >= 0 && a.act < ACT_COUNT, "%s: unknown activation %d", who, a.act);
+  SDMI_REQUIRE(a.B <= 65535, "%s: batch %d is beyond 65535", who, a.B);
+  return SDMI_OK;
+}
+
+GnaParams gna_params(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop) {
+  GnaParams p = {};
+  p.x0 = a.x0; p.x1 = a.c1 ? a.x1 : nullptr; p.dy = a.dy;
+  p.c0 = a.c0; p.c1 = a.c1; p.C = a.c0 + a.c1; p.G = a.groups; p.cpg = p.C / a.groups; p.B = a.B; p.HW = a.HW;
+  p.div_cpg = fast_div((unsigned)(pl.slice ? p.cpg / pl.w : p.cpg));
+  p.eps = a.eps; p.gamma = a.gamma; p.beta = a.beta; p.act = a.act; p.drop = drop; p.stats = a.stats;
+  p.strips = pl.strips; p.px_per_strip = pl.px_per_strip;
+  p.part = (float*)((char*)a.workspace + pl.part); p.cpart = (float*)((char*)a.workspace + pl.cpart);
+  p.dgamma = a.dgamma; p.dbeta = a.dbeta;
+  return p;
+}
+
+int slice_threads(const GnaPlan& pl, const GnaParams& p) {
+  const int64_t nv = p.HW * (p.cpg / pl.w);
+  int t = 64;
+  while (t < 1024 && t * 2 < nv) t <<= 1;
+  return t;
+}
+
+template <typename T>
+int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
+  GnaParams p = gna_params(a, pl, drop);
+  p.out0 = a.out;
+  char label[64];
+  snprintf(label, sizeof(label), "gn_act B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
+  ProfScope prof(PROF_GROUPNORM, s, 0.0, 2.0 * p.B * (double)p.HW * p.C * sizeof(T), label);
+  if (pl.slice) {
+    const dim3 grid((unsigned)p.B * (unsigned)p.G), block(slice_threads(pl, p));
+    if (pl.w == 8) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 8>), grid, block, pl.lds, s, p);
+    else if (pl.w == 4) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 4>), grid, block, pl.lds, s, p);
+    else if (pl.w == 2) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 2>), grid, block, pl.lds, s, p);
+    else hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 1>), grid, block, pl.lds, s, p);
+  } else {
+    const dim3 grid(pl.strips, p.B);
+    hipLaunchKernelGGL(gna_stats_kernel<T>, grid, dim3(256), pl.lds, s, p);
+    hipLaunchKernelGGL(gna_apply_kernel<T>, grid, dim3(256), 2 * p.G * 4, s, p);
+  }
+  SDMI_CHECK_HIP(hipGetLastError());
+  return SDMI_OK;
+}
+
+template <typename T>
+int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
+  GnaParams p = gna_params(a, pl, drop);
+  p.out0 = a.dx0; p.out1 = a.dx1;
+  char label[64];
+  snprintf(label, sizeof(label), "gn_act bwd B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
+  ProfScope prof(PROF_GROUPNORM, s, 0.0, 3.0 * p.B * (double)p.HW * p.C * sizeof(T), label);
+  const bool weights = p.dgamma || p.dbeta;
+  const unsigned fold_blocks = weights ? (unsigned)(p.C + 15) / 16 : 0;
+  if (pl.slice) {
+    const dim3 grid((unsigned)p.B * (unsigned)p.G), block(slice_threads(pl, p));
+    if (pl.w == 8) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 8>), grid, block, pl.lds, s, p);
+    else if (pl.w == 4) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 4>), grid, block, pl.lds, s, p);
+    else if (pl.w == 2) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 2>), grid, block, pl.lds, s, p);
+    else hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 1>), grid, block, pl.lds, s, p);
+    if (weights && p.B > 1) hipLaunchKernelGGL(gna_fold_channels_kernel, dim3(fold_blocks), dim3(256), 0, s, p, (int64_t)p.B);
+  } else {
+    hipLaunchKernelGGL(gna_grad_sums_kernel<T>, dim3(pl.strips, p.B), dim3(256), pl.lds, s, p);
+    p.apply_blocks = (a.dx0 || a.dx1) ? pl.strips : 0;
+    const int lds = 2 * p.G * 4 > 2048 ? 2 * p.G * 4 : 2048;
+    if (p.apply_blocks + fold_blocks)
+      hipLaunchKernelGGL(gna_grad_apply_kernel<T>, dim3(p.apply_blocks + fold_blocks, p.B), dim3(256), lds, s, p);
+  }
+  SDMI_CHECK_HIP(hipGetLastError());
+  return SDMI_OK;
+}
+
+}  // namespace
+
+int64_t groupnorm_act_workspace_bytes(int batch, int64_t hw, int c0, int c1, int groups, int dtype, int backward) {
+  if (batch <= 0 || hw <= 0 || c0 <= 0 || c1 < 0 || groups <= 0 || (c0 + c1) % groups) return 0;
+  return (int64_t)gna_plan(batch, hw, c0, c1, groups, dtype, backward).total;
+}
+
+int groupnorm_act(const GroupNormActArgs& a, hipStream_t stream) {
+  SDMI_TRY(gna_check(a, "groupnorm_act"));
+  DropArgs drop;
+  SDMI_TRY(drop_args(&drop, a.p, a.seed, a.seed_dev, a.offset, "groupnorm_act"));
+  if (a.B == 0 || a.HW == 0) return SDMI_OK;
+  SDMI_REQUIRE(a.x0 && (a.x1 || !a.c1) && a.gamma && a.beta && a.out && a.stats, "groupnorm_act: null pointer");
+  const GnaPlan pl = gna_plan(a.B, a.HW, a.c0, a.c1, a.groups, a.dtype, 0);
+  SDMI_REQUIRE(pl.total == 0 || a.workspace, "groupnorm_act: this size needs a workspace of %lld bytes", (long long)pl.total);
+  SDMI_DISPATCH_DTYPE(a.dtype, T, return gna_fwd<T>(a, pl, drop, stream));
+  return SDMI_OK;
+}
+
+int groupnorm_act_backward(const GroupNormActArgs& a, hipStream_t stream) {
+  SDMI_TRY(gna_check(a, "groupnorm_act_backward"));
+  DropArgs drop;
+  SDMI_TRY(drop_args(&drop, a.p, a.seed, a.seed_dev, a.offset, "groupnorm_act_backward"));
+  if (!a.dx0 && !a.dx1 && !a.dgamma && !a.dbeta) return SDMI_OK;
+  if (a.B == 0 || a.HW == 0) {
+    GnaPlan pl = {};
+    GnaParams p = gna_params(a, pl, drop);
+    if (p.dgamma || p.dbeta) {
+      hipLaunchKernelGGL(gna_fold_channels_kernel, dim3((p.C + 15) / 16), dim3(256), 0, stream, p, (int64_t)0);
+      SDMI_CHECK_HIP(hipGetLastError());
+    }
+    return SDMI_OK;
+  }
+  SDMI_REQUIRE(a.dy && a.x0 && (a.x1 || !a.c1) && a.gamma && a.beta && a.stats, "groupnorm_act_backward: null pointer");
+  SDMI_REQUIRE(!a.c1 || (a.dx0 != nullptr) == (a.dx1 != nullptr), "groupnorm_act_backward: dx of both sources or of neither");
+  const GnaPlan pl = gna_plan(a.B, a.HW, a.c0, a.c1, a.groups, a.dtype, 1);
+  SDMI_REQUIRE(pl.total == 0 || a.workspace, "groupnorm_act_backward: this size needs a workspace of %lld bytes",
+               (long long)pl.total);
+  SDMI_DISPATCH_DTYPE(a.dtype, T, return gna_bwd<T>(a, pl, drop, stream));
+  return SDMI_OK;
+}

@@ -127,6 +127,58 @@ int attention(const AttentionArgs& a, hipStream_t stream);
 int attention_init();   // one-time kernel attribute setup; call outside stream capture
 int elementwise_init(); // same, for the first-convolution kernel
 
+// ---- layers with gradients: counter-based dropout, linear with epilogue -----------------------------
+struct DropoutArgs {
+  const void* x = nullptr; int64_t ldx = 0;      // [rows][ldx]
+  const void* resid = nullptr; int64_t ldr = 0;  // optional, added behind the dropout
+  void* out = nullptr;                           // [rows][cols]
+  int64_t rows = 0; int cols = 0;
+  double p = 0.0;
+  int64_t seed = 0; const int64_t* seed_dev = nullptr; int64_t offset = 0;
+  int dtype = SDMI_F16;
+};
+int dropout(const DropoutArgs& a, hipStream_t stream);
+
+struct LinearActArgs {
+  int64_t rows = 0; int k = 0, n = 0;
+  const void* x = nullptr; int64_t ldx = 0;      // [rows][ldx]
+  const void* w = nullptr; int64_t ldw = 0;      // [n][ldw]
+  const float* bias = nullptr;
+  const void* resid = nullptr; int64_t ldr = 0;
+  void* out = nullptr;                           // [rows][n]
+  float* preact = nullptr;                       // [rows][n]: written forward (optional), read backward
+  int act = 0;
+  double p = 0.0;
+  int64_t seed = 0; const int64_t* seed_dev = nullptr; int64_t offset = 0;
+  const void* dy = nullptr; int64_t lddy = 0;    // backward
+  void* dx = nullptr; void* dw = nullptr; float* db = nullptr;
+  void* workspace = nullptr;
+  int dtype = SDMI_F16;
+};
+int linear_act(const LinearActArgs& a, hipStream_t stream);
+int linear_act_backward(const LinearActArgs& a, hipStream_t stream);
+int64_t linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype);
+int64_t linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype);
+
+struct GroupNormActArgs {
+  const void* x0 = nullptr; const void* x1 = nullptr; int c0 = 0, c1 = 0;   // NHWC [B][HW][c0] (| [B][HW][c1])
+  int B = 0; int64_t HW = 0; int groups = 32;
+  float eps = 1e-5f;
+  const float* gamma = nullptr; const float* beta = nullptr;
+  int act = 0;
+  double p = 0.0;
+  int64_t seed = 0; const int64_t* seed_dev = nullptr; int64_t offset = 0;
+  void* out = nullptr;                           // forward
+  float* stats = nullptr;                        // [B][groups][2] (mean, rstd): written forward, read backward
+  const void* dy = nullptr;                      // backward
+  void* dx0 = nullptr; void* dx1 = nullptr; float* dgamma = nullptr; float* dbeta = nullptr;
+  void* workspace = nullptr;
+  int dtype = SDMI_F16;
+};
+int groupnorm_act(const GroupNormActArgs& a, hipStream_t stream);
+int groupnorm_act_backward(const GroupNormActArgs& a, hipStream_t stream);
+int64_t groupnorm_act_workspace_bytes(int batch, int64_t hw, int c0, int c1, int groups, int dtype, int backward);
+
 // ---- small / elementwise ---------------------------------------------------------------------
 // emb[b][:] = [cos(t*f) | sin(t*f)], f_k = exp(-ln(max_period) k / half)            (fp32 out)
 int timestep_embedding(const int64_t* t, float* out, int B, int dim, float max_period, hipStream_t s);

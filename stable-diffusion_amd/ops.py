@@ -285,3 +285,281 @@ def inpaint_composite(image, mask, predicted):
     check(_lib.lib().sdmi_inpaint_composite(ptr(image), ptr(mask), ptr(predicted), ptr(out), b, c, h * w, stream_ptr()),
           "inpaint_composite")
     return out
+
+
+# ---- layers with dropout and gradients -----------------------------------------------------------------------
+# dropout, linear_act and groupnorm_act are differentiable (torch.autograd, first derivatives).  They take tensors of
+# any device, launch on that device's current stream and allocate with torch, so they can be captured into a graph;
+# there a `seed` in device memory makes every replay draw anew.  Capture a backward pass together with its forward
+# pass, and with no eager graph of the same leaves alive (torch joins the streams of a leaf's graphs).
+
+_ACTS = {None: 0, "silu": 1, "gelu": 2, "quick_gelu": 3}
+
+
+def _act_code(act):
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}: one of {list(_ACTS)}")
+    return _ACTS[act]
+
+
+def _run(device, name, *args):
+    """One call of the library on ``device``'s current stream."""
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _check_like(what, t, device, dtype, shape=None):
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _check_input(what, x):
+    if not x.is_cuda:
+        raise ValueError(f"{what} is on {x.device}: there is no CPU path")
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"{what} is {x.dtype}, expected float32, float16 or bfloat16")
+
+
+def _drop_state(p, seed, offset, device):
+    """(p, host seed, seed tensor or None, offset), checked."""
+    p, offset = float(p), int(offset)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability {p} is not in [0, 1]")
+    if not 0 <= offset < 1 << 32:
+        raise ValueError(f"dropout offset {offset} does not fit 32 bits")
+    if p == 0.0:
+        return 0.0, 0, None, 0
+    if seed is None:
+        raise ValueError("dropout needs a seed")
+    if torch.is_tensor(seed):
+        _check_like("seed", seed, device, torch.int64)
+        if seed.numel() != 1:
+            raise ValueError(f"seed holds {seed.numel()} numbers, expected one")
+        return p, 0, seed, offset
+    seed = int(seed)
+    if not -(1 << 63) <= seed < 1 << 64:
+        raise ValueError(f"seed {seed} does not fit 64 bits")
+    return p, seed, None, offset
+
+
+def _rows(t, cols):
+    """``t`` as (rows, cols) with unit column stride (a view where the strides allow it), and its row stride."""
+    rows = 1
+    for s in t.shape[:-1]:
+        rows *= s
+    if rows == 0 or cols == 0:
+        return t, cols, rows
+    t = t.reshape(rows, cols)
+    if cols > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else cols), rows
+
+
+def _dropout(x, resid, p, seed, seed_t, offset):
+    cols = x.shape[-1] if x.dim() else 1
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x2, ldx, rows = _rows(x, cols)
+    r2, ldr = (None, 0) if resid is None else _rows(resid, cols)[:2]
+    _run(x.device, "sdmi_dropout", _p(x2), ldx, _p(r2), ldr, _p(out), rows, cols, p, seed, _p(seed_t), offset,
+         dtype_code(x.dtype))
+    return out
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, resid, seed_t, p, seed, offset):
+        ctx.save_for_backward(seed_t)
+        ctx.drop = (p, seed, offset)
+        return _dropout(x, resid, p, seed, seed_t, offset)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        p, seed, offset = ctx.drop
+        seed_t, = ctx.saved_tensors
+        dx = _dropout(dy, None, p, seed, seed_t, offset) if ctx.needs_input_grad[0] else None
+        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None, None
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def dropout(x, p, seed, offset=0, resid=None):
+    """Dropout with a counter-based mask that is never stored: ``[resid +] keep * x / (1 - p)``, differentiable.
+
+    Which elements of a row are kept is a function of (seed, offset, row, column) alone, where the last dimension is
+    the columns and all others number the rows, so that ``linear_act`` and ``groupnorm_act`` with the same seed and
+    offset drop the same elements.  ``seed``: an integer of 64 bits, or a one-element int64 tensor on ``x``'s device
+    (read when the kernel runs); ``offset``: one number per layer or call, below 2^32.  ``p`` counts in steps of
+    2^-16, and the scale is that of the probability used.  Dropped elements are 0 whatever they held."""
+    _check_input("x", x)
+    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
+    if resid is not None:
+        _check_like("resid", resid, x.device, x.dtype, x.shape)
+    if _wants_grad(x, resid):
+        return _DropoutFn.apply(x, resid, seed_t, p, seed, offset)
+    return _dropout(x, resid, p, seed, seed_t, offset)
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, want_preact):
+    n, k = w.shape
+    dt = dtype_code(x.dtype)
+    out = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    x2, ldx, rows = _rows(x, k)
+    w2, ldw, _ = _rows(w, k)
+    r2, ldr = (None, 0) if resid is None else _rows(resid, n)[:2]
+    preact = torch.empty((rows, n), dtype=torch.float32, device=x.device) if want_preact else None
+    ws = _workspace(_lib.lib().sdmi_linear_act_workspace_bytes(rows, k, n, dt), x.device)
+    _run(x.device, "sdmi_linear_act", _p(x2), ldx, _p(w2), ldw, _p(bias), _p(r2), ldr, _p(out), _p(preact), rows, k, n,
+         act, p, seed, _p(seed_t), offset, _p(ws), dt)
+    return out, preact
+
+
+class _LinearActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, resid, seed_t, act, p, seed, offset):
+        need = ctx.needs_input_grad
+        product = need[0] or need[1] or need[2]
+        out, preact = _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, act != 0 and product)
+        ctx.save_for_backward(x if need[1] else None, w if need[0] else None, preact, seed_t)
+        ctx.drop = (p, seed, offset)
+        ctx.act, ctx.kn, ctx.xshape = act, (w.shape[1], w.shape[0]), x.shape
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, preact, seed_t = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        k, n = ctx.kn
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            p, seed, offset = ctx.drop
+            dev, dt = dy.device, dtype_code(dy.dtype)
+            d2, ldd, rows = _rows(dy, n)
+            x2, ldx = (None, 0) if x is None else _rows(x, k)[:2]
+            w2, ldw = (None, 0) if w is None else _rows(w, k)[:2]
+            if need_x:
+                dx = torch.empty(ctx.xshape, dtype=dy.dtype, device=dev)
+            if need_w:
+                dw = torch.empty((n, k), dtype=dy.dtype, device=dev)
+            if need_b:
+                db = torch.empty((n,), dtype=torch.float32, device=dev)
+            want = (1 if need_x else 0) | (2 if need_w else 0) | (4 if need_b else 0)
+            ws = _workspace(_lib.lib().sdmi_linear_act_backward_workspace_bytes(rows, k, n, ctx.act, p, want, dt), dev)
+            _run(dev, "sdmi_linear_act_backward", _p(d2), ldd, _p(preact), _p(x2), ldx, _p(w2), ldw, _p(dx), _p(dw),
+                 _p(db), rows, k, n, ctx.act, p, seed, _p(seed_t), offset, _p(ws), dt)
+        return dx, dw, db, (dy if need_r else None), None, None, None, None, None
+
+
+def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0):
+    """``[resid +] dropout(act(x w^T + bias))``, differentiable in x, w, bias and resid.
+
+    x (..., K), w (N, K) and resid (..., N) in one dtype (fp32, fp16, bf16), bias fp32 (N,).  act: None, "silu",
+    "gelu" (erf) or "quick_gelu" (z sigmoid(1.702 z)); p, seed, offset as in ``dropout``.  With an activation a
+    training call keeps x w^T + bias in fp32.  Any sizes from one on; rows of whole 16-byte pieces are fastest."""
+    _check_input("x", x)
+    act = _act_code(act)
+    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or 0 in w.shape:
+        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (..., K) and (N, K)")
+    _check_like("w", w, x.device, x.dtype)
+    n = w.shape[0]
+    if bias is not None:
+        _check_like("bias", bias, x.device, torch.float32, (n,))
+        bias = bias.contiguous()
+    if resid is not None:
+        _check_like("resid", resid, x.device, x.dtype, tuple(x.shape[:-1]) + (n,))
+    if _wants_grad(x, w, bias, resid):
+        return _LinearActFn.apply(x, w, bias, resid, seed_t, act, p, seed, offset)
+    return _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, False)[0]
+
+
+def _gn_sizes(x, x1):
+    b, hw = x.shape[0], 1
+    for s in x.shape[1:-1]:
+        hw *= s
+    return b, hw, x.shape[-1], 0 if x1 is None else x1.shape[-1]
+
+
+def _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset):
+    b, hw, c0, c1 = _gn_sizes(x, x1)
+    dt = dtype_code(x.dtype)
+    out = torch.empty(x.shape[:-1] + (c0 + c1,), dtype=x.dtype, device=x.device)
+    stats = torch.empty((b, groups, 2), dtype=torch.float32, device=x.device)
+    ws = _workspace(_lib.lib().sdmi_groupnorm_act_workspace_bytes(b, hw, c0, c1, groups, dt, 0), x.device)
+    _run(x.device, "sdmi_groupnorm_act", _p(x), c0, _p(x1), c1, b, hw, groups, eps, _p(gamma), _p(beta), act, p, seed,
+         _p(seed_t), offset, _p(out), _p(stats), _p(ws), dt)
+    return out, stats
+
+
+class _GroupNormActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, x1, gamma, beta, seed_t, eps, act, groups, p, seed, offset):
+        out, stats = _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset)
+        ctx.save_for_backward(x, x1, gamma, beta, stats, seed_t)
+        ctx.args = (act, groups, p, seed, offset)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, x1, gamma, beta, stats, seed_t = ctx.saved_tensors
+        act, groups, p, seed, offset = ctx.args
+        b, hw, c0, c1 = _gn_sizes(x, x1)
+        dt = dtype_code(x.dtype)
+        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        dy = dy.contiguous()
+        dx = torch.empty_like(x) if need_x else None
+        dx1 = torch.empty_like(x1) if need_x and x1 is not None else None
+        dgamma = torch.empty_like(gamma) if ctx.needs_input_grad[2] else None
+        dbeta = torch.empty_like(beta) if ctx.needs_input_grad[3] else None
+        ws = _workspace(_lib.lib().sdmi_groupnorm_act_workspace_bytes(b, hw, c0, c1, groups, dt, 1), x.device)
+        _run(x.device, "sdmi_groupnorm_act_backward", _p(dy), _p(x), c0, _p(x1), c1, b, hw, groups, _p(gamma), _p(beta),
+             _p(stats), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1), _p(dgamma), _p(dbeta), _p(ws), dt)
+        return (dx if ctx.needs_input_grad[0] else None, dx1 if ctx.needs_input_grad[1] else None, dgamma, dbeta,
+                None, None, None, None, None, None, None)
+
+
+def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.0, seed=None, offset=0):
+    """``dropout(act(GroupNorm([x | x1])))`` channels last, differentiable in x, x1, gamma and beta.
+
+    x (B, ..., C0) [and x1 (B, ..., C1), concatenated behind it] -> (B, ..., C0 + C1); gamma, beta fp32 (C0 + C1,).
+    act as in ``linear_act``, p / seed / offset as in ``dropout`` (a pixel is a row).  Any number of channels per
+    group (8192 channels in all at most) and any image size; ``groupnorm`` is the inference path's own kernel."""
+    _check_input("x", x)
+    act = _act_code(act)
+    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
+    if x.dim() < 2:
+        raise ValueError(f"x {tuple(x.shape)} has no batch and channel dimension")
+    c = x.shape[-1]
+    if x1 is not None:
+        _check_like("x1", x1, x.device, x.dtype, tuple(x.shape[:-1]) + (x1.shape[-1] if x1.dim() else 0,))
+        c += x1.shape[-1]
+        x1 = x1.contiguous() if x1.shape[-1] else None
+    groups = int(groups)
+    if c == 0 or x.shape[-1] == 0 or groups < 1 or c % groups:
+        raise ValueError(f"{c} channels do not split into {groups} groups")
+    _check_like("gamma", gamma, x.device, torch.float32, (c,))
+    _check_like("beta", beta, x.device, torch.float32, (c,))
+    x, gamma, beta, eps = x.contiguous(), gamma.contiguous(), beta.contiguous(), float(eps)
+    if _wants_grad(x, x1, gamma, beta):
+        return _GroupNormActFn.apply(x, x1, gamma, beta, seed_t, eps, act, groups, p, seed, offset)
+    return _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset)[0]

@@ -1,0 +1,126 @@
+"""CPU: the generator of the dropout mask against its published vectors, and the refusals of the layers with dropout
+and gradients (library and Python), none of which reaches a GPU."""
+import ctypes
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+import _layers_ref as R
+
+_lib = importlib.import_module("stable-diffusion_amd._lib")
+ops = importlib.import_module("stable-diffusion_amd.ops")
+
+# known answers of Philox4x32-10 published with the paper's library (counter, key, output words)
+KAT = [((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+       ((0xFFFFFFFF,) * 4, (0xFFFFFFFF,) * 2, (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+       ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+        (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))]
+
+
+@pytest.mark.parametrize("ctr,key,want", KAT)
+def test_oracle_generator_gives_the_published_numbers(ctr, key, want):
+    got = R.philox([np.uint64(c) for c in ctr], key)
+    assert tuple(int(g) for g in got) == want
+
+
+def test_oracle_mask_drops_the_share_it_is_asked_for():
+    n = 1 << 20
+    for p in (0.1, 0.5, 0.9):
+        k = R.keep_scale((1024, n // 1024), p, 1234, 7)
+        dropped = float((k == 0).double().mean())
+        assert abs(dropped - p) < 5 * (p * (1 - p) / n) ** 0.5 + 2.0 ** -17          # five deviations
+
+
+def _refused(name, *args):
+    lib = _lib.lib()
+    rc = getattr(lib, name)(*args)
+    assert rc == -22, (name, rc)
+    return lib.sdmi_last_error().decode()
+
+
+D = ctypes.c_void_p(4096)        # a pointer that no refused call looks behind
+
+
+def test_library_refuses_bad_calls():
+    drop = lambda p=0.1, off=0, dt=1, rows=4, cols=8, x=D, sd=None, ld=8: (x, ld, None, 0, D, rows, cols, p, 1, sd, off, dt, None)
+    assert "probability" in _refused("sdmi_dropout", *drop(p=1.5))
+    assert "probability" in _refused("sdmi_dropout", *drop(p=float("nan")))
+    assert "offset" in _refused("sdmi_dropout", *drop(off=1 << 32))
+    assert "offset" in _refused("sdmi_dropout", *drop(off=-1))
+    assert "dtype" in _refused("sdmi_dropout", *drop(dt=3))
+    assert "negative" in _refused("sdmi_dropout", *drop(rows=-1))
+    assert "negative" in _refused("sdmi_dropout", *drop(ld=-8))
+    assert "null" in _refused("sdmi_dropout", *drop(x=None))
+    assert "aligned" in _refused("sdmi_dropout", *drop(sd=ctypes.c_void_p(4100)))
+
+    lin = lambda rows=4, k=8, n=8, act=0, dt=1, w=D, ws=None: (D, k, w, k, None, None, 0, D, None, rows, k, n, act, 0.0, 0,
+                                                             None, 0, ws, dt, None)
+    assert "size" in _refused("sdmi_linear_act", *lin(k=0))
+    assert "size" in _refused("sdmi_linear_act", *lin(rows=-1))
+    assert "activation" in _refused("sdmi_linear_act", *lin(act=4))
+    assert "dtype" in _refused("sdmi_linear_act", *lin(dt=-1))
+    assert "null" in _refused("sdmi_linear_act", *lin(w=None))
+    lib = _lib.lib()
+    sizes = [(r, k, n) for r in (64, 308, 1024) for k in (4096, 8192) for n in (64, 256)]
+    needs = [s for s in sizes if lib.sdmi_linear_act_workspace_bytes(*s, 1) > 0]
+    assert needs, "no size splits its contraction"
+    assert "workspace" in _refused("sdmi_linear_act", *lin(*needs[0]))
+
+    back = lambda act=0, pre=None, dx=D, dw=D, db=D, x=D, ws=D: (D, 8, pre, x, 8, D, 8, dx, dw, db, 4, 8, 8, act, 0.0, 0, None,
+                                                                0, ws, 1, None)
+    assert "preact" in _refused("sdmi_linear_act_backward", *back(act=1))
+    assert "null" in _refused("sdmi_linear_act_backward", *back(x=None))
+    assert "workspace" in _refused("sdmi_linear_act_backward", *back(ws=None))
+    assert lib.sdmi_linear_act_backward(*back(dx=None, dw=None, db=None)) == 0
+
+    gn = lambda c0=64, c1=0, x1=None, b=1, hw=4, g=32, act=1, dt=1, eps=1e-5, st=D, ws=D: (
+        D, c0, x1, c1, b, hw, g, eps, D, D, act, 0.0, 0, None, 0, D, st, ws, dt, None)
+    assert "groups" in _refused("sdmi_groupnorm_act", *gn(c0=65))
+    assert "groups" in _refused("sdmi_groupnorm_act", *gn(g=0))
+    assert "channels" in _refused("sdmi_groupnorm_act", *gn(c0=8224))
+    assert "eps" in _refused("sdmi_groupnorm_act", *gn(eps=-1.0))
+    assert "null" in _refused("sdmi_groupnorm_act", *gn(c1=32, g=32))
+    assert "null" in _refused("sdmi_groupnorm_act", *gn(st=None))
+    assert "batch" in _refused("sdmi_groupnorm_act", *gn(b=65536))
+    assert "size" in _refused("sdmi_groupnorm_act", *gn(c0=0))
+    assert "workspace" in _refused("sdmi_groupnorm_act", *gn(hw=65536, ws=None))
+    gb = lambda dx0=D, dx1=None, c1=0, x1=None: (D, D, 64, x1, c1, 1, 4, 32, D, D, D, 1, 0.0, 0, None, 0, dx0, dx1, D, D, D, 1,
+                                                 None)
+    assert "neither" in _refused("sdmi_groupnorm_act_backward", *gb(c1=32, x1=D))
+    assert "null" in _refused("sdmi_groupnorm_act_backward", *gb(c1=32, dx1=D))
+
+
+def test_empty_calls_succeed_without_a_gpu():
+    lib = _lib.lib()
+    assert lib.sdmi_dropout(None, 8, None, 0, None, 0, 8, 0.1, 1, None, 0, 1, None) == 0
+    assert lib.sdmi_linear_act(None, 8, None, 8, None, None, 0, None, None, 0, 8, 8, 0, 0.0, 0, None, 0, None, 1, None) == 0
+    assert lib.sdmi_groupnorm_act(None, 64, None, 0, 0, 4, 32, 1e-5, None, None, 1, 0.0, 0, None, 0, None, None, None, 1,
+                                  None) == 0
+
+
+def test_python_refuses_cpu_tensors_and_bad_arguments():
+    x, w = torch.zeros(4, 8), torch.zeros(16, 8)
+    with pytest.raises(ValueError, match="CPU"):
+        ops.dropout(x, 0.1, 1)
+    with pytest.raises(ValueError, match="CPU"):
+        ops.linear_act(x, w)
+    with pytest.raises(ValueError, match="CPU"):
+        ops.groupnorm_act(x.view(1, 4, 8), torch.ones(8), torch.zeros(8), groups=2)
+    dev = torch.device("cpu")
+    for p in (-0.1, 1.1, float("nan")):
+        with pytest.raises(ValueError, match="probability"):
+            ops._drop_state(p, 1, 0, dev)
+    with pytest.raises(ValueError, match="needs a seed"):
+        ops._drop_state(0.5, None, 0, dev)
+    with pytest.raises(ValueError, match="offset"):
+        ops._drop_state(0.5, 1, 1 << 32, dev)
+    with pytest.raises(ValueError, match="64 bits"):
+        ops._drop_state(0.5, 1 << 64, 0, dev)
+    with pytest.raises(ValueError, match="int64"):
+        ops._drop_state(0.5, torch.zeros(1), 0, dev)
+    with pytest.raises(ValueError, match="one"):
+        ops._drop_state(0.5, torch.zeros(2, dtype=torch.int64), 0, dev)
+    with pytest.raises(ValueError, match="activation"):
+        ops._act_code("relu")
