@@ -9,6 +9,9 @@
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
+#ifdef SDMI_TUNE
+#include <stdlib.h>
+#endif
 
 namespace {
 
@@ -45,15 +48,20 @@ struct Epilogue {
   const void* resid; int64_t ldr;
   void* out; int64_t ldo;
   float* preact;                // [M][N] fp32 or null: z, for the backward pass
+  float alpha;                  // the sums are scaled by it first (1, or a gradient's dropout scale)
   int act;
   DropArgs drop;
   int64_t M; int N;
 };
 
-// columns n .. n + 7 of row m (n a multiple of 8; the row's last group may be short)
-template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue& e, unsigned k0, unsigned k1, int64_t m, int n, float (&v)[8]) {
-  const int cnt = e.N - n;
+// columns n .. n + 7 of row m (n a multiple of 8; the row's last group may be short); r: the residual's, if there is one
+// TAIL: short groups may come
+template <typename T, bool TAIL>
+__device__ __forceinline__ void finish8(const Epilogue& e, unsigned k0, unsigned k1, int64_t m, int n, const float (&r)[8],
+                                        float (&v)[8]) {
+  const int cnt = TAIL ? e.N - n : 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= e.alpha;
   if (e.bias) {
     float b[8];
     load8<float>(e.bias + n, cnt, b);
@@ -67,8 +75,6 @@ __device__ __forceinline__ void finish8(const Epilogue& e, unsigned k0, unsigned
   }
   if (e.drop.thr) drop8(v, philox8(k0, k1, (unsigned)n >> 3, (uint64_t)m, e.drop.offset), e.drop.thr, e.drop.scale);
   if (e.resid) {
-    float r[8];
-    load8<T>((const T*)e.resid + m * e.ldr + n, cnt, r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += r[i];
   }
@@ -85,11 +91,11 @@ struct GemmParams {
   Epilogue e;
 };
 
-__device__ const u32x4 g_zero16 = {0, 0, 0, 0};      // contraction indices beyond the end are read here
-
-__device__ __forceinline__ void glds16(const char* src, char* lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+// LDS-DMA of 16 bytes a lane from a uniform base plus a 32-bit offset; an offset beyond the 2 GiB that the descriptor
+// spans is out of its bounds and brings zeros (contraction indices beyond the end)
+constexpr unsigned DMA_SPAN = 0x80000000u, DMA_ZERO = 0x80000000u;
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned off, char* lds_wave_base) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds_wave_base, 16, (int)off, 0, 0, 0);
 }
 
 // An operand's K-tile in LDS is 8 ROWS chunks of 16 bytes; the contraction is KT = 128 bytes deep.
@@ -99,11 +105,12 @@ __device__ __forceinline__ void glds16(const char* src, char* lds_wave_base) {
 // The XOR is applied to the address a lane reads from (LDS-DMA writes lane by lane), and undone where fragments are read.
 template <typename T, int ROWS, bool COLS> struct Tile {
   static constexpr int EPC = 16 / (int)sizeof(T), KT = 8 * EPC, CPR = ROWS / EPC;
+  static_assert(ROWS % 64 == 0, "the XOR stays inside a stored row");
   __device__ static __forceinline__ int swz(int k) {
     if constexpr (!COLS) return k & 7;
     else if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
-    else if constexpr (ROWS >= 128) return ((k & 3) | ((k >> 1) & 4)) << 1;
-    else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;
+    else if constexpr (ROWS % 128 == 0) return ((k & 3) | ((k >> 1) & 4)) << 1;
+    else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;      // rows an odd multiple of 128 bytes apart
   }
   // what chunk `pos` of the tile holds: stored row a (output row, or contraction index), chunk c of it
   __device__ static __forceinline__ void at(int pos, int& a, int& c) {
@@ -142,10 +149,14 @@ template <typename T, int ROWS, bool COLS> struct Tile {
   }
 };
 
-// A workgroup of WQ x WP waves, each FQ x FP fragments; NST LDS stages.  VEC: rows are whole 16-byte chunks at
-// 16-byte addresses and go to LDS by DMA; otherwise chunks are put together in registers, element by element where
-// they end, and written to the other stage behind the products.
-template <typename T, int WQ, int WP, int FQ, int FP, int NST, bool QC, bool PC, bool VEC>
+// A workgroup of WQ x WP waves, each FQ x FP fragments; two LDS stages.  VEC: rows are whole 16-byte chunks at 16-byte
+// addresses and go to LDS by DMA; otherwise chunks are put together in registers, element by element where they end,
+// and written to the other stage behind the products.
+// VEC also means whole groups of eight output columns.
+// PAIR > 0 (the large tiles, one workgroup per CU): the wave groups wp = 0 and 1, one wave of each per SIMD, run the same
+// program one segment apart, so that one group reads fragments while the other keeps the matrix cores busy; a k-step
+// is PAIR segments of FP / PAIR column fragments.
+template <typename T, int WQ, int WP, int FQ, int FP, bool QC, bool PC, bool VEC, int PAIR>
 __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p) {
   constexpr int NW = WQ * WP, NT = 64 * NW, BM = 16 * WQ * FQ, BN = 16 * WP * FP;
   typedef Tile<T, BM, QC> TQ;
@@ -153,8 +164,9 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   constexpr int EPC = TQ::EPC, KT = TQ::KT, SZ = (int)sizeof(T);
   constexpr int NQ = BM * 8 / NT, NP = BN * 8 / NT, STAGE = (BM + BN) * 128;
   static_assert(NQ * NT == BM * 8 && NP * NT == BN * 8, "chunks must divide over the threads");
-  static_assert(VEC || NST == 2, "register staging writes the other of two stages");
-  static_assert(FP % 2 == 0, "the epilogue joins pairs of column fragments");
+  constexpr int NST = 2;
+  static_assert(!PAIR || (VEC && WP == 2), "two groups of waves, staged by DMA");
+  static_assert(FP % 2 == 0, "the epilogue's column groups divide over the lanes");
   __shared__ __align__(16) char smem[NST * STAGE];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
@@ -170,66 +182,74 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   const int64_t ke = kb + p.k_per_split < p.K ? kb + p.k_per_split : p.K;
   const int nk = (int)((ke - kb + KT - 1) / KT);
 
-  // per-thread chunk sources.  Output rows beyond the end repeat the last ones (their results are not stored).
-  const char* src[NQ + NP];
-  int kidx[NQ + NP];                 // contraction index of the chunk inside a K-tile
-  int cnt[NQ + NP];                  // columns operand: elements of the chunk inside the matrix (register staging)
+  // Per-thread chunk sources: offsets from a uniform base that moves with the K-tile.  Output rows beyond the end repeat
+  // the last ones (their results are not stored).  Chunk i of a thread lies i * NT chunks behind its first one.
+  const char* baseq = p.q + (QC ? kb * p.ldq + m0 : m0 * p.ldq + kb) * SZ;
+  const char* basep = p.p + (PC ? kb * p.ldp + n0 : (int64_t)n0 * p.ldp + kb) * SZ;
   const int64_t stepq = QC ? (int64_t)KT * p.ldq * SZ : 128, stepp = PC ? (int64_t)KT * p.ldp * SZ : 128;
-#pragma unroll
-  for (int i = 0; i < NQ + NP; ++i) {
-    const bool isq = i < NQ;
-    const int pos = ((isq ? i : i - NQ) * NW + wave) * 64 + lane;
-    int a, c;
+  const int64_t leftq = p.e.M - m0, leftp = (int64_t)p.e.N - n0;      // output rows / columns from this tile on
+  auto place = [&](int i, bool isq, int& a, int& c) {
+    const int pos = (i * NW + wave) * 64 + lane;
     if (isq) TQ::at(pos, a, c); else TP::at(pos, a, c);
-    const bool cols = isq ? QC : PC;
-    const char* base = isq ? p.q : p.p;
-    const int64_t ld = isq ? p.ldq : p.ldp;
-    const int64_t r0 = isq ? m0 : (int64_t)n0, R = isq ? p.e.M : (int64_t)p.e.N;
-    if (!cols) {
-      const int64_t row = r0 + a < R ? r0 + a : R - 1;
-      kidx[i] = c * EPC; cnt[i] = EPC;
-      src[i] = base + (row * ld + kb + c * EPC) * SZ;
-    } else {
-      int64_t col = r0 + c * EPC;
-      kidx[i] = a;
-      if (VEC) { if (col > R - EPC) col = R - EPC; cnt[i] = EPC; }
-      else { const int64_t left = R - col; cnt[i] = left < 0 ? 0 : (left > EPC ? EPC : (int)left); }
-      src[i] = base + ((kb + a) * ld + col) * SZ;
+  };
+  unsigned off[VEC ? NQ + NP : 1];
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < NQ + NP; ++i) {
+      const bool isq = i < NQ, cols = isq ? QC : PC;
+      const int64_t ld = isq ? p.ldq : p.ldp, left = isq ? leftq : leftp;
+      int a, c;
+      place(isq ? i : i - NQ, isq, a, c);
+      if (!cols) off[i] = (unsigned)(((a < left ? a : left - 1) * ld + c * EPC) * SZ);
+      else off[i] = (unsigned)((a * ld + (c * EPC + EPC <= left ? c * EPC : left - EPC)) * SZ);
     }
   }
 
   u32x4 reg[VEC ? 1 : NQ + NP];
-  auto stage_in = [&](int t) {       // K-tile t: DMA into its stage, or loads into registers
+  auto stage_in = [&](int t) {       // K-tile t: DMA into its stage, or loads into registers; called for t = 0, 1, 2, ...
     const int64_t left = ke - kb - (int64_t)t * KT;
     if constexpr (VEC) {
       char* buf = smem + (t % NST) * STAGE + wave * 1024;
-      const char* zero = reinterpret_cast<const char*>(&g_zero16);
-      const bool full = left >= KT;
+      const auto rq = __builtin_amdgcn_make_buffer_rsrc((void*)baseq, 0, DMA_SPAN, 0x00020000);
+      const auto rp = __builtin_amdgcn_make_buffer_rsrc((void*)basep, 0, DMA_SPAN, 0x00020000);
+      if (left >= KT) {
 #pragma unroll
-      for (int i = 0; i < NQ + NP; ++i) {
-        const char* s = full || kidx[i] < left ? src[i] : zero;
-        glds16(s, buf + i * (NW * 1024));
-        src[i] += i < NQ ? stepq : stepp;
+        for (int i = 0; i < NQ + NP; ++i) dma16(i < NQ ? rq : rp, off[i], buf + i * (NW * 1024));
+      } else {
+#pragma unroll
+        for (int i = 0; i < NQ + NP; ++i) {
+          const bool isq = i < NQ, cols = isq ? QC : PC;
+          int a, c;
+          place(isq ? i : i - NQ, isq, a, c);
+          dma16(isq ? rq : rp, (cols ? a : c * EPC) < left ? off[i] : DMA_ZERO, buf + i * (NW * 1024));
+        }
       }
     } else {
       typedef typename Frag<T>::type F;
       typedef F Fu __attribute__((aligned(sizeof(T))));
 #pragma unroll
       for (int i = 0; i < NQ + NP; ++i) {
-        const bool cols = i < NQ ? QC : PC;
-        const int64_t kleft = left - kidx[i];
-        const int n = kleft <= 0 ? 0 : (cols ? cnt[i] : (kleft < EPC ? (int)kleft : EPC));
+        const bool isq = i < NQ, cols = isq ? QC : PC;
+        const int64_t ld = isq ? p.ldq : p.ldp, out = isq ? leftq : leftp;
+        int a, c;
+        place(isq ? i : i - NQ, isq, a, c);
+        // elements of the chunk that are there
+        const int64_t have = cols ? (a < left ? out - c * EPC : 0) : left - c * EPC;
+        const int n = have <= 0 ? 0 : (have < EPC ? (int)have : EPC);
+        const T* src = reinterpret_cast<const T*>(isq ? baseq : basep) +
+                       (cols ? a * ld + c * EPC : (a < out ? a : out - 1) * ld + c * EPC);
         F f;
         if (n == EPC) {
-          f = *reinterpret_cast<const Fu*>(src[i]);
+          f = *reinterpret_cast<const Fu*>(src);
         } else {
 #pragma unroll
-          for (int e = 0; e < EPC; ++e) f[e] = e < n ? reinterpret_cast<const T*>(src[i])[e] : (T)0.f;
+          for (int e = 0; e < EPC; ++e) f[e] = e < n ? src[e] : (T)0.f;
         }
         reg[i] = __builtin_bit_cast(u32x4, f);
-        src[i] += i < NQ ? stepq : stepp;
       }
     }
+    baseq += stepq;
+    basep += stepp;
   };
   auto regs_to_lds = [&](int t) {
     if constexpr (!VEC) {
@@ -246,74 +266,156 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
 #pragma unroll
     for (int j = 0; j < FQ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](int t) {
+  constexpr int PH = PAIR ? PAIR : 1, FPH = FP / PH;
+  static_assert(FPH * PH == FP, "segments share the column fragments evenly");
+  typename Frag<T>::type fp[FPH], fq[FQ];
+  auto read_frags = [&](int t, int kk, int ph) {
     const char* lq = smem + (t % NST) * STAGE;
     const char* lp = lq + BM * 128;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      typename Frag<T>::type fp[FP], fq[FQ];
-#pragma unroll
-      for (int i = 0; i < FP; ++i) fp[i] = TP::frag(lp, wp * (16 * FP) + i * 16, kk, lane);
+    for (int i = 0; i < FPH; ++i) fp[i] = TP::frag(lp, wp * (16 * FP) + (ph * FPH + i) * 16, kk, lane);
+    if (ph == 0) {
 #pragma unroll
       for (int j = 0; j < FQ; ++j) fq[j] = TQ::frag(lq, wq * (16 * FQ) + j * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < FP; ++i)
-#pragma unroll
-        for (int j = 0; j < FQ; ++j) acc[i][j] = mma(fp[i], fq[j], acc[i][j]);
     }
   };
-
-  if constexpr (VEC) {
-    // ring of NST stages, one barrier per K-tile: a wave waits for its own part of tile t (younger tiles stay in
-    // flight) and for its reads of tile t - 1; behind the barrier the whole tile is there, and the stage of tile
-    // t - 1 is free for tile t + NST - 1
-    constexpr int PER = NQ + NP;
+  auto multiply = [&](int ph) {
 #pragma unroll
-    for (int t = 0; t < NST - 1; ++t)
-      if (t < nk) stage_in(t);
-    for (int t = 0; t < nk; ++t) {
-      const int younger = nk - 1 - t < NST - 2 ? nk - 1 - t : NST - 2;
-      if (younger <= 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      else if (younger == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER) : "memory");
-      else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * PER) : "memory");
+    for (int i = 0; i < FPH; ++i)
+#pragma unroll
+      for (int j = 0; j < FQ; ++j) acc[ph * FPH + i][j] = mma(fp[i], fq[j], acc[ph * FPH + i][j]);
+  };
+
+  if constexpr (PAIR > 0) {
+    // Between two barriers one group reads the fragments of a segment and the other multiplies; group 1 enters one
+    // barrier late.  With I = 4 PH intervals to a K-tile, tile t is read in the intervals I t .. I t + I - 1; its stage
+    // takes the DMA of tile t + 2 from interval I t + I on, and every wave waits for its own part of that before the
+    // barrier that ends interval I t + 2 I - 1.
+    auto barrier = [&]() {
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_barrier();
-      if (t + NST - 1 < nk) stage_in(t + NST - 1);
-      compute(t);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (nk > 0) stage_in(0);
+    if (nk > 1) {
+      stage_in(1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NQ + NP) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    barrier();
+    if (wp == 1) barrier();
+    for (int t = 0; t < nk; ++t) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int ph = 0; ph < PH; ++ph) {
+          const bool last = kk == 1 && ph == PH - 1;
+          read_frags(t, kk, ph);
+          if (kk == 0 && ph == 0 && t >= 1 && t + 1 < nk) stage_in(t + 1);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (last && wp == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          barrier();
+          __builtin_amdgcn_s_setprio(1);
+          multiply(ph);
+          __builtin_amdgcn_s_setprio(0);
+          if (last && wp == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          barrier();
+        }
+    }
+    if (wp == 0) barrier();
+  } else if constexpr (VEC) {
+    // one barrier per K-tile: a wave waits for its own part of tile t and for its reads of tile t - 1; behind the
+    // barrier the whole tile is there, and the stage of tile t - 1 is free for tile t + 1
+    if (nk > 0) stage_in(0);
+    for (int t = 0; t < nk; ++t) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      if (t + 1 < nk) stage_in(t + 1);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) { read_frags(t, kk, 0); multiply(0); }
     }
   } else {
     if (nk > 0) { stage_in(0); regs_to_lds(0); }
     for (int t = 0; t < nk; ++t) {
       __syncthreads();
       if (t + 1 < nk) stage_in(t + 1);
-      compute(t);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) { read_frags(t, kk, 0); multiply(0); }
       if (t + 1 < nk) regs_to_lds(t + 1);      // last read in iteration t - 1, before this iteration's barrier
     }
   }
 
-  // acc[i][j]: lane l holds columns 4 (l / 16) .. + 3 of fragment i, row l % 16 of fragment j.  Swapping 16-lane rows
-  // between two column fragments leaves every lane with 8 consecutive columns (one generator call, 16-byte stores).
-  const int g = lane >> 4;
+  // acc[i][j]: lane l holds columns 4 (l / 16) .. + 3 of fragment i, row l % 16 of fragment j.  Each wave takes its tile
+  // through LDS sixteen rows at a time, so that a lane ends up with eight consecutive columns (one generator call) and
+  // neighbouring lanes with neighbouring columns (whole lines to memory).  The residual of the next sixteen rows is
+  // on its way meanwhile, and goes through LDS too, so that the loop over a lane's items stays rolled: unrolled it
+  // would be 20 copies of the epilogue.
+  typedef typename Vec8u<T>::type V8;
+  constexpr int PITCH = 16 * FP + 4, ITEMS = FP / 2, GPR = 2 * FP;      // floats; items per lane; column groups per row
+  constexpr int STRIP = 16 * PITCH * 4, RES = 16 * 16 * FP * SZ;
+  static_assert(NW * (STRIP + RES) <= NST * STAGE, "the strips reuse the stages");
+  if constexpr (PAIR == 0) __syncthreads();      // (the groups' last barrier stands behind every read of the stages)
+  float* strip = reinterpret_cast<float*>(smem + wave * (STRIP + RES));
+  typedef T V8a __attribute__((ext_vector_type(8)));
+  V8a* rstrip = reinterpret_cast<V8a*>(smem + wave * (STRIP + RES) + STRIP);
+  const bool resid = p.e.resid && !p.partial;
   unsigned k0 = 0, k1 = 0;
   if (p.e.drop.thr && !p.partial) drop_key(p.e.drop, k0, k1);
+  const int nw0 = n0 + wp * (16 * FP);
+  const int64_t mw0 = m0 + wq * (16 * FQ);
+  V8 res[ITEMS];
+  auto load_resid = [&](int j) {
 #pragma unroll
-  for (int j = 0; j < FQ; ++j) {
-    const int64_t m = m0 + wq * (16 * FQ) + j * 16 + (lane & 15);
-#pragma unroll
-    for (int i = 0; i < FP; i += 2) {
-      const int n = n0 + wp * (16 * FP) + i * 16 + (g & 1) * 16 + (g >> 1) * 8;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, (float)acc[i][j][e]),
-                                                        __builtin_bit_cast(unsigned, (float)acc[i + 1][j][e]), false, false);
-        v[e] = __builtin_bit_cast(float, (unsigned)s[0]);
-        v[4 + e] = __builtin_bit_cast(float, (unsigned)s[1]);
-      }
+    for (int q = 0; q < ITEMS; ++q) {
+      const int idx = q * 64 + lane, row = idx / GPR, n = nw0 + (idx - row * GPR) * 8;
+      const int64_t m = mw0 + j * 16 + row;
       if (m < p.e.M && n < p.e.N) {
-        if (p.partial) store8<float>(p.partial + ((int64_t)split * p.e.M + m) * p.e.N + n, p.e.N - n, v);
-        else finish8<T>(p.e, k0, k1, m, n, v);
+        const T* r = (const T*)p.e.resid + m * p.e.ldr + n;
+        if (VEC || n + 8 <= p.e.N) res[q] = *reinterpret_cast<const V8*>(r);
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) res[q][e] = n + e < p.e.N ? r[e] : (T)0.f;
+        }
       }
     }
+  };
+  auto wave_sync = [&]() {                        // the wave's own LDS writes before its reads, and the other way round
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  if (resid) load_resid(0);
+#pragma unroll
+  for (int j = 0; j < FQ; ++j) {
+#pragma unroll
+    for (int i = 0; i < FP; ++i)
+      *reinterpret_cast<f32x4*>(strip + (lane & 15) * PITCH + i * 16 + (lane >> 4) * 4) = acc[i][j];
+    if (resid) {
+#pragma unroll
+      for (int q = 0; q < ITEMS; ++q) rstrip[q * 64 + lane] = res[q];
+      if (j + 1 < FQ) load_resid(j + 1);
+    }
+    wave_sync();
+#pragma unroll 1
+    for (int q = 0; q < ITEMS; ++q) {
+      const int idx = q * 64 + lane, row = idx / GPR, grp = idx - row * GPR;
+      const int64_t m = mw0 + j * 16 + row;
+      const int n = nw0 + grp * 8;
+      float v[8], r[8];
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(strip + row * PITCH + grp * 8);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(strip + row * PITCH + grp * 8 + 4);
+      if (resid) {
+        const V8a rr = rstrip[idx];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = to_f32<T>(rr[e]);
+      }
+      if (m < p.e.M && n < p.e.N) {
+        if (p.partial) store8<float>(p.partial + ((int64_t)split * p.e.M + m) * p.e.N + n, VEC ? 8 : p.e.N - n, v);
+        else finish8<T, !VEC>(p.e, k0, k1, m, n, r, v);
+      }
+    }
+    wave_sync();
   }
 }
 
@@ -329,13 +431,22 @@ struct JoinParams {
 
 template <typename T>
 __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
+  __shared__ float red[16][16];
   if (blockIdx.x >= p.join_blocks) {
     if (blockIdx.y) return;
-    const int n = (int)(blockIdx.x - p.join_blocks) * 256 + (int)threadIdx.x;
-    if (n >= p.db_n) return;
+    // 16 columns x 16 lanes over the strips
+    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, n = (int)(blockIdx.x - p.join_blocks) * 16 + cl;
     float s = 0.f;
-    for (int i = 0; i < p.strips; ++i) s += p.db_partial[(size_t)i * p.db_n + n];
-    p.db[n] = s;
+    if (n < p.db_n)
+      for (int i = rl; i < p.strips; i += 16) s += p.db_partial[(size_t)i * p.db_n + n];
+    red[rl][cl] = s;
+    __syncthreads();
+    if (rl == 0 && n < p.db_n) {
+      s = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s += red[r][cl];
+      p.db[n] = s;
+    }
     return;
   }
   const int64_t row_base = (int64_t)blockIdx.y * p.rows_per_y, left = p.e.M - row_base;
@@ -356,7 +467,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
   }
   unsigned k0 = 0, k1 = 0;
   if (p.e.drop.thr) drop_key(p.e.drop, k0, k1);
-  finish8<T>(p.e, k0, k1, m, n, v);
+  float r8[8];
+  if (p.e.resid) load8<T>((const T*)p.e.resid + m * p.e.ldr + n, p.e.N - n, r8);
+  finish8<T, true>(p.e, k0, k1, m, n, r8, v);
 }
 
 // ---- dz = drop(dy) act'(z), and the strips' column sums ----------------------------------------------
@@ -366,16 +479,18 @@ struct DzParams {
   void* dz;                     // [M][N], null: only the sums are wanted
   float* db_partial;            // [strips][N] or null
   int64_t M, rows_per_strip;
-  int N, act;
+  int N, act, groups;
+  float db_scale;
   DropArgs drop;
 };
 
-// A block takes 32 column groups (256 columns) x 8 row lanes of a strip: consecutive threads read consecutive columns.
+// A block takes `groups` column groups of eight (256 at most) x as many row lanes as its threads give, of one strip:
+// consecutive threads read consecutive columns.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
-  __shared__ float red[8][32 * 8 + 4];
-  const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const int n = (int)(blockIdx.x * 32 + cg) * 8;
+  __shared__ float red[256 * 8];
+  const int lanes = 256 / p.groups, rl = (int)threadIdx.x / p.groups, cg = (int)threadIdx.x - rl * p.groups;
+  const int cgg = (int)blockIdx.x * p.groups + cg, n = cgg * 8;
   const int cnt = p.N - n;
   const int64_t rb = (int64_t)blockIdx.y * p.rows_per_strip;
   const int64_t re = rb + p.rows_per_strip < p.M ? rb + p.rows_per_strip : p.M;
@@ -384,11 +499,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
   for (int e = 0; e < 8; ++e) s[e] = 0.f;
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  if (cnt > 0) {
-    for (int64_t m = rb + rl; m < re; m += 8) {
+  if (cnt > 0 && rl < lanes) {
+    for (int64_t m = rb + rl; m < re; m += lanes) {
       float v[8];
       load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)n >> 3, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
       if (p.act != ACT_NONE) {
         float z[8];
         load8<float>(p.preact + m * p.N + n, cnt, z);
@@ -401,53 +516,102 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
     }
   }
   if (!p.db_partial) return;
+  if (rl < lanes) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) red[rl][cg * 8 + e] = s[e];
+    for (int e = 0; e < 8; ++e) red[threadIdx.x * 8 + e] = s[e];
+  }
   __syncthreads();
-  const int col = (int)blockIdx.x * 256 + (int)threadIdx.x;
-  if (col < p.N) {
+  const int width = p.groups * 8, col0 = (int)blockIdx.x * width;
+  for (int c = threadIdx.x; c < width; c += 256) {
+    if (col0 + c >= p.N) break;
     float t = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x];
-    p.db_partial[(size_t)blockIdx.y * p.N + col] = t;
+    for (int r = 0; r < lanes; ++r) t += red[r * width + c];
+    p.db_partial[(size_t)blockIdx.y * p.N + col0 + c] = t * p.db_scale;
   }
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-// Tile and split of a product.  A workgroup of the large tile does the most work per byte it loads; when there are too
-// few tiles to fill the chip the contraction is split, in shares that are worth a launch.
+// Tile and split of a product: the least of an estimate in microseconds.  A CU works through ceil(workgroups / 256) of
+// them, each costing `step` per K-tile of 128 bytes and its stores (a CU's share of HBM, 20 KB a microsecond); a split
+// contraction stores fp32 and pays a join.  Measured steps (fp16, MI355X, contraction long enough to hide the rest):
+//   256x320 1.85 (forward only: its column operands need more registers than there are), 256x256 1.63 (1.85 with a
+//   column operand), 128x128 0.585 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone)
+// and what the choice is worth (us): 8192x4096x4096 227 at 256x256, 300 at 128x128, 549 at 64x64; 4096x5120x1280 55 at
+// 256x320 (256 tiles, one round), 75 at 256x256 (two rounds); 320x320x65536 41 at 64x64 in 32 splits, 98 at 256x320;
+// 308x768x768 6.6 at 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128 1.8, 64x64
+// 0.48.
 struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; };
 
-Plan plan_product(int64_t M, int N, int64_t K, int esize) {
-  Plan pl;
+enum Form { FORWARD, GRAD_X, GRAD_W };
+// sizes that are no whole 16-byte chunks stay off the large tiles
+Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
+  const bool forward = form == FORWARD;
   const int kt = 128 / esize;
-  auto tiles = [&](int b) { return ((M + b - 1) / b) * (int64_t)((N + b - 1) / b); };
-  int b = tiles(128) >= 192 ? 128 : 64;
-  if (M > 512 && N > 512 && K >= 4096) b = 128;
-  pl.bm = pl.bn = b;
-  pl.tiles_m = (unsigned)((M + b - 1) / b); pl.tiles_n = (unsigned)((N + b - 1) / b);
-  const int64_t t = tiles(b), nkt = (K + kt - 1) / kt;
-  int64_t s = t >= 256 ? 1 : 512 / t;
-  if (s > nkt / 4) s = nkt / 4;
-  if (s < 1) s = 1;
-  const int64_t per = (nkt + s - 1) / s;
-  pl.k_per_split = per * kt;
-  pl.splits = (unsigned)(nkt ? (nkt + per - 1) / per : 1);
-  if (pl.k_per_split == 0) pl.k_per_split = kt;
-  return pl;
+  const int64_t nkt = (K + kt - 1) / kt;
+  const bool whole = esize == 2 && N % 8 == 0 && (form == GRAD_W ? M : K) % 8 == 0;
+  struct Opt { int bm, bn; double step, alone; };
+  const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.48, esize == 2 ? 0.35 : 0.48},
+                       {128, 128, esize == 2 ? 0.585 : 1.8, esize == 2 ? 0.8 : 1.8},
+                       {256, 256, forward ? 1.63 : 1.85, forward ? 1.63 : 1.85},
+                       {256, 320, 1.85, 1.85}};
+  Plan best = {};
+  double best_us = 1e30;
+  const double out = (double)M * N;
+  for (int o = 0; o < (!whole ? 2 : forward ? 4 : 3); ++o) {
+    const Opt& t = opts[o];
+    const int64_t tm = (M + t.bm - 1) / t.bm, tn = (N + t.bn - 1) / t.bn, tiles = tm * tn;
+    if (tiles >= (1ll << 31)) continue;
+    for (int64_t s = 1; s <= 64 && s * 2 <= (nkt > 2 ? nkt : 2); s += s < 4 ? 1 : s < 16 ? 2 : 8) {
+      if (s > 1 && tiles * s > 1536) break;
+      const int64_t per = nkt > 0 ? (nkt + s - 1) / s : 1, used = nkt > 0 ? (nkt + per - 1) / per : 1;
+      const double load = (double)((tiles * used + 255) / 256);
+      double us = load * t.step > t.alone ? load * t.step : t.alone;
+      us = us * per + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
+      if (used > 1) us += out * (4.0 * used + esize) / 8e6 + 3.0;
+      if (us < best_us) {
+        best_us = us;
+        best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt};
+      }
+    }
+  }
+#ifdef SDMI_TUNE
+  if (const char* ev = getenv("TILE")) {
+    int bm, bn, sp;
+    if (sscanf(ev, "%d,%d,%d", &bm, &bn, &sp) == 3) {
+      best.bm = bm; best.bn = bn; best.tiles_m = (unsigned)((M + bm - 1) / bm); best.tiles_n = (unsigned)((N + bn - 1) / bn);
+      if (sp > nkt) sp = (int)nkt;
+      const int64_t per2 = (nkt + sp - 1) / sp;
+      best.k_per_split = per2 * kt; best.splits = (unsigned)((nkt + per2 - 1) / per2);
+    }
+  }
+#endif
+  return best;
 }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 size_t partial_bytes(const Plan& pl, int64_t M, int N) { return pl.splits > 1 ? up256((size_t)pl.splits * M * N * 4) : 0; }
 
-bool chunked(const void* p, int64_t ld, int64_t len, int esize) {      // rows are whole 16-byte chunks at 16-byte addresses
-  return ((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0 && (len * esize) % 16 == 0;
+// rows are whole 16-byte chunks at 16-byte addresses, and the at most 320 of them that a tile takes span less than 2 GiB
+bool chunked(const void* p, int64_t ld, int64_t len, int esize) {
+  return ((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0 && (len * esize) % 16 == 0 && ld * esize < (1 << 22);
 }
 
 template <typename T, bool QC, bool PC, bool VEC>
 void launch_tiles(const GemmParams& g, const Plan& pl, hipStream_t stream) {
   const dim3 grid(g.tiles * g.splits);
-  if (pl.bm == 128) hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 2, 4, 4, 2, QC, PC, VEC>), grid, dim3(256), 0, stream, g);
-  else hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 2, 2, 2, 2, QC, PC, VEC>), grid, dim3(256), 0, stream, g);
+  if constexpr (VEC && sizeof(T) == 2) {
+    if (pl.bm == 256) {
+      if constexpr (!QC && !PC) {
+        if (pl.bn == 320) {
+          hipLaunchKernelGGL((linear_gemm_kernel<T, 4, 2, 4, 10, QC, PC, true, 2>), grid, dim3(512), 0, stream, g);
+          return;
+        }
+      }
+      hipLaunchKernelGGL((linear_gemm_kernel<T, 4, 2, 4, 8, QC, PC, true, 1>), grid, dim3(512), 0, stream, g);
+      return;
+    }
+  }
+  if (pl.bm == 128) hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 2, 4, 4, QC, PC, VEC, 0>), grid, dim3(256), 0, stream, g);
+  else hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 2, 2, 2, QC, PC, VEC, 0>), grid, dim3(256), 0, stream, g);
 }
 
 // db_*: a bias gradient to fold in the join's launch (or in one of its own)
@@ -465,7 +629,7 @@ int launch_join(const float* partial, unsigned splits, const Epilogue& e, const 
   const unsigned ny = rows ? (unsigned)((rows + j.rows_per_y - 1) / j.rows_per_y) : 1u;
   j.join_blocks = (unsigned)(((uint64_t)j.rows_per_y * groups + 255) / 256);
   if (!partial) j.join_blocks = 0;
-  const unsigned db_blocks = f.db ? (unsigned)(f.n + 255) / 256 : 0;
+  const unsigned db_blocks = f.db ? (unsigned)(f.n + 15) / 16 : 0;
   hipLaunchKernelGGL(linear_join_kernel<T>, dim3(j.join_blocks + db_blocks, ny), dim3(256), 0, stream, j);
   SDMI_CHECK_HIP(hipGetLastError());
   return SDMI_OK;
@@ -476,15 +640,19 @@ template <typename T, bool QC, bool PC>
 int product(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e, float* partial,
             const DbFold& fold, bool* folded, hipStream_t stream) {
   const int sz = (int)sizeof(T);
-  const Plan pl = plan_product(e.M, e.N, K, sz);
+  Plan pl = plan_product(e.M, e.N, K, sz, QC ? GRAD_W : PC ? GRAD_X : FORWARD);
+  const bool vec = chunked(q, ldq, QC ? e.M : K, sz) && chunked(p, ldp, PC ? e.N : K, sz) && e.N % 8 == 0;
+  if (!vec && pl.bm == 256) {      // pointers or strides that the sizes do not tell; the splits (and the workspace) stay
+    pl.bm = pl.bn = 128;
+    pl.tiles_m = (unsigned)((e.M + 127) / 128); pl.tiles_n = (unsigned)((e.N + 127) / 128);
+  }
   GemmParams g;
   g.q = (const char*)q; g.p = (const char*)p; g.ldq = ldq; g.ldp = ldp; g.K = K; g.k_per_split = pl.k_per_split;
   g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.e = e;
   const uint64_t total = (uint64_t)pl.tiles_m * pl.tiles_n * pl.splits;
-  SDMI_REQUIRE(total < (1ull << 31), "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
+  SDMI_REQUIRE(pl.bm && total < (1ull << 31), "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
   g.tiles = pl.tiles_m * pl.tiles_n;
   g.partial = pl.splits > 1 ? partial : nullptr;
-  const bool vec = chunked(q, ldq, QC ? e.M : K, sz) && chunked(p, ldp, PC ? e.N : K, sz);
   {
     char label[96];
     snprintf(label, sizeof(label), "linear M%lld N%d K%lld", (long long)e.M, e.N, (long long)K);
@@ -500,29 +668,35 @@ int product(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t K, c
   return SDMI_OK;
 }
 
-struct BwdLayout { size_t dz, dbp, px, pw, total; int strips; int64_t rows_per_strip; bool need_dz; };
+struct BwdLayout { size_t dz, dbp, px, pw, total; int strips, col_blocks, groups; int64_t rows_per_strip; bool need_dz; };
 BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int esize) {
   BwdLayout w;
   size_t o = 0;
   w.need_dz = (act != ACT_NONE || drop) && (want & 3);
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
-  // strips of rows: about 1024 blocks in all, at least 32 rows each
-  const int64_t cblocks = (N + 255) / 256;
-  int64_t strips = (1024 + cblocks - 1) / (cblocks ? cblocks : 1);
-  if (strips > (M + 31) / 32) strips = (M + 31) / 32;
+  // column groups a block takes (all, or an even share), and strips of rows: about 1024 blocks, every row lane at
+  // least four rows where there are that many
+  const int ncg = (N + 7) / 8;
+  w.col_blocks = (ncg + 255) / 256;
+  w.groups = (ncg + w.col_blocks - 1) / w.col_blocks;
+  const int lanes = 256 / w.groups;
+  int64_t strips = 1024 / w.col_blocks;
+  if (strips < 1) strips = 1;
+  const int64_t by_work = (M + 4 * lanes - 1) / (4 * lanes), by_lane = (M + lanes - 1) / lanes;
+  if (strips > by_work) strips = by_work < 64 ? (by_lane < 64 ? by_lane : 64) : by_work;
   if (strips < 1) strips = 1;
   w.rows_per_strip = (M + strips - 1) / strips;
   w.strips = w.rows_per_strip ? (int)((M + w.rows_per_strip - 1) / w.rows_per_strip) : 0;
   w.dbp = o; o += (want & 4) ? up256((size_t)w.strips * N * 4) : 0;
-  w.px = o; o += (want & 1) ? partial_bytes(plan_product(M, K, N, esize), M, K) : 0;
-  w.pw = o; o += (want & 2) ? partial_bytes(plan_product(N, K, M, esize), N, K) : 0;
+  w.px = o; o += (want & 1) ? partial_bytes(plan_product(M, K, N, esize, GRAD_X), M, K) : 0;
+  w.pw = o; o += (want & 2) ? partial_bytes(plan_product(N, K, M, esize, GRAD_W), N, K) : 0;
   w.total = o;
   return w;
 }
 
-Epilogue plain_out(void* out, int64_t M, int N) {
+Epilogue plain_out(void* out, int64_t M, int N, float alpha) {
   Epilogue e = {};
-  e.out = out; e.ldo = N; e.M = M; e.N = N;
+  e.out = out; e.ldo = N; e.M = M; e.N = N; e.alpha = alpha;
   return e;
 }
 
@@ -533,29 +707,33 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
   char* ws = (char*)a.workspace;
   const void* dz = a.dy;
   int64_t lddz = a.lddy;
+  // without an activation dz is dy, masked: its scale waits for the products' epilogue, so that nothing is rounded here
+  const float alpha = a.act == ACT_NONE && drop.thr ? drop.scale : 1.f;
   DbFold fold;
   if (a.rows > 0 && (w.need_dz || a.db)) {
     DzParams d;
     d.dy = a.dy; d.lddy = a.lddy; d.preact = a.act != ACT_NONE ? a.preact : nullptr;
     d.dz = w.need_dz ? ws + w.dz : nullptr;
     d.db_partial = a.db ? (float*)(ws + w.dbp) : nullptr;
-    d.M = a.rows; d.rows_per_strip = w.rows_per_strip; d.N = a.n; d.act = a.act; d.drop = drop;
+    d.M = a.rows; d.rows_per_strip = w.rows_per_strip; d.N = a.n; d.act = a.act; d.drop = drop; d.groups = w.groups;
+    if (a.act == ACT_NONE) d.drop.scale = 1.f;
+    d.db_scale = alpha;
     char label[64];
     snprintf(label, sizeof(label), "linear dz %lldx%d", (long long)a.rows, a.n);
     ProfScope prof(PROF_OTHER, s, 0.0, 2.0 * a.rows * (double)a.n * sizeof(T), label);
-    hipLaunchKernelGGL(linear_dz_kernel<T>, dim3((a.n + 255) / 256, w.strips), dim3(256), 0, s, d);
+    hipLaunchKernelGGL(linear_dz_kernel<T>, dim3(w.col_blocks, w.strips), dim3(256), 0, s, d);
     SDMI_CHECK_HIP(hipGetLastError());
     if (w.need_dz) { dz = d.dz; lddz = a.n; }
   }
   if (a.db) { fold.partial = (const float*)(ws + w.dbp); fold.strips = a.rows > 0 ? w.strips : 0; fold.n = a.n; fold.db = a.db; }
   bool folded = false;
   if (a.dw)
-    SDMI_TRY((product<T, true, true>(dz, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k), (float*)(ws + w.pw), fold,
+    SDMI_TRY((product<T, true, true>(dz, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha), (float*)(ws + w.pw), fold,
                                      &folded, s)));
   if (a.dx && a.rows > 0)
-    SDMI_TRY((product<T, false, true>(dz, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k), (float*)(ws + w.px),
+    SDMI_TRY((product<T, false, true>(dz, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha), (float*)(ws + w.px),
                                       folded ? DbFold() : fold, folded ? nullptr : &folded, s)));
-  if (a.db && !folded) SDMI_TRY(launch_join<T>(nullptr, 0, plain_out(nullptr, 0, 0), fold, s));
+  if (a.db && !folded) SDMI_TRY(launch_join<T>(nullptr, 0, plain_out(nullptr, 0, 0, 1.f), fold, s));
   return SDMI_OK;
 }
 
@@ -572,7 +750,7 @@ int check_common(const LinearActArgs& a, const char* who) {
 
 int64_t linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype) {
   if (rows <= 0 || k <= 0 || n <= 0) return 0;
-  return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype)), rows, n);
+  return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype), FORWARD), rows, n);
 }
 int64_t linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype) {
   if (rows <= 0 || k <= 0 || n <= 0) return 0;
@@ -588,7 +766,7 @@ int linear_act(const LinearActArgs& a, hipStream_t stream) {
   const int64_t need = linear_act_workspace_bytes(a.rows, a.k, a.n, a.dtype);
   SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %lld bytes", (long long)need);
   e.bias = a.bias; e.resid = a.resid; e.ldr = a.ldr; e.out = a.out; e.ldo = a.n;
-  e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
+  e.alpha = 1.f; e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
   SDMI_DISPATCH_DTYPE(a.dtype, T, return (product<T, false, false>(a.x, a.ldx, a.w, a.ldw, a.k, e, (float*)a.workspace,
                                                                      DbFold(), nullptr, stream)));
   return SDMI_OK;
