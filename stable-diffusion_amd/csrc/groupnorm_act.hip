@@ -61,33 +61,51 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[W]) {
     *reinterpret_cast<V*>(p) = r;
   }
 }
-// eight columns that may be short (the row's last) or straddle the two sources
-template <typename T>
-__device__ __forceinline__ void load_cols(const void* x0, const void* x1, int c0, int c1, int64_t row, int c, float (&v)[8]) {
-  if (!x1) load8<T>((const T*)x0 + row * c0 + c, c0 - c, v);
-  else if (c + 8 <= c0) load8<T>((const T*)x0 + row * c0 + c, 8, v);
-  else if (c >= c0) load8<T>((const T*)x1 + row * c1 + (c - c0), c1 - (c - c0), v);
-  else {
+// Eight columns of a two-source row that a thread walks down: where they lie and how many there are.  Whole groups of one
+// source are 16-byte pieces (32 in fp32) that stay packed until they are used; a row's short last group, and one that
+// straddles the sources, go element by element.
+template <typename T> struct Cols {
+  typedef T Raw __attribute__((ext_vector_type(8)));
+  typedef typename Vec8u<T>::type RawU;
+  const T* p0; const T* p1;       // element 0 of row 0 in each source (the columns' own offset included)
+  int c0, c1, n0, n;              // row strides; elements in the first source, in both
+  bool whole;
+  __device__ __forceinline__ Cols(const void* x0, const void* x1, int c0_, int c1_, int c) : c0(c0_), c1(c1_) {
+    const int left = c0 - c, all = c0 + c1 - c;
+    n0 = left < 0 ? 0 : (left < 8 ? left : 8);
+    n = all < 8 ? all : 8;
+    p0 = (const T*)x0 + c;
+    p1 = (const T*)x1 - left;
+    whole = n0 == 8 || (n0 == 0 && n == 8);
+  }
+  __device__ __forceinline__ Raw load(int64_t row) const {
+    Raw r;
+    if (whole) {
+      r = *reinterpret_cast<const RawU*>(n0 ? p0 + row * c0 : p1 + row * c1);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int ce = c + e;
-      v[e] = ce < c0 ? to_f32<T>(((const T*)x0)[row * c0 + ce])
-                     : (ce < c0 + c1 ? to_f32<T>(((const T*)x1)[row * c1 + (ce - c0)]) : 0.f);
+      for (int e = 0; e < 8; ++e) r[e] = e < n0 ? p0[row * c0 + e] : (e < n ? p1[row * c1 + e] : (T)0.f);
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(int64_t row, const float (&v)[8]) const {
+    if (whole) {
+      store8<T>(const_cast<T*>(n0 ? p0 + row * c0 : p1 + row * c1), 8, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (e < n0) const_cast<T*>(p0)[row * c0 + e] = from_f32<T>(v[e]);
+        else if (e < n) const_cast<T*>(p1)[row * c1 + e] = from_f32<T>(v[e]);
+      }
     }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store_cols(void* x0, void* x1, int c0, int c1, int64_t row, int c, const float (&v)[8]) {
-  if (!x1) store8<T>((T*)x0 + row * c0 + c, c0 - c, v);
-  else if (c + 8 <= c0) store8<T>((T*)x0 + row * c0 + c, 8, v);
-  else if (c >= c0) store8<T>((T*)x1 + row * c1 + (c - c0), c1 - (c - c0), v);
+};
+// per-channel fp32 parameters of eight columns (the last one repeated beyond the row)
+__device__ __forceinline__ void load_params(const float* p, int c, int C, float (&v)[8]) {
+  if (c + 8 <= C) load8<float>(p + c, 8, v);
   else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int ce = c + e;
-      if (ce < c0) ((T*)x0)[row * c0 + ce] = from_f32<T>(v[e]);
-      else if (ce < c0 + c1) ((T*)x1)[row * c1 + (ce - c0)] = from_f32<T>(v[e]);
-    }
+    for (int e = 0; e < 8; ++e) v[e] = p[c + e < C ? c + e : C - 1];
   }
 }
 template <typename T> __device__ __forceinline__ float first_of(const GnaParams& p, int b, int c) {
@@ -271,6 +289,7 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
 // ---- strips ------------------------------------------------------------------------------------------
 // A thread owns one group of eight columns and walks every lanes-th pixel of its strip; tensors of more than 2048
 // channels make a thread take several column groups, one after the other.
+constexpr int WALK = 4, WALK_BWD = 2;      // pixels a thread has in flight
 struct Walk { int ncg, lanes, pl, cg0, cgs; int64_t pb, pe; };
 __device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip) {
   Walk w;
@@ -316,6 +335,7 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
   float* s2 = s1 + w.lanes * width;
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
+    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c);
     float sh[8], s[8], q[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -323,21 +343,16 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
       sh[e] = first_of<T>(p, b, (int)div_by((unsigned)ce, p.div_cpg) * p.cpg);
       s[e] = 0.f; q[e] = 0.f;
     }
-    int64_t px = w.pb + w.pl;
-    for (; px + 3 * w.lanes < w.pe; px += 4 * w.lanes) {       // four independent loads in flight
-      float v[4][8];
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK * w.lanes) {
+      typename Cols<T>::Raw r[WALK];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px + u * w.lanes, c, v[u]);
+      for (int u = 0; u < WALK; ++u) r[u] = x.load((int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1));
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < WALK; ++u) {
+        if (px + u * w.lanes >= w.pe) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { const float t = v[u][e] - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
-    }
-    for (; px < w.pe; px += w.lanes) {
-      float v[8];
-      load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px, c, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { const float t = v[e] - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
+        for (int e = 0; e < 8; ++e) { const float t = to_f32<T>(r[u][e]) - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
+      }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
@@ -366,7 +381,15 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
     double a = 0.0, q = 0.0;
     if (g < p.G) {
       const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.strips * p.G + g;
-      for (int s = j; s < p.strips; s += tpg) { const float2 v = src[(size_t)s * p.G]; a += (double)v.x; q += (double)v.y; }
+      int s = j;
+      for (; s + 7 * tpg < p.strips; s += 8 * tpg) {         // eight loads in flight
+        float2 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(s + u * tpg) * p.G];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { a += (double)v[u].x; q += (double)v[u].y; }
+      }
+      for (; s < p.strips; s += tpg) { const float2 v = src[(size_t)s * p.G]; a += (double)v.x; q += (double)v.y; }
     }
     a = fold_lanes(a, tpg);
     q = fold_lanes(q, tpg);
@@ -397,30 +420,29 @@ __global__ __launch_bounds__(256) void gna_apply_kernel(GnaParams p) {
   if (p.drop.thr) drop_key(p.drop, k0, k1);
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
+    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c);
     float mn[8], sc[8], bt[8];
+    load_params(p.gamma, c, p.C, sc);
+    load_params(p.beta, c, p.C, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
-      mn[e] = s_mean[g]; sc[e] = s_rstd[g] * p.gamma[ce]; bt[e] = p.beta[ce];
+      const int g = (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg);
+      mn[e] = s_mean[g]; sc[e] *= s_rstd[g];
     }
-    auto put = [&](int64_t row, float (&v)[8]) {
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK * w.lanes) {
+      typename Cols<T>::Raw r[WALK];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = act_f<T>(fmaf(v[e] - mn[e], sc[e], bt[e]), p.act);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
-      store8<T>((T*)p.out0 + row * p.C + c, p.C - c, v);
-    };
-    int64_t px = w.pb + w.pl;
-    for (; px + 3 * w.lanes < w.pe; px += 4 * w.lanes) {
-      float v[4][8];
+      for (int u = 0; u < WALK; ++u) r[u] = x.load((int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px + u * w.lanes, c, v[u]);
+      for (int u = 0; u < WALK; ++u) {
+        if (px + u * w.lanes >= w.pe) break;
+        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        float v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) put((int64_t)b * p.HW + px + u * w.lanes, v[u]);
-    }
-    for (; px < w.pe; px += w.lanes) {
-      float v[8];
-      load_cols<T>(p.x0, p.x1, p.c0, p.c1, (int64_t)b * p.HW + px, c, v);
-      put((int64_t)b * p.HW + px, v);
+        for (int e = 0; e < 8; ++e) v[e] = act_f<T>(fmaf(to_f32<T>(r[u][e]) - mn[e], sc[e], bt[e]), p.act);
+        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+        store8<T>((T*)p.out0 + row * p.C + c, p.C - c, v);
+      }
     }
   }
 }
@@ -438,26 +460,38 @@ __global__ __launch_bounds__(256) void gna_grad_sums_kernel(GnaParams p) {
   if (p.drop.thr) drop_key(p.drop, k0, k1);
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
+    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c);
     float mn[8], rs[8], ga[8], bt[8], s[8], q[8];
+    load_params(p.gamma, c, p.C, ga);
+    load_params(p.beta, c, p.C, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
-      const float* st = p.stats + ((size_t)b * p.G + g) * 2;
-      mn[e] = st[0]; rs[e] = st[1]; ga[e] = p.gamma[ce]; bt[e] = p.beta[ce];
+      const float* st = p.stats + ((size_t)b * p.G + (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg)) * 2;
+      mn[e] = st[0]; rs[e] = st[1];
       s[e] = 0.f; q[e] = 0.f;
     }
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += w.lanes) {
-      const int64_t row = (int64_t)b * p.HW + px;
-      float x[8], v[8];
-      load_cols<T>(p.x0, p.x1, p.c0, p.c1, row, c, x);
-      load8<T>((const T*)p.dy + row * p.C + c, p.C - c, v);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
+      typename Cols<T>::Raw rx[WALK_BWD], rd[WALK_BWD];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float xh = (x[e] - mn[e]) * rs[e];
-        const float du = v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
-        s[e] += du;
-        q[e] = fmaf(du, xh, q[e]);
+      for (int u = 0; u < WALK_BWD; ++u) {
+        const int64_t row = (int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1);
+        rx[u] = x.load(row); rd[u] = dy.load(row);
+      }
+#pragma unroll
+      for (int u = 0; u < WALK_BWD; ++u) {
+        if (px + u * w.lanes >= w.pe) break;
+        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(rd[u][e]);
+        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float xh = (to_f32<T>(rx[u][e]) - mn[e]) * rs[e];
+          const float du = v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
+          s[e] += du;
+          q[e] = fmaf(du, xh, q[e]);
+        }
       }
     }
 #pragma unroll
@@ -530,27 +564,40 @@ __global__ __launch_bounds__(256) void gna_grad_apply_kernel(GnaParams p) {
   if (p.drop.thr) drop_key(p.drop, k0, k1);
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
+    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c), dx(p.out0, p.out1, p.c0, p.c1, c);
     float mn[8], rs[8], ga[8], bt[8], ma[8], mq[8];
+    load_params(p.gamma, c, p.C, ga);
+    load_params(p.beta, c, p.C, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int ce = c + e < p.C ? c + e : p.C - 1, g = (int)div_by((unsigned)ce, p.div_cpg);
+      const int g = (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg);
       const float* st = p.stats + ((size_t)b * p.G + g) * 2;
-      mn[e] = st[0]; rs[e] = st[1]; ga[e] = p.gamma[ce]; bt[e] = p.beta[ce];
+      mn[e] = st[0]; rs[e] = st[1];
       ma[e] = s_a[g]; mq[e] = s_q[g];
     }
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += w.lanes) {
-      const int64_t row = (int64_t)b * p.HW + px;
-      float x[8], v[8];
-      load_cols<T>(p.x0, p.x1, p.c0, p.c1, row, c, x);
-      load8<T>((const T*)p.dy + row * p.C + c, p.C - c, v);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
+      typename Cols<T>::Raw rx[WALK_BWD], rd[WALK_BWD];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float xh = (x[e] - mn[e]) * rs[e];
-        const float h = ga[e] * v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
-        x[e] = rs[e] * (h - ma[e] - xh * mq[e]);
+      for (int u = 0; u < WALK_BWD; ++u) {
+        const int64_t row = (int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1);
+        rx[u] = x.load(row); rd[u] = dy.load(row);
       }
-      store_cols<T>(p.out0, p.out1, p.c0, p.c1, row, c, x);
+#pragma unroll
+      for (int u = 0; u < WALK_BWD; ++u) {
+        if (px + u * w.lanes >= w.pe) break;
+        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(rd[u][e]);
+        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float xh = (to_f32<T>(rx[u][e]) - mn[e]) * rs[e];
+          const float h = ga[e] * v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
+          v[e] = rs[e] * (h - ma[e] - xh * mq[e]);
+        }
+        dx.store(row, v);
+      }
     }
   }
 }
@@ -588,6 +635,7 @@ GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backwa
   if (strips > 256) strips = 256;
   if (strips < 1) strips = 1;
   pl.px_per_strip = (HW + strips - 1) / strips;
+  pl.px_per_strip = (pl.px_per_strip + 4 * lanes - 1) / (4 * lanes) * (4 * lanes);      // whole walks of every lane
   pl.strips = (int)((HW + pl.px_per_strip - 1) / pl.px_per_strip);
   pl.lds = 2 * lanes * ncg * 8 * 4;
   pl.part = 0;

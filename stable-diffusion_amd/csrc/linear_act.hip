@@ -117,37 +117,45 @@ template <typename T, int ROWS, bool COLS> struct Tile {
     if constexpr (!COLS) { a = pos >> 3; c = (pos & 7) ^ swz(a); }
     else { a = pos / CPR; c = (pos % CPR) ^ swz(a); }
   }
-  // fragment of rows r0 .. r0 + 15 (a multiple of 16), k-step kk (of 2)
-  __device__ static __forceinline__ typename Frag<T>::type frag(const char* lds, int r0, int kk, int lane) {
+  // fragment dyn + i of sixteen rows, k-step kk (of 2); dyn is the wave's, i a constant, and they have no bit in common:
+  // the chunk XOR then is one value per lane that constants are XORed to and added to
+  __device__ static __forceinline__ typename Frag<T>::type frag(const char* lds, int dyn, int i, int kk, int lane) {
     typedef typename Frag<T>::type F;
-    const int i = lane & 15, g = lane >> 4;
+    const int r = lane & 15, g = lane >> 4;
     if constexpr (!COLS) {
-      const int row = r0 + i;
-      return *reinterpret_cast<const F*>(lds + row * 128 + (((kk * 4 + g) ^ swz(row)) << 4));
+      return *reinterpret_cast<const F*>(lds + (dyn * 16 + r) * 128 + (((kk * 4 + g) ^ (r & 7)) << 4) + i * 2048);
     } else if constexpr (sizeof(T) == 4) {
       F f;
-      const int k = kk * 16 + g * 4, c = (r0 + i) >> 2;
+      const int k = kk * 16 + g * 4, c = (dyn + i) * 4 + (r >> 2);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        f[e] = *reinterpret_cast<const float*>(lds + (k + e) * (ROWS * 4) + ((c ^ swz(k)) << 4) + ((i & 3) << 2));
+        f[e] = *reinterpret_cast<const float*>(lds + (k + e) * (ROWS * 4) + ((c ^ swz(k)) << 4) + ((r & 3) << 2));
       return f;
     } else {
       // two transposing reads of 4 contraction indices each: in every group of 16 lanes, lanes 4 j + q point at
-      // columns 4 q .. 4 q + 3 of index j, and lane i gets column i of the four indices
-      const int c = (r0 >> 3) + ((i & 3) >> 1);
+      // columns 4 q .. 4 q + 3 of index j, and lane r gets column r of the four indices
+      constexpr int MASK = ROWS % 128 == 0 ? 7 : 3;            // fragments the XOR permutes among themselves
+      const int k = g * 8 + (r >> 2);                          // swz(k) is that of every index read here
+      const int lane_at = k * (ROWS * 2) + ((r & 3) << 3);
+      const int seg = dyn ^ (swz(k) >> 1) ^ (i & MASK);
+      const char* a = lds + lane_at + (seg << 5) + ((i & ~MASK) << 5) + kk * 32 * (ROWS * 2);
       u32x2 h[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int k = kk * 32 + g * 8 + t * 4 + (i >> 2);
-        const char* a = lds + k * (ROWS * 2) + ((c ^ swz(k)) << 4) + ((i & 1) << 3);
+      for (int t = 0; t < 2; ++t)
         h[t] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                   (__attribute__((address_space(3))) s16x4*)(a)));
-      }
+                   (__attribute__((address_space(3))) s16x4*)(a + t * 4 * (ROWS * 2))));
       const u32x4 w = {h[0].x, h[0].y, h[1].x, h[1].y};
       return __builtin_bit_cast(F, w);
     }
   }
 };
+
+// Column fragment i of wave group wp: the wave's own run of FP, but for FP = 10 (no power of two) eight of a run and two
+// behind all runs, so that the wave's part and the constant part of the index have no bit in common.
+template <int FP, int WP> __device__ __forceinline__ int col_dyn(int wp, int i) {
+  if constexpr (FP == 10) return i < 8 ? wp * 8 : WP * 8 + wp * 2; else return wp * FP;
+}
+template <int FP> __device__ __forceinline__ constexpr int col_const(int i) { return FP == 10 && i >= 8 ? i - 8 : i; }
 
 // A workgroup of WQ x WP waves, each FQ x FP fragments; two LDS stages.  VEC: rows are whole 16-byte chunks at 16-byte
 // addresses and go to LDS by DMA; otherwise chunks are put together in registers, element by element where they end,
@@ -273,10 +281,13 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
     const char* lq = smem + (t % NST) * STAGE;
     const char* lp = lq + BM * 128;
 #pragma unroll
-    for (int i = 0; i < FPH; ++i) fp[i] = TP::frag(lp, wp * (16 * FP) + (ph * FPH + i) * 16, kk, lane);
+    for (int i = 0; i < FPH; ++i) {
+      const int f = ph * FPH + i;
+      fp[i] = TP::frag(lp, col_dyn<FP, WP>(wp, f), col_const<FP>(f), kk, lane);
+    }
     if (ph == 0) {
 #pragma unroll
-      for (int j = 0; j < FQ; ++j) fq[j] = TQ::frag(lq, wq * (16 * FQ) + j * 16, kk, lane);
+      for (int j = 0; j < FQ; ++j) fq[j] = TQ::frag(lq, wq * FQ, j, kk, lane);
     }
   };
   auto multiply = [&](int ph) {
@@ -362,13 +373,16 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   const bool resid = p.e.resid && !p.partial;
   unsigned k0 = 0, k1 = 0;
   if (p.e.drop.thr && !p.partial) drop_key(p.e.drop, k0, k1);
-  const int nw0 = n0 + wp * (16 * FP);
+  auto col_of = [&](int grp) {                   // first column of the wave's group of eight
+    const int i = grp >> 1;
+    return n0 + (col_dyn<FP, WP>(wp, i) + col_const<FP>(i)) * 16 + (grp & 1) * 8;
+  };
   const int64_t mw0 = m0 + wq * (16 * FQ);
   V8 res[ITEMS];
   auto load_resid = [&](int j) {
 #pragma unroll
     for (int q = 0; q < ITEMS; ++q) {
-      const int idx = q * 64 + lane, row = idx / GPR, n = nw0 + (idx - row * GPR) * 8;
+      const int idx = q * 64 + lane, row = idx / GPR, n = col_of(idx - row * GPR);
       const int64_t m = mw0 + j * 16 + row;
       if (m < p.e.M && n < p.e.N) {
         const T* r = (const T*)p.e.resid + m * p.e.ldr + n;
@@ -401,7 +415,7 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
     for (int q = 0; q < ITEMS; ++q) {
       const int idx = q * 64 + lane, row = idx / GPR, grp = idx - row * GPR;
       const int64_t m = mw0 + j * 16 + row;
-      const int n = nw0 + grp * 8;
+      const int n = col_of(grp);
       float v[8], r[8];
       *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(strip + row * PITCH + grp * 8);
       *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(strip + row * PITCH + grp * 8 + 4);
@@ -420,7 +434,9 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
 }
 
 // ---- joins -----------------------------------------------------------------------------------------
-// Sum of the splits in a fixed order, then the epilogue; the blocks behind the rows' fold the bias gradient's strips.
+// Sum of the splits in a fixed order, then the epilogue.  A group of eight columns is summed by LANES threads, each over
+// every LANES-th split (four loads in flight), and finished by the first of them.  The blocks behind the rows' fold the
+// bias gradient's strips.
 struct JoinParams {
   const float* partial; unsigned splits;
   unsigned rows_per_y; FastDiv groups;
@@ -429,42 +445,84 @@ struct JoinParams {
   unsigned join_blocks;
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
-  __shared__ float red[16][16];
-  if (blockIdx.x >= p.join_blocks) {
-    if (blockIdx.y) return;
-    // 16 columns x 16 lanes over the strips
-    const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, n = (int)(blockIdx.x - p.join_blocks) * 16 + cl;
-    float s = 0.f;
-    if (n < p.db_n)
-      for (int i = rl; i < p.strips; i += 16) s += p.db_partial[(size_t)i * p.db_n + n];
-    red[rl][cl] = s;
-    __syncthreads();
-    if (rl == 0 && n < p.db_n) {
-      s = 0.f;
+__device__ __forceinline__ void fold_bias_gradient(const JoinParams& p, float (*red)[16]) {
+  // 16 columns x 16 lanes over the strips
+  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, n = (int)(blockIdx.x - p.join_blocks) * 16 + cl;
+  float s = 0.f;
+  if (n < p.db_n) {
+    const float* src = p.db_partial + n;
+    int i = rl;
+    for (; i + 48 < p.strips; i += 64) {
+      const float a = src[(size_t)i * p.db_n], b = src[(size_t)(i + 16) * p.db_n], c = src[(size_t)(i + 32) * p.db_n],
+                  d = src[(size_t)(i + 48) * p.db_n];
+      s += (a + b) + (c + d);
+    }
+    for (; i < p.strips; i += 16) s += src[(size_t)i * p.db_n];
+  }
+  red[rl][cl] = s;
+  __syncthreads();
+  if (rl == 0 && n < p.db_n) {
+    s = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += red[r][cl];
-      p.db[n] = s;
+    for (int r = 0; r < 16; ++r) s += red[r][cl];
+    p.db[n] = s;
+  }
+}
+
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
+  __shared__ float red[LANES > 1 ? LANES - 1 : 1][256 / LANES][8];
+  if (blockIdx.x >= p.join_blocks) {
+    if (blockIdx.y == 0) {
+      __shared__ float db_red[16][16];
+      fold_bias_gradient(p, db_red);
     }
     return;
   }
+  constexpr unsigned GROUPS = 256 / LANES;
   const int64_t row_base = (int64_t)blockIdx.y * p.rows_per_y, left = p.e.M - row_base;
   const unsigned rows = left < (int64_t)p.rows_per_y ? (unsigned)left : p.rows_per_y;
-  const unsigned i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= rows * p.groups.d) return;
-  const unsigned r = div_by(i, p.groups);
-  const int n = (int)(i - r * p.groups.d) * 8;
+  const unsigned gl = threadIdx.x % GROUPS, sl = threadIdx.x / GROUPS;
+  const unsigned i = blockIdx.x * GROUPS + gl;
+  const bool live = i < rows * p.groups.d;
+  const unsigned r = div_by(live ? i : 0, p.groups);
+  const int n = (int)((live ? i : 0) - r * p.groups.d) * 8;
   const int64_t m = row_base + r;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = 0.f;
-  for (unsigned s = 0; s < p.splits; ++s) {
-    float w[8];
-    load8<float>(p.partial + ((int64_t)s * p.e.M + m) * p.e.N + n, p.e.N - n, w);
+  if (live) {
+    const float* src = p.partial + m * p.e.N + n;
+    const int64_t step = p.e.M * p.e.N;
+    const int cnt = p.e.N - n;
+    unsigned s = sl;
+    for (; s + 3 * LANES < p.splits; s += 4 * LANES) {
+      float w[4][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += w[e];
+      for (int u = 0; u < 4; ++u) load8<float>(src + (s + u * LANES) * step, cnt, w[u]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += (w[0][e] + w[1][e]) + (w[2][e] + w[3][e]);
+    }
+    for (; s < p.splits; s += LANES) {
+      float w[8];
+      load8<float>(src + s * step, cnt, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += w[e];
+    }
   }
+  if constexpr (LANES > 1) {
+    if (sl > 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) red[sl - 1][gl][e] = v[e];
+    }
+    __syncthreads();
+    if (sl > 0) return;
+#pragma unroll
+    for (int l = 0; l < LANES - 1; ++l)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += red[l][gl][e];
+  }
+  if (!live) return;
   unsigned k0 = 0, k1 = 0;
   if (p.e.drop.thr) drop_key(p.e.drop, k0, k1);
   float r8[8];
@@ -500,19 +558,29 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
   if (cnt > 0 && rl < lanes) {
-    for (int64_t m = rb + rl; m < re; m += lanes) {
-      float v[8];
-      load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
-      if (p.act != ACT_NONE) {
-        float z[8];
-        load8<float>(p.preact + m * p.N + n, cnt, z);
+    // U rows at a time, their loads ahead of the arithmetic; rows beyond the strip repeat its last one and count nothing
+    constexpr int U = 2;
+    for (int64_t m0 = rb + rl; m0 < re; m0 += U * lanes) {
+      float v[U][8], z[U][8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= act_grad<T>(z[e], p.act);
+      for (int u = 0; u < U; ++u) {
+        const int64_t m = m0 + u * lanes < re ? m0 + u * lanes : re - 1;
+        load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v[u]);
+        if (p.act != ACT_NONE) load8<float>(p.preact + m * p.N + n, cnt, z[u]);
       }
-      if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += v[e];
+      for (int u = 0; u < U; ++u) {
+        const int64_t m = m0 + u * lanes;
+        if (m >= re) break;
+        if (p.drop.thr) drop8(v[u], philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
+        if (p.act != ACT_NONE) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[u][e] *= act_grad<T>(z[u][e], p.act);
+        }
+        if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v[u]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += v[u][e];
+      }
     }
   }
   if (!p.db_partial) return;
@@ -533,13 +601,12 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // ---- host ------------------------------------------------------------------------------------------
 // Tile and split of a product: the least of an estimate in microseconds.  A CU works through ceil(workgroups / 256) of
 // them, each costing `step` per K-tile of 128 bytes and its stores (a CU's share of HBM, 20 KB a microsecond); a split
-// contraction stores fp32 and pays a join.  Measured steps (fp16, MI355X, contraction long enough to hide the rest):
-//   256x320 1.85 (forward only: its column operands need more registers than there are), 256x256 1.63 (1.85 with a
-//   column operand), 128x128 0.585 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone)
-// and what the choice is worth (us): 8192x4096x4096 227 at 256x256, 300 at 128x128, 549 at 64x64; 4096x5120x1280 55 at
-// 256x320 (256 tiles, one round), 75 at 256x256 (two rounds); 320x320x65536 41 at 64x64 in 32 splits, 98 at 256x320;
-// 308x768x768 6.6 at 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128 1.8, 64x64
-// 0.48.
+// contraction stores fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.6
+// with a column operand, not for two: their addresses do not fit the registers beside 160 accumulators), 256x256 1.55
+// (1.72 with column operands), 128x128 0.55 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone).  What the choice is
+// worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
+// round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
+// 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128 1.8, 64x64 0.48.
 struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; };
 
 enum Form { FORWARD, GRAD_X, GRAD_W };
@@ -551,13 +618,13 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
   const bool whole = esize == 2 && N % 8 == 0 && (form == GRAD_W ? M : K) % 8 == 0;
   struct Opt { int bm, bn; double step, alone; };
   const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.48, esize == 2 ? 0.35 : 0.48},
-                       {128, 128, esize == 2 ? 0.585 : 1.8, esize == 2 ? 0.8 : 1.8},
-                       {256, 256, forward ? 1.63 : 1.85, forward ? 1.63 : 1.85},
-                       {256, 320, 1.85, 1.85}};
+                       {128, 128, esize == 2 ? 0.55 : 1.8, esize == 2 ? 0.8 : 1.8},
+                       {256, 256, forward ? 1.55 : 1.72, 0.0},
+                       {256, 320, forward ? 1.85 : 2.6, 0.0}};
   Plan best = {};
   double best_us = 1e30;
   const double out = (double)M * N;
-  for (int o = 0; o < (!whole ? 2 : forward ? 4 : 3); ++o) {
+  for (int o = 0; o < (!whole ? 2 : form == GRAD_W ? 3 : 4); ++o) {
     const Opt& t = opts[o];
     const int64_t tm = (M + t.bm - 1) / t.bm, tn = (N + t.bn - 1) / t.bn, tiles = tm * tn;
     if (tiles >= (1ll << 31)) continue;
@@ -567,7 +634,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
       const double load = (double)((tiles * used + 255) / 256);
       double us = load * t.step > t.alone ? load * t.step : t.alone;
       us = us * per + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
-      if (used > 1) us += out * (4.0 * used + esize) / 8e6 + 3.0;
+      if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 4.0;
       if (us < best_us) {
         best_us = us;
         best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt};
@@ -600,7 +667,7 @@ void launch_tiles(const GemmParams& g, const Plan& pl, hipStream_t stream) {
   const dim3 grid(g.tiles * g.splits);
   if constexpr (VEC && sizeof(T) == 2) {
     if (pl.bm == 256) {
-      if constexpr (!QC && !PC) {
+      if constexpr (!QC) {
         if (pl.bn == 320) {
           hipLaunchKernelGGL((linear_gemm_kernel<T, 4, 2, 4, 10, QC, PC, true, 2>), grid, dim3(512), 0, stream, g);
           return;
@@ -624,13 +691,16 @@ int launch_join(const float* partial, unsigned splits, const Epilogue& e, const 
   j.db_partial = f.partial; j.strips = f.strips; j.db_n = f.n; j.db = f.db;
   const unsigned groups = (unsigned)(e.N + 7) / 8;
   j.groups = fast_div(groups ? groups : 1);
-  const int64_t cap = 0x70000000u / j.groups.d, rows = partial ? e.M : 0;
+  const int64_t cap = 0x08000000u / j.groups.d, rows = partial ? e.M : 0;
   j.rows_per_y = (unsigned)(rows < cap ? rows : cap);
   const unsigned ny = rows ? (unsigned)((rows + j.rows_per_y - 1) / j.rows_per_y) : 1u;
-  j.join_blocks = (unsigned)(((uint64_t)j.rows_per_y * groups + 255) / 256);
-  if (!partial) j.join_blocks = 0;
+  // eight threads a group where there are that many splits to read and too few groups to fill the chip with one each
+  const int lanes = splits >= 8 && e.M * (int64_t)groups < (1 << 18) ? 8 : 1;
+  j.join_blocks = partial ? (unsigned)(((uint64_t)j.rows_per_y * groups * lanes + 255) / 256) : 0;
   const unsigned db_blocks = f.db ? (unsigned)(f.n + 15) / 16 : 0;
-  hipLaunchKernelGGL(linear_join_kernel<T>, dim3(j.join_blocks + db_blocks, ny), dim3(256), 0, stream, j);
+  const dim3 grid(j.join_blocks + db_blocks, ny);
+  if (lanes == 8) hipLaunchKernelGGL((linear_join_kernel<T, 8>), grid, dim3(256), 0, stream, j);
+  else hipLaunchKernelGGL((linear_join_kernel<T, 1>), grid, dim3(256), 0, stream, j);
   SDMI_CHECK_HIP(hipGetLastError());
   return SDMI_OK;
 }
