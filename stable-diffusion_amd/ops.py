@@ -302,15 +302,28 @@ def _act_code(act):
     return _ACTS[act]
 
 
+# The wrappers below cost as much as the kernels of a small call, and backward passes run in a thread of torch's own, on
+# cold caches: hence the table of entry points, the raw device and stream queries (the Stream object that
+# torch.cuda.current_stream builds costs 3 us, and 16 us there) and what forward leaves ready in ctx.
+_CODES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ENTRIES = {}
+
+
+def _entry(name):
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
+    return fn
+
+
 def _run(device, name, *args):
-    """One call of the library on ``device``'s current stream (the raw stream: the Stream object that
-    torch.cuda.current_stream builds costs 3 us, and 16 us in the thread that runs backward passes)."""
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    """One call of the library on the current stream of device number ``device``."""
+    fn = _ENTRIES.get(name) or _entry(name)
+    if device == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
     if code:
         check(code, name)
 
@@ -334,14 +347,14 @@ def _check_like(what, t, device, dtype, shape=None):
         raise ValueError(f"{what} is on {t.device}, expected {device}")
     if t.dtype != dtype:
         raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _check_input(what, x):
     if not x.is_cuda:
         raise ValueError(f"{what} is on {x.device}: there is no CPU path")
-    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if x.dtype not in _CODES:
         raise ValueError(f"{what} is {x.dtype}, expected float32, float16 or bfloat16")
 
 
@@ -383,29 +396,33 @@ def _dropout(x, resid, p, seed, seed_t, offset):
     out = x.new_empty(x.shape)
     x2, ldx, rows = _rows(x, cols)
     r2, ldr = (None, 0) if resid is None else _rows(resid, cols)[:2]
-    _run(x.device, "sdmi_dropout", _p(x2), ldx, _p(r2), ldr, _p(out), rows, cols, p, seed, _p(seed_t), offset,
-         dtype_code(x.dtype))
+    _run(x.get_device(), "sdmi_dropout", x2.data_ptr(), ldx, _p(r2), ldr, out.data_ptr(), rows, cols, p, seed, _p(seed_t),
+         offset, _CODES[x.dtype])
     return out
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, resid, seed_t, p, seed, offset):
-        ctx.save_for_backward(seed_t)
-        ctx.drop = (p, seed, offset)
+        if seed_t is not None:
+            ctx.save_for_backward(seed_t)
+        ctx.args = (p, seed, offset, seed_t is not None) + ctx.needs_input_grad[:2]
         return _dropout(x, resid, p, seed, seed_t, offset)
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
-        p, seed, offset = ctx.drop
-        seed_t, = ctx.saved_tensors
-        dx = _dropout(dy, None, p, seed, seed_t, offset) if ctx.needs_input_grad[0] else None
-        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None, None
+        p, seed, offset, seeded, need_x, need_r = ctx.args
+        dx = _dropout(dy, None, p, seed, ctx.saved_tensors[0] if seeded else None, offset) if need_x else None
+        return dx, (dy if need_r else None), None, None, None, None
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def dropout(x, p, seed, offset=0, resid=None):
@@ -425,58 +442,60 @@ def dropout(x, p, seed, offset=0, resid=None):
     return _dropout(x, resid, p, seed, seed_t, offset)
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, want_preact):
     n, k = w.shape
-    dt = dtype_code(x.dtype)
+    dt = _CODES[x.dtype]
     out = x.new_empty(x.shape[:-1] + (n,))
     x2, ldx, rows = _rows(x, k)
     w2, ldw, _ = _rows(w, k)
     r2, ldr = (None, 0) if resid is None else _rows(resid, n)[:2]
-    preact = torch.empty((rows, n), dtype=torch.float32, device=x.device) if want_preact else None
-    ws = _workspace(_lib.lib().sdmi_linear_act_workspace_bytes(rows, k, n, dt), x.device)
-    _run(x.device, "sdmi_linear_act", _p(x2), ldx, _p(w2), ldw, _p(bias), _p(r2), ldr, _p(out), _p(preact), rows, k, n,
-         act, p, seed, _p(seed_t), offset, _p(ws), dt)
+    preact = x.new_empty((rows, n), dtype=torch.float32) if want_preact else None
+    ws = _workspace(_entry("sdmi_linear_act_workspace_bytes")(rows, k, n, dt), x)
+    _run(x.get_device(), "sdmi_linear_act", x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(bias), _p(r2), ldr, out.data_ptr(),
+         _p(preact), rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
     return out, preact
 
 
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, resid, seed_t, act, p, seed, offset):
-        need = ctx.needs_input_grad
-        product = need[0] or need[1] or need[2]
-        out, preact = _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, act != 0 and product)
-        ctx.save_for_backward(x if need[1] else None, w if need[0] else None, preact, seed_t)
-        ctx.drop = (p, seed, offset)
-        ctx.act, ctx.kn, ctx.xshape = act, (w.shape[1], w.shape[0]), x.shape
+        need_x, need_w, need_b, need_r = need = ctx.needs_input_grad[:4]
+        want = (1 if need_x else 0) | (2 if need_w else 0) | (4 if need_b else 0)
+        out, preact = _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, act != 0 and want != 0)
+        if want:
+            ctx.save_for_backward(x if need_w else None, w if need_x else None, preact, seed_t)
+        ctx.args = (want, need_r, w.shape, x.shape, act, p, seed, offset)
         return out
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
-        x, w, preact, seed_t = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        k, n = ctx.kn
+        want, need_r, (n, k), xshape, act, p, seed, offset = ctx.args
         dx = dw = db = None
-        if need_x or need_w or need_b:
-            p, seed, offset = ctx.drop
-            dev, dt = dy.device, dtype_code(dy.dtype)
+        if want:
+            x, w, preact, seed_t = ctx.saved_tensors
+            dt = _CODES[dy.dtype]
             d2, ldd, rows = _rows(dy, n)
-            x2, ldx = (None, 0) if x is None else _rows(x, k)[:2]
-            w2, ldw = (None, 0) if w is None else _rows(w, k)[:2]
-            if need_x:
-                dx = dy.new_empty(ctx.xshape)
-            if need_w:
+            xp = wp = dxp = dwp = dbp = None
+            ldx = ldw = 0
+            if want & 1:
+                w, ldw, _ = _rows(w, k)
+                dx = dy.new_empty(xshape)
+                wp, dxp = w.data_ptr(), dx.data_ptr()
+            if want & 2:
+                x, ldx, _ = _rows(x, k)
                 dw = dy.new_empty((n, k))
-            if need_b:
-                db = torch.empty((n,), dtype=torch.float32, device=dev)
-            want = (1 if need_x else 0) | (2 if need_w else 0) | (4 if need_b else 0)
-            ws = _workspace(_lib.lib().sdmi_linear_act_backward_workspace_bytes(rows, k, n, ctx.act, p, want, dt), dev)
-            _run(dev, "sdmi_linear_act_backward", _p(d2), ldd, _p(preact), _p(x2), ldx, _p(w2), ldw, _p(dx), _p(dw),
-                 _p(db), rows, k, n, ctx.act, p, seed, _p(seed_t), offset, _p(ws), dt)
+                xp, dwp = x.data_ptr(), dw.data_ptr()
+            if want & 4:
+                db = dy.new_empty((n,), dtype=torch.float32)
+                dbp = db.data_ptr()
+            ws = _workspace(_entry("sdmi_linear_act_backward_workspace_bytes")(rows, k, n, act, p, want, dt), dy)
+            _run(dy.get_device(), "sdmi_linear_act_backward", d2.data_ptr(), ldd, _p(preact), xp, ldx, wp, ldw, dxp, dwp, dbp,
+                 rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
         return dx, dw, db, (dy if need_r else None), None, None, None, None, None
 
 
@@ -497,7 +516,7 @@ def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0
         _check_like("bias", bias, x.device, torch.float32, (n,))
         bias = bias.contiguous()
     if resid is not None:
-        _check_like("resid", resid, x.device, x.dtype, tuple(x.shape[:-1]) + (n,))
+        _check_like("resid", resid, x.device, x.dtype, x.shape[:-1] + (n,))
     if _wants_grad(x, w, bias, resid):
         return _LinearActFn.apply(x, w, bias, resid, seed_t, act, p, seed, offset)
     return _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, False)[0]
@@ -512,12 +531,12 @@ def _gn_sizes(x, x1):
 
 def _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset):
     b, hw, c0, c1 = _gn_sizes(x, x1)
-    dt = dtype_code(x.dtype)
+    dt = _CODES[x.dtype]
     out = x.new_empty(x.shape[:-1] + (c0 + c1,))
-    stats = torch.empty((b, groups, 2), dtype=torch.float32, device=x.device)
-    ws = _workspace(_lib.lib().sdmi_groupnorm_act_workspace_bytes(b, hw, c0, c1, groups, dt, 0), x.device)
-    _run(x.device, "sdmi_groupnorm_act", _p(x), c0, _p(x1), c1, b, hw, groups, eps, _p(gamma), _p(beta), act, p, seed,
-         _p(seed_t), offset, _p(out), _p(stats), _p(ws), dt)
+    stats = x.new_empty((b, groups, 2), dtype=torch.float32)
+    ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 0), x)
+    _run(x.get_device(), "sdmi_groupnorm_act", x.data_ptr(), c0, _p(x1), c1, b, hw, groups, eps, gamma.data_ptr(),
+         beta.data_ptr(), act, p, seed, _p(seed_t), offset, out.data_ptr(), stats.data_ptr(), _p(ws), dt)
     return out, stats
 
 
@@ -526,27 +545,28 @@ class _GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, x1, gamma, beta, seed_t, eps, act, groups, p, seed, offset):
         out, stats = _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset)
         ctx.save_for_backward(x, x1, gamma, beta, stats, seed_t)
-        ctx.args = (act, groups, p, seed, offset)
+        ctx.args = (act, groups, p, seed, offset) + ctx.needs_input_grad[:4]
         return out
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
         x, x1, gamma, beta, stats, seed_t = ctx.saved_tensors
-        act, groups, p, seed, offset = ctx.args
+        act, groups, p, seed, offset, need_x, need_x1, need_g, need_b = ctx.args
         b, hw, c0, c1 = _gn_sizes(x, x1)
-        dt = dtype_code(x.dtype)
-        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        dt = _CODES[x.dtype]
         dy = dy.contiguous()
-        dx = torch.empty_like(x) if need_x else None
-        dx1 = torch.empty_like(x1) if need_x and x1 is not None else None
-        dgamma = torch.empty_like(gamma) if ctx.needs_input_grad[2] else None
-        dbeta = torch.empty_like(beta) if ctx.needs_input_grad[3] else None
-        ws = _workspace(_lib.lib().sdmi_groupnorm_act_workspace_bytes(b, hw, c0, c1, groups, dt, 1), x.device)
-        _run(x.device, "sdmi_groupnorm_act_backward", _p(dy), _p(x), c0, _p(x1), c1, b, hw, groups, _p(gamma), _p(beta),
-             _p(stats), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1), _p(dgamma), _p(dbeta), _p(ws), dt)
-        return (dx if ctx.needs_input_grad[0] else None, dx1 if ctx.needs_input_grad[1] else None, dgamma, dbeta,
-                None, None, None, None, None, None, None)
+        dx = dx1 = None
+        if need_x or need_x1:
+            dx = torch.empty_like(x)
+            dx1 = None if x1 is None else torch.empty_like(x1)
+        dgamma = torch.empty_like(gamma) if need_g else None
+        dbeta = torch.empty_like(beta) if need_b else None
+        ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 1), x)
+        _run(x.get_device(), "sdmi_groupnorm_act_backward", dy.data_ptr(), x.data_ptr(), c0, _p(x1), c1, b, hw, groups,
+             gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1),
+             _p(dgamma), _p(dbeta), _p(ws), dt)
+        return (dx if need_x else None, dx1 if need_x1 else None, dgamma, dbeta, None, None, None, None, None, None, None)
 
 
 def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.0, seed=None, offset=0):
@@ -562,7 +582,7 @@ def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.
         raise ValueError(f"x {tuple(x.shape)} has no batch and channel dimension")
     c = x.shape[-1]
     if x1 is not None:
-        _check_like("x1", x1, x.device, x.dtype, tuple(x.shape[:-1]) + (x1.shape[-1] if x1.dim() else 0,))
+        _check_like("x1", x1, x.device, x.dtype, x.shape[:-1] + (x1.shape[-1] if x1.dim() else 0,))
         c += x1.shape[-1]
         x1 = x1.contiguous() if x1.shape[-1] else None
     groups = int(groups)
