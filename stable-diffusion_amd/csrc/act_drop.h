@@ -57,13 +57,19 @@ __device__ __forceinline__ Keep8 philox8(unsigned k0, unsigned k1, unsigned col8
   }
   return Keep8{{c0, c1, c2, c3}};
 }
-// dropped elements are zero whatever they held (infinities and NaN included)
+// whether column e (of 8) is kept: the high half compares in place, the low one shifted up; thr16 = thr << 16 (thr < 65536)
+__device__ __forceinline__ bool keeps(const Keep8& k, int e, unsigned thr16) {
+  return ((e & 1) ? k.w[e >> 1] : k.w[e >> 1] << 16) >= thr16;
+}
+// dropped elements are zero whatever they held (infinities and NaN included); thr = 65536 keeps none
 __device__ __forceinline__ void drop8(float (&v)[8], const Keep8& k, unsigned thr, float scale) {
+  if (thr > 65535u) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const unsigned num = (e & 1) ? k.w[e >> 1] >> 16 : k.w[e >> 1] & 0xFFFFu;
-    v[e] = num >= thr ? v[e] * scale : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    return;
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = keeps(k, e, thr << 16) ? v[e] * scale : 0.f;
 }
 
 // ---- activations ---------------------------------------------------------------------------------
@@ -96,27 +102,37 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float z, float
     return z < 0.f ? q : 1.f - q;
   }
 }
-// x g with x -> -inf, g -> 0 would be NaN where the limit is 0: a value this low has no weight left
-template <typename T> __device__ __forceinline__ float act_f(float z, int act) {
-  if (act == ACT_SILU) { return z < -1e4f ? 0.f : z * sigmoid_for<T>(z); }
-  if (act == ACT_GELU) { return z < -1e4f ? 0.f : z * normal_cdf<T>(z, nullptr); }
-  if (act == ACT_QUICK_GELU) { return z < -1e4f ? 0.f : z * sigmoid_for<T>(1.702f * z); }
-  return z;
-}
-template <typename T> __device__ __forceinline__ float act_grad(float z, int act) {
-  if (act == ACT_NONE) return 1.f;
-  const float zc = fminf(fmaxf(z, -1e4f), 1e4f);     // keeps z * 0 a number; NaN is put back below
-  float g;
+// z g with z -> -inf, g -> 0 would be NaN where the limit is 0: the factor z stops at -1e4, where g has long been 0 (the
+// gate still sees z itself, so a NaN stays one)
+template <typename T, int N> __device__ __forceinline__ void act_n(float (&z)[N], int act) {
+  if (act == ACT_NONE) return;
   if (act == ACT_GELU) {
-    float pdf;
-    const float cdf = normal_cdf<T>(zc, &pdf);
-    g = fmaf(zc, pdf, cdf);
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] = fmaxf(z[e], -1e4f) * normal_cdf<T>(z[e], nullptr);
   } else {
     const float a = act == ACT_QUICK_GELU ? 1.702f : 1.f;
-    const float s = sigmoid_for<T>(a * zc);
-    g = fmaf(a * zc * s, 1.f - s, s);
+#pragma unroll
+    for (int e = 0; e < N; ++e) z[e] = fmaxf(z[e], -1e4f) * sigmoid_for<T>(a * z[e]);
   }
-  return z != z ? z : g;
+}
+// g[e] *= act'(z[e])
+template <typename T, int N> __device__ __forceinline__ void act_grad_n(const float (&z)[N], float (&g)[N], int act) {
+  if (act == ACT_NONE) return;
+  if (act == ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      float pdf;
+      const float cdf = normal_cdf<T>(z[e], &pdf);
+      g[e] *= fmaf(__builtin_amdgcn_fmed3f(z[e], -1e4f, 1e4f), pdf, cdf);
+    }
+  } else {
+    const float a = act == ACT_QUICK_GELU ? 1.702f : 1.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float s = sigmoid_for<T>(a * z[e]);
+      g[e] *= fmaf(a * __builtin_amdgcn_fmed3f(z[e], -1e4f, 1e4f) * s, 1.f - s, s);
+    }
+  }
 }
 
 // ---- eight columns of a row ------------------------------------------------------------------------

@@ -113,6 +113,19 @@ template <typename T> __device__ __forceinline__ float first_of(const GnaParams&
   return c < p.c0 ? to_f32<T>(((const T*)p.x0)[row * p.c0 + c]) : to_f32<T>(((const T*)p.x1)[row * p.c1 + (c - p.c0)]);
 }
 
+// W columns from c on, that do not leave their group of eight
+template <int W>
+__device__ __forceinline__ void drop_n(const DropArgs& d, unsigned k0, unsigned k1, int64_t row, int c, float (&v)[W]) {
+  if (!d.thr) return;
+  const Keep8 k = philox8(k0, k1, (unsigned)c >> 3, (uint64_t)row, d.offset);
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    const int ce = (c & (8 - W)) + e;
+    const unsigned wd = ce < 4 ? (ce < 2 ? k.w[0] : k.w[1]) : (ce < 6 ? k.w[2] : k.w[3]);
+    v[e] = ((ce & 1) ? wd >> 16 : wd & 0xFFFFu) >= d.thr ? v[e] * d.scale : 0.f;
+  }
+}
+
 // ---- one workgroup per (sample, group) ---------------------------------------------------------------
 __device__ __forceinline__ float block_sum(float v, float* red) {       // red: 16 floats; same value on every thread
   v = wave_sum(v);
@@ -173,16 +186,9 @@ __global__ __launch_bounds__(1024) void gna_slice_fwd_kernel(GnaParams p) {
     float v[W];
     load_n<T, W>(xs + i * W, v);
 #pragma unroll
-    for (int e = 0; e < W; ++e) v[e] = act_f<T>(fmaf(v[e] - mean, rstd * p.gamma[c + e], p.beta[c + e]), p.act);
-    if (p.drop.thr) {
-      const Keep8 k = philox8(k0, k1, (unsigned)c >> 3, (uint64_t)row, p.drop.offset);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        const int ce = (c + e) & 7;
-        const unsigned wd = ce < 4 ? (ce < 2 ? k.w[0] : k.w[1]) : (ce < 6 ? k.w[2] : k.w[3]);
-        v[e] = ((ce & 1) ? wd >> 16 : wd & 0xFFFFu) >= p.drop.thr ? v[e] * p.drop.scale : 0.f;
-      }
-    }
+    for (int e = 0; e < W; ++e) v[e] = fmaf(v[e] - mean, rstd * p.gamma[c + e], p.beta[c + e]);
+    act_n<T>(v, p.act);
+    drop_n<W>(p.drop, k0, k1, row, c, v);
     store_n<T, W>((T*)p.out0 + row * p.C + c, v);
   }
 }
@@ -191,23 +197,15 @@ __global__ __launch_bounds__(1024) void gna_slice_fwd_kernel(GnaParams p) {
 template <typename T, int W>
 __device__ __forceinline__ void grad_u(const GnaParams& p, unsigned k0, unsigned k1, int64_t row, int c, float mean, float rstd,
                                        const float (&x)[W], const float (&dy)[W], float (&xh)[W], float (&du)[W]) {
-  unsigned num[W];
-  if (p.drop.thr) {
-    const Keep8 k = philox8(k0, k1, (unsigned)c >> 3, (uint64_t)row, p.drop.offset);
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      const int ce = (c + e) & 7;
-      const unsigned wd = ce < 4 ? (ce < 2 ? k.w[0] : k.w[1]) : (ce < 6 ? k.w[2] : k.w[3]);
-      num[e] = (ce & 1) ? wd >> 16 : wd & 0xFFFFu;
-    }
-  }
+  float u[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     xh[e] = (x[e] - mean) * rstd;
-    float t = dy[e];
-    if (p.drop.thr) t = num[e] >= p.drop.thr ? t * p.drop.scale : 0.f;
-    du[e] = t * act_grad<T>(fmaf(xh[e], p.gamma[c + e], p.beta[c + e]), p.act);
+    u[e] = fmaf(xh[e], p.gamma[c + e], p.beta[c + e]);
+    du[e] = dy[e];
   }
+  drop_n<W>(p.drop, k0, k1, row, c, du);
+  act_grad_n<T>(u, du, p.act);
 }
 
 // Backward of a slice: x and du in LDS.  Channel sums: a thread keeps one vector column (blockDim is a multiple of
@@ -381,15 +379,14 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
     double a = 0.0, q = 0.0;
     if (g < p.G) {
       const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.strips * p.G + g;
-      int s = j;
-      for (; s + 7 * tpg < p.strips; s += 8 * tpg) {         // eight loads in flight
+      for (int s0 = j; s0 < p.strips; s0 += 8 * tpg) {       // eight loads in flight, the ones beyond the end count nothing
         float2 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(s + u * tpg) * p.G];
+        for (int u = 0; u < 8; ++u) v[u] = src[(size_t)min(s0 + u * tpg, p.strips - 1) * p.G];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) { a += (double)v[u].x; q += (double)v[u].y; }
+        for (int u = 0; u < 8; ++u)
+          if (s0 + u * tpg < p.strips) { a += (double)v[u].x; q += (double)v[u].y; }
       }
-      for (; s < p.strips; s += tpg) { const float2 v = src[(size_t)s * p.G]; a += (double)v.x; q += (double)v.y; }
     }
     a = fold_lanes(a, tpg);
     q = fold_lanes(q, tpg);
@@ -397,8 +394,9 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void gna_apply_kernel(GnaParams p) {
+template <typename T, int ACT, bool DROP>
+__global__ __launch_bounds__(256, 5) void gna_apply_kernel(GnaParams p) {
+  const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   float* s_mean = reinterpret_cast<float*>(smem);
   float* s_rstd = s_mean + p.G;
@@ -439,8 +437,9 @@ __global__ __launch_bounds__(256) void gna_apply_kernel(GnaParams p) {
         const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = act_f<T>(fmaf(to_f32<T>(r[u][e]) - mn[e], sc[e], bt[e]), p.act);
-        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(to_f32<T>(r[u][e]) - mn[e], sc[e], bt[e]);
+        act_n<T>(v, act);
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
         store8<T>((T*)p.out0 + row * p.C + c, p.C - c, v);
       }
     }
@@ -448,8 +447,9 @@ __global__ __launch_bounds__(256) void gna_apply_kernel(GnaParams p) {
 }
 
 // backward, first launch: channel sums of du and du xh over the strip, and the group sums of gamma times them
-template <typename T>
-__global__ __launch_bounds__(256) void gna_grad_sums_kernel(GnaParams p) {
+template <typename T, int ACT, bool DROP>
+__global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
+  const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
   const Walk w = walk_of(p, strip);
@@ -461,13 +461,16 @@ __global__ __launch_bounds__(256) void gna_grad_sums_kernel(GnaParams p) {
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
     const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c);
-    float mn[8], rs[8], ga[8], bt[8], s[8], q[8];
-    load_params(p.gamma, c, p.C, ga);
+    // u = (x - mean) sc + beta with sc = rstd gamma; the sums take (x - mean) and the unscaled mask, rstd and the
+    // dropout's scale come in at the end
+    float mn[8], rs[8], sc[8], bt[8], s[8], q[8];
+    load_params(p.gamma, c, p.C, sc);
     load_params(p.beta, c, p.C, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float* st = p.stats + ((size_t)b * p.G + (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg)) * 2;
       mn[e] = st[0]; rs[e] = st[1];
+      sc[e] *= rs[e];
       s[e] = 0.f; q[e] = 0.f;
     }
     for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
@@ -481,19 +484,22 @@ __global__ __launch_bounds__(256) void gna_grad_sums_kernel(GnaParams p) {
       for (int u = 0; u < WALK_BWD; ++u) {
         if (px + u * w.lanes >= w.pe) break;
         const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(rd[u][e]);
-        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+        float v[8], d[8], z[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float xh = (to_f32<T>(rx[u][e]) - mn[e]) * rs[e];
-          const float du = v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
-          s[e] += du;
-          q[e] = fmaf(du, xh, q[e]);
+          v[e] = to_f32<T>(rd[u][e]);
+          d[e] = to_f32<T>(rx[u][e]) - mn[e];
+          z[e] = fmaf(d[e], sc[e], bt[e]);
         }
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, 1.f);
+        act_grad_n<T>(z, v, act);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { s[e] += v[e]; q[e] = fmaf(v[e], d[e], q[e]); }
       }
     }
+    const float ds = DROP ? p.drop.scale : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { s[e] *= ds; q[e] *= ds * rs[e]; }
 #pragma unroll
     for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
   }
@@ -543,8 +549,9 @@ __global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int
 }
 
 // backward, second launch: dx; the blocks behind the strips' fold dgamma and dbeta
-template <typename T>
-__global__ __launch_bounds__(256) void gna_grad_apply_kernel(GnaParams p) {
+template <typename T, int ACT, bool DROP>
+__global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
+  const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   if ((int)blockIdx.x >= p.apply_blocks) {
     if (blockIdx.y == 0)
@@ -565,16 +572,19 @@ __global__ __launch_bounds__(256) void gna_grad_apply_kernel(GnaParams p) {
   for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
     const int c = cg * 8;
     const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c), dx(p.out0, p.out1, p.c0, p.c1, c);
-    float mn[8], rs[8], ga[8], bt[8], ma[8], mq[8];
-    load_params(p.gamma, c, p.C, ga);
+    // dx = rstd (h - a - xh q) = sc du - (rstd a + (x - mean) rstd^2 q)
+    float mn[8], sc[8], bt[8], ka[8], kq[8];
+    load_params(p.gamma, c, p.C, sc);
     load_params(p.beta, c, p.C, bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int g = (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg);
       const float* st = p.stats + ((size_t)b * p.G + g) * 2;
-      mn[e] = st[0]; rs[e] = st[1];
-      ma[e] = s_a[g]; mq[e] = s_q[g];
+      const float rs = st[1];
+      mn[e] = st[0]; sc[e] *= rs;
+      ka[e] = rs * s_a[g]; kq[e] = rs * rs * s_q[g];
     }
+    const float ds = DROP ? p.drop.scale : 1.f;
     for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
       typename Cols<T>::Raw rx[WALK_BWD], rd[WALK_BWD];
 #pragma unroll
@@ -586,16 +596,17 @@ __global__ __launch_bounds__(256) void gna_grad_apply_kernel(GnaParams p) {
       for (int u = 0; u < WALK_BWD; ++u) {
         if (px + u * w.lanes >= w.pe) break;
         const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = to_f32<T>(rd[u][e]);
-        if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
+        float v[8], d[8], z[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float xh = (to_f32<T>(rx[u][e]) - mn[e]) * rs[e];
-          const float h = ga[e] * v[e] * act_grad<T>(fmaf(xh, ga[e], bt[e]), p.act);
-          v[e] = rs[e] * (h - ma[e] - xh * mq[e]);
+          v[e] = to_f32<T>(rd[u][e]);
+          d[e] = to_f32<T>(rx[u][e]) - mn[e];
+          z[e] = fmaf(d[e], sc[e], bt[e]);
         }
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, ds);
+        act_grad_n<T>(z, v, act);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(sc[e], v[e], -fmaf(d[e], kq[e], ka[e]));
         dx.store(row, v);
       }
     }
@@ -675,6 +686,21 @@ int slice_threads(const GnaPlan& pl, const GnaParams& p) {
   return t;
 }
 
+// the kernels over strips with the activation (SiLU and none; the others by a branch) and dropout compiled in
+#define GNA_LAUNCH(K, A, D, GRID, LDS) hipLaunchKernelGGL((K<T, A, D>), GRID, dim3(256), LDS, s, p)
+#define GNA_VARIANTS(K, GRID, LDS)                                                   \
+  {                                                                                  \
+    if (p.drop.thr) {                                                                \
+      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, true, GRID, LDS);               \
+      else if (p.act == ACT_NONE) GNA_LAUNCH(K, ACT_NONE, true, GRID, LDS);          \
+      else GNA_LAUNCH(K, -1, true, GRID, LDS);                                       \
+    } else {                                                                         \
+      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, false, GRID, LDS);              \
+      else if (p.act == ACT_NONE) GNA_LAUNCH(K, ACT_NONE, false, GRID, LDS);         \
+      else GNA_LAUNCH(K, -1, false, GRID, LDS);                                      \
+    }                                                                                \
+  }
+
 template <typename T>
 int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
   GnaParams p = gna_params(a, pl, drop);
@@ -691,7 +717,7 @@ int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
   } else {
     const dim3 grid(pl.strips, p.B);
     hipLaunchKernelGGL(gna_stats_kernel<T>, grid, dim3(256), pl.lds, s, p);
-    hipLaunchKernelGGL(gna_apply_kernel<T>, grid, dim3(256), 2 * p.G * 4, s, p);
+    GNA_VARIANTS(gna_apply_kernel, grid, 2 * p.G * 4)
   }
   SDMI_CHECK_HIP(hipGetLastError());
   return SDMI_OK;
@@ -714,11 +740,10 @@ int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
     else hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 1>), grid, block, pl.lds, s, p);
     if (weights && p.B > 1) hipLaunchKernelGGL(gna_fold_channels_kernel, dim3(fold_blocks), dim3(256), 0, s, p, (int64_t)p.B);
   } else {
-    hipLaunchKernelGGL(gna_grad_sums_kernel<T>, dim3(pl.strips, p.B), dim3(256), pl.lds, s, p);
+    GNA_VARIANTS(gna_grad_sums_kernel, dim3(pl.strips, p.B), pl.lds)
     p.apply_blocks = (a.dx0 || a.dx1) ? pl.strips : 0;
     const int lds = 2 * p.G * 4 > 2048 ? 2 * p.G * 4 : 2048;
-    if (p.apply_blocks + fold_blocks)
-      hipLaunchKernelGGL(gna_grad_apply_kernel<T>, dim3(p.apply_blocks + fold_blocks, p.B), dim3(256), lds, s, p);
+    if (p.apply_blocks + fold_blocks) GNA_VARIANTS(gna_grad_apply_kernel, dim3(p.apply_blocks + fold_blocks, p.B), lds)
   }
   SDMI_CHECK_HIP(hipGetLastError());
   return SDMI_OK;

@@ -69,10 +69,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, unsigned k0, unsigned
     for (int i = 0; i < 8; ++i) v[i] += b[i];
   }
   if (e.preact) store8<float>(e.preact + m * e.N + n, cnt, v);
-  if (e.act != ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = act_f<T>(v[i], e.act);
-  }
+  act_n<T>(v, e.act);
   if (e.drop.thr) drop8(v, philox8(k0, k1, (unsigned)n >> 3, (uint64_t)m, e.drop.offset), e.drop.thr, e.drop.scale);
   if (e.resid) {
 #pragma unroll
@@ -573,10 +570,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
         const int64_t m = m0 + u * lanes;
         if (m >= re) break;
         if (p.drop.thr) drop8(v[u], philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
-        if (p.act != ACT_NONE) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] *= act_grad<T>(z[u][e], p.act);
-        }
+        act_grad_n<T>(z[u], v[u], p.act);
         if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v[u]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] += v[u][e];
