@@ -42,6 +42,9 @@ __device__ __forceinline__ void drop_key(const DropArgs& d, unsigned& k0, unsign
   if (d.seed_dev) { k0 = d.seed_dev[0]; k1 = d.seed_dev[1]; }
 }
 
+__device__ __forceinline__ unsigned xor3(unsigned a, unsigned b, unsigned c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
 struct Keep8 { unsigned w[4]; };     // 16-bit number of column e: half (e & 1) of word e / 2
 
 __device__ __forceinline__ Keep8 philox8(unsigned k0, unsigned k1, unsigned col8, uint64_t row, unsigned offset) {
@@ -49,8 +52,8 @@ __device__ __forceinline__ Keep8 philox8(unsigned k0, unsigned k1, unsigned col8
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
-    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+    c0 = xor3((unsigned)(b >> 32), c1, k0);
+    c2 = xor3((unsigned)(a >> 32), c3, k1);
     c1 = (unsigned)b;
     c3 = (unsigned)a;
     k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;

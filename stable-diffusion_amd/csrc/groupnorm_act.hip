@@ -61,42 +61,48 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[W]) {
     *reinterpret_cast<V*>(p) = r;
   }
 }
-// Eight columns of a two-source row that a thread walks down: where they lie and how many there are.  Whole groups of one
-// source are 16-byte pieces (32 in fp32) that stay packed until they are used; a row's short last group, and one that
-// straddles the sources, go element by element.
-template <typename T> struct Cols {
+// Eight columns of a two-source tensor that a thread walks down, from row `row0` on.  WHOLE: all groups of eight lie in one
+// source, 16-byte pieces (32 in fp32) that stay packed until they are used; otherwise a row's short last group and one
+// that straddles the sources go element by element.
+template <typename T, bool WHOLE> struct Cols;
+template <typename T> struct Cols<T, true> {
   typedef T Raw __attribute__((ext_vector_type(8)));
-  typedef typename Vec8u<T>::type RawU;
-  const T* p0; const T* p1;       // element 0 of row 0 in each source (the columns' own offset included)
+  char* p;
+  unsigned step;                  // bytes from row to row
+  __device__ __forceinline__ Cols(const void* x0, const void* x1, int c0, int c1, int c, int64_t row0) {
+    const bool second = c >= c0;
+    step = (unsigned)(second ? c1 : c0) * (unsigned)sizeof(T);
+    p = (char*)(second ? x1 : x0) + row0 * step + (second ? c - c0 : c) * (int)sizeof(T);
+  }
+  __device__ __forceinline__ Raw load(int r) const {
+    return *reinterpret_cast<const typename Vec8u<T>::type*>(p + (unsigned)r * step);
+  }
+  __device__ __forceinline__ void store(int r, const float (&v)[8]) const {
+    store8<T>(reinterpret_cast<T*>(p + (unsigned)r * step), 8, v);
+  }
+};
+template <typename T> struct Cols<T, false> {
+  typedef T Raw __attribute__((ext_vector_type(8)));
+  T* p0; T* p1;                   // element 0 of row row0 in each source (the columns' own offset included)
   int c0, c1, n0, n;              // row strides; elements in the first source, in both
-  bool whole;
-  __device__ __forceinline__ Cols(const void* x0, const void* x1, int c0_, int c1_, int c) : c0(c0_), c1(c1_) {
+  __device__ __forceinline__ Cols(const void* x0, const void* x1, int c0_, int c1_, int c, int64_t row0) : c0(c0_), c1(c1_) {
     const int left = c0 - c, all = c0 + c1 - c;
     n0 = left < 0 ? 0 : (left < 8 ? left : 8);
     n = all < 8 ? all : 8;
-    p0 = (const T*)x0 + c;
-    p1 = (const T*)x1 - left;
-    whole = n0 == 8 || (n0 == 0 && n == 8);
+    p0 = (T*)x0 + row0 * c0 + c;
+    p1 = (T*)x1 + row0 * c1 - left;
   }
-  __device__ __forceinline__ Raw load(int64_t row) const {
-    Raw r;
-    if (whole) {
-      r = *reinterpret_cast<const RawU*>(n0 ? p0 + row * c0 : p1 + row * c1);
-    } else {
+  __device__ __forceinline__ Raw load(int64_t r) const {
+    Raw v;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = e < n0 ? p0[row * c0 + e] : (e < n ? p1[row * c1 + e] : (T)0.f);
-    }
-    return r;
+    for (int e = 0; e < 8; ++e) v[e] = e < n0 ? p0[r * c0 + e] : (e < n ? p1[r * c1 + e] : (T)0.f);
+    return v;
   }
-  __device__ __forceinline__ void store(int64_t row, const float (&v)[8]) const {
-    if (whole) {
-      store8<T>(const_cast<T*>(n0 ? p0 + row * c0 : p1 + row * c1), 8, v);
-    } else {
+  __device__ __forceinline__ void store(int64_t r, const float (&v)[8]) const {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (e < n0) const_cast<T*>(p0)[row * c0 + e] = from_f32<T>(v[e]);
-        else if (e < n) const_cast<T*>(p1)[row * c1 + e] = from_f32<T>(v[e]);
-      }
+    for (int e = 0; e < 8; ++e) {
+      if (e < n0) p0[r * c0 + e] = from_f32<T>(v[e]);
+      else if (e < n) p1[r * c1 + e] = from_f32<T>(v[e]);
     }
   }
 };
@@ -288,19 +294,26 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
 // A thread owns one group of eight columns and walks every lanes-th pixel of its strip; tensors of more than 2048
 // channels make a thread take several column groups, one after the other.
 constexpr int WALK = 4, WALK_BWD = 2;      // pixels a thread has in flight
-struct Walk { int ncg, lanes, pl, cg0, cgs; int64_t pb, pe; };
-__device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip) {
+struct Walk { int ncg, lanes, pl, cg0, count; int64_t row0; };      // count pixels from row row0 on
+constexpr int WALK_CGS = 256;
+__device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip, int b) {
   Walk w;
   w.ncg = (p.C + 7) >> 3;
   const bool fits = w.ncg <= 256;
   w.lanes = fits ? 256 / w.ncg : 1;
   w.pl = fits ? (int)threadIdx.x / w.ncg : 0;
   w.cg0 = fits ? (int)threadIdx.x - w.pl * w.ncg : (int)threadIdx.x;
-  w.cgs = 256;
   if (w.pl >= w.lanes) w.cg0 = w.ncg;                    // threads left over
-  w.pb = (int64_t)strip * p.px_per_strip;
-  w.pe = w.pb + p.px_per_strip < p.HW ? w.pb + p.px_per_strip : p.HW;
+  const int64_t pb = (int64_t)strip * p.px_per_strip, left = p.HW - pb;
+  w.count = (int)(left < p.px_per_strip ? left : p.px_per_strip);
+  w.row0 = (int64_t)b * p.HW + pb;
   return w;
+}
+// the pixels px, px + lanes, ... of a walk (beyond the strip its last one again, which the caller does not count)
+template <typename C, int N>
+__device__ __forceinline__ void fetch(const C& x, const Walk& w, int px, typename C::Raw (&r)[N]) {
+#pragma unroll
+  for (int u = 0; u < N; ++u) r[u] = x.load(min(px + u * w.lanes, w.count - 1));
 }
 // threads per group for folds over the groups: a power of two, at most a wave
 __device__ __forceinline__ int threads_per_group(int G) {
@@ -323,17 +336,18 @@ __device__ __forceinline__ void fold_pixel_lanes(float* s1, float* s2, int lanes
   __syncthreads();
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
-  const Walk w = walk_of(p, strip);
+  const Walk w = walk_of(p, strip, b);
+  typedef Cols<T, WHOLE> C;
   const int width = w.ncg * 8;
   float* s1 = reinterpret_cast<float*>(smem);
   float* s2 = s1 + w.lanes * width;
-  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
     const int c = cg * 8;
-    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c);
+    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
     float sh[8], s[8], q[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -341,13 +355,12 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
       sh[e] = first_of<T>(p, b, (int)div_by((unsigned)ce, p.div_cpg) * p.cpg);
       s[e] = 0.f; q[e] = 0.f;
     }
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK * w.lanes) {
-      typename Cols<T>::Raw r[WALK];
-#pragma unroll
-      for (int u = 0; u < WALK; ++u) r[u] = x.load((int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1));
+    for (int px = w.pl; px < w.count; px += WALK * w.lanes) {
+      typename C::Raw r[WALK];
+      fetch(x, w, px, r);
 #pragma unroll
       for (int u = 0; u < WALK; ++u) {
-        if (px + u * w.lanes >= w.pe) break;
+        if (px + u * w.lanes >= w.count) break;
 #pragma unroll
         for (int e = 0; e < 8; ++e) { const float t = to_f32<T>(r[u][e]) - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
       }
@@ -394,13 +407,17 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
   }
 }
 
-template <typename T, int ACT, bool DROP>
-__global__ __launch_bounds__(256, 5) void gna_apply_kernel(GnaParams p) {
+template <typename T, int ACT, bool DROP, bool WHOLE>
+__global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   float* s_mean = reinterpret_cast<float*>(smem);
   float* s_rstd = s_mean + p.G;
   const int strip = blockIdx.x, b = blockIdx.y;
+  const Walk w = walk_of(p, strip, b);
+  typedef Cols<T, WHOLE> C;
+  typename C::Raw r[WALK];                     // the first pixels come while the strips' sums are folded
+  if (w.cg0 < w.ncg) fetch(C(p.x0, p.x1, p.c0, p.c1, w.cg0 * 8, w.row0), w, w.pl, r);
   fold_strips(p, b, [&](int g, double a, double q) {
     const double n = (double)p.HW * (double)p.cpg, m = a / n;
     double var = q / n - m * m;
@@ -413,12 +430,12 @@ __global__ __launch_bounds__(256, 5) void gna_apply_kernel(GnaParams p) {
     }
   });
   __syncthreads();
-  const Walk w = walk_of(p, strip);
   unsigned k0 = 0, k1 = 0;
-  if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+  if (DROP) drop_key(p.drop, k0, k1);
+  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
     const int c = cg * 8;
-    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c);
+    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), y(p.out0, p.out0, p.C, 0, c, w.row0);
+    if (cg != w.cg0) fetch(x, w, w.pl, r);
     float mn[8], sc[8], bt[8];
     load_params(p.gamma, c, p.C, sc);
     load_params(p.beta, c, p.C, bt);
@@ -427,40 +444,44 @@ __global__ __launch_bounds__(256, 5) void gna_apply_kernel(GnaParams p) {
       const int g = (int)div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg);
       mn[e] = s_mean[g]; sc[e] *= s_rstd[g];
     }
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK * w.lanes) {
-      typename Cols<T>::Raw r[WALK];
+    for (int px = w.pl; px < w.count; px += WALK * w.lanes) {
+      typename C::Raw now[WALK];
 #pragma unroll
-      for (int u = 0; u < WALK; ++u) r[u] = x.load((int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1));
+      for (int u = 0; u < WALK; ++u) now[u] = r[u];
+      if (px + WALK * w.lanes < w.count) fetch(x, w, px + WALK * w.lanes, r);
 #pragma unroll
       for (int u = 0; u < WALK; ++u) {
-        if (px + u * w.lanes >= w.pe) break;
-        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        if (px + u * w.lanes >= w.count) break;
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf(to_f32<T>(r[u][e]) - mn[e], sc[e], bt[e]);
+        for (int e = 0; e < 8; ++e) v[e] = fmaf(to_f32<T>(now[u][e]) - mn[e], sc[e], bt[e]);
         act_n<T>(v, act);
-        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, p.drop.scale);
-        store8<T>((T*)p.out0 + row * p.C + c, p.C - c, v);
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)(w.row0 + px + u * w.lanes), p.drop.offset), p.drop.thr, p.drop.scale);
+        y.store(px + u * w.lanes, v);
       }
     }
   }
 }
 
 // backward, first launch: channel sums of du and du xh over the strip, and the group sums of gamma times them
-template <typename T, int ACT, bool DROP>
+template <typename T, int ACT, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
-  const Walk w = walk_of(p, strip);
+  const Walk w = walk_of(p, strip, b);
+  typedef Cols<T, WHOLE> C;
   const int width = w.ncg * 8;
   float* s1 = reinterpret_cast<float*>(smem);
   float* s2 = s1 + w.lanes * width;
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
     const int c = cg * 8;
-    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c);
+    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0);
+    typename C::Raw rx[WALK_BWD], rd[WALK_BWD];
+    fetch(x, w, w.pl, rx);
+    fetch(dy, w, w.pl, rd);
     // u = (x - mean) sc + beta with sc = rstd gamma; the sums take (x - mean) and the unscaled mask, rstd and the
     // dropout's scale come in at the end
     float mn[8], rs[8], sc[8], bt[8], s[8], q[8];
@@ -473,22 +494,23 @@ __global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
       sc[e] *= rs[e];
       s[e] = 0.f; q[e] = 0.f;
     }
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
-      typename Cols<T>::Raw rx[WALK_BWD], rd[WALK_BWD];
+    for (int px = w.pl; px < w.count; px += WALK_BWD * w.lanes) {
+      typename C::Raw nx[WALK_BWD], nd[WALK_BWD];
 #pragma unroll
-      for (int u = 0; u < WALK_BWD; ++u) {
-        const int64_t row = (int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1);
-        rx[u] = x.load(row); rd[u] = dy.load(row);
+      for (int u = 0; u < WALK_BWD; ++u) { nx[u] = rx[u]; nd[u] = rd[u]; }
+      if (px + WALK_BWD * w.lanes < w.count) {
+        fetch(x, w, px + WALK_BWD * w.lanes, rx);
+        fetch(dy, w, px + WALK_BWD * w.lanes, rd);
       }
 #pragma unroll
       for (int u = 0; u < WALK_BWD; ++u) {
-        if (px + u * w.lanes >= w.pe) break;
-        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        if (px + u * w.lanes >= w.count) break;
+        const int64_t row = w.row0 + px + u * w.lanes;
         float v[8], d[8], z[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = to_f32<T>(rd[u][e]);
-          d[e] = to_f32<T>(rx[u][e]) - mn[e];
+          v[e] = to_f32<T>(nd[u][e]);
+          d[e] = to_f32<T>(nx[u][e]) - mn[e];
           z[e] = fmaf(d[e], sc[e], bt[e]);
         }
         if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, 1.f);
@@ -549,7 +571,7 @@ __global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int
 }
 
 // backward, second launch: dx; the blocks behind the strips' fold dgamma and dbeta
-template <typename T, int ACT, bool DROP>
+template <typename T, int ACT, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
@@ -561,17 +583,27 @@ __global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
   float* s_a = reinterpret_cast<float*>(smem);
   float* s_q = s_a + p.G;
   const int strip = blockIdx.x, b = blockIdx.y;
+  const Walk w = walk_of(p, strip, b);
+  typedef Cols<T, WHOLE> C;
+  typename C::Raw rx[WALK_BWD], rd[WALK_BWD];
+  if (w.cg0 < w.ncg) {
+    fetch(C(p.x0, p.x1, p.c0, p.c1, w.cg0 * 8, w.row0), w, w.pl, rx);
+    fetch(C(p.dy, p.dy, p.C, 0, w.cg0 * 8, w.row0), w, w.pl, rd);
+  }
   fold_strips(p, b, [&](int g, double a, double q) {
     const double n = (double)p.HW * (double)p.cpg;
     s_a[g] = (float)(a / n); s_q[g] = (float)(q / n);
   });
   __syncthreads();
-  const Walk w = walk_of(p, strip);
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += w.cgs) {
+  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
     const int c = cg * 8;
-    const Cols<T> x(p.x0, p.x1, p.c0, p.c1, c), dy(p.dy, p.dy, p.C, 0, c), dx(p.out0, p.out1, p.c0, p.c1, c);
+    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0), dx(p.out0, p.out1, p.c0, p.c1, c, w.row0);
+    if (cg != w.cg0) {
+      fetch(x, w, w.pl, rx);
+      fetch(dy, w, w.pl, rd);
+    }
     // dx = rstd (h - a - xh q) = sc du - (rstd a + (x - mean) rstd^2 q)
     float mn[8], sc[8], bt[8], ka[8], kq[8];
     load_params(p.gamma, c, p.C, sc);
@@ -585,29 +617,30 @@ __global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
       ka[e] = rs * s_a[g]; kq[e] = rs * rs * s_q[g];
     }
     const float ds = DROP ? p.drop.scale : 1.f;
-    for (int64_t px = w.pb + w.pl; px < w.pe; px += WALK_BWD * w.lanes) {
-      typename Cols<T>::Raw rx[WALK_BWD], rd[WALK_BWD];
+    for (int px = w.pl; px < w.count; px += WALK_BWD * w.lanes) {
+      typename C::Raw nx[WALK_BWD], nd[WALK_BWD];
 #pragma unroll
-      for (int u = 0; u < WALK_BWD; ++u) {
-        const int64_t row = (int64_t)b * p.HW + min(px + u * w.lanes, w.pe - 1);
-        rx[u] = x.load(row); rd[u] = dy.load(row);
+      for (int u = 0; u < WALK_BWD; ++u) { nx[u] = rx[u]; nd[u] = rd[u]; }
+      if (px + WALK_BWD * w.lanes < w.count) {
+        fetch(x, w, px + WALK_BWD * w.lanes, rx);
+        fetch(dy, w, px + WALK_BWD * w.lanes, rd);
       }
 #pragma unroll
       for (int u = 0; u < WALK_BWD; ++u) {
-        if (px + u * w.lanes >= w.pe) break;
-        const int64_t row = (int64_t)b * p.HW + px + u * w.lanes;
+        if (px + u * w.lanes >= w.count) break;
+        const int64_t row = w.row0 + px + u * w.lanes;
         float v[8], d[8], z[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = to_f32<T>(rd[u][e]);
-          d[e] = to_f32<T>(rx[u][e]) - mn[e];
+          v[e] = to_f32<T>(nd[u][e]);
+          d[e] = to_f32<T>(nx[u][e]) - mn[e];
           z[e] = fmaf(d[e], sc[e], bt[e]);
         }
         if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, ds);
         act_grad_n<T>(z, v, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(sc[e], v[e], -fmaf(d[e], kq[e], ka[e]));
-        dx.store(row, v);
+        dx.store(px + u * w.lanes, v);
       }
     }
   }
@@ -663,6 +696,7 @@ int gna_check(const GroupNormActArgs& a, const char* who) {
   SDMI_REQUIRE(a.groups > 0 && C % a.groups == 0, "%s: %lld channels do not split into %d groups", who, (long long)C, a.groups);
   SDMI_REQUIRE(a.eps >= 0.f, "%s: negative eps", who);
   SDMI_REQUIRE(a.act >= 0 && a.act < ACT_COUNT, "%s: unknown activation %d", who, a.act);
+  SDMI_REQUIRE(a.HW < ((int64_t)1 << 38), "%s: %lld pixels a sample are too many", who, (long long)a.HW);
   SDMI_REQUIRE(a.B <= 65535, "%s: batch %d is beyond 65535", who, a.B);
   return SDMI_OK;
 }
@@ -686,20 +720,27 @@ int slice_threads(const GnaPlan& pl, const GnaParams& p) {
   return t;
 }
 
-// the kernels over strips with the activation (SiLU and none; the others by a branch) and dropout compiled in
-#define GNA_LAUNCH(K, A, D, GRID, LDS) hipLaunchKernelGGL((K<T, A, D>), GRID, dim3(256), LDS, s, p)
-#define GNA_VARIANTS(K, GRID, LDS)                                                   \
-  {                                                                                  \
-    if (p.drop.thr) {                                                                \
-      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, true, GRID, LDS);               \
-      else if (p.act == ACT_NONE) GNA_LAUNCH(K, ACT_NONE, true, GRID, LDS);          \
-      else GNA_LAUNCH(K, -1, true, GRID, LDS);                                       \
-    } else {                                                                         \
-      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, false, GRID, LDS);              \
-      else if (p.act == ACT_NONE) GNA_LAUNCH(K, ACT_NONE, false, GRID, LDS);         \
-      else GNA_LAUNCH(K, -1, false, GRID, LDS);                                      \
-    }                                                                                \
+// the kernels over strips with SiLU (others by a branch), dropout and whole column groups compiled in
+#define GNA_LAUNCH(K, A, D, W, GRID, LDS) hipLaunchKernelGGL((K<T, A, D, W>), GRID, dim3(256), LDS, s, p)
+#define GNA_VARIANTS_W(K, W, GRID, LDS)                                   \
+  {                                                                       \
+    if (p.drop.thr) {                                                     \
+      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, true, W, GRID, LDS); \
+      else GNA_LAUNCH(K, -1, true, W, GRID, LDS);                         \
+    } else {                                                              \
+      if (p.act == ACT_SILU) GNA_LAUNCH(K, ACT_SILU, false, W, GRID, LDS);\
+      else GNA_LAUNCH(K, -1, false, W, GRID, LDS);                        \
+    }                                                                     \
   }
+#define GNA_VARIANTS(K, GRID, LDS)                 \
+  {                                                \
+    if (whole) GNA_VARIANTS_W(K, true, GRID, LDS)  \
+    else GNA_VARIANTS_W(K, false, GRID, LDS)       \
+  }
+// whole groups of eight columns in each source, and strips within 2 GiB (offsets of 32 bits)
+bool gna_whole(const GnaParams& p) {
+  return p.c0 % 8 == 0 && p.c1 % 8 == 0 && p.px_per_strip * (int64_t)p.C * 4 < ((int64_t)1 << 31);
+}
 
 template <typename T>
 int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
@@ -716,7 +757,9 @@ int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
     else hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 1>), grid, block, pl.lds, s, p);
   } else {
     const dim3 grid(pl.strips, p.B);
-    hipLaunchKernelGGL(gna_stats_kernel<T>, grid, dim3(256), pl.lds, s, p);
+    const bool whole = gna_whole(p);
+    if (whole) hipLaunchKernelGGL((gna_stats_kernel<T, true>), grid, dim3(256), pl.lds, s, p);
+    else hipLaunchKernelGGL((gna_stats_kernel<T, false>), grid, dim3(256), pl.lds, s, p);
     GNA_VARIANTS(gna_apply_kernel, grid, 2 * p.G * 4)
   }
   SDMI_CHECK_HIP(hipGetLastError());
@@ -740,6 +783,7 @@ int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
     else hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 1>), grid, block, pl.lds, s, p);
     if (weights && p.B > 1) hipLaunchKernelGGL(gna_fold_channels_kernel, dim3(fold_blocks), dim3(256), 0, s, p, (int64_t)p.B);
   } else {
+    const bool whole = gna_whole(p);
     GNA_VARIANTS(gna_grad_sums_kernel, dim3(pl.strips, p.B), pl.lds)
     p.apply_blocks = (a.dx0 || a.dx1) ? pl.strips : 0;
     const int lds = 2 * p.G * 4 > 2048 ? 2 * p.G * 4 : 2048;
