@@ -293,7 +293,8 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
 // ---- strips ------------------------------------------------------------------------------------------
 // A thread owns one group of eight columns and walks every lanes-th pixel of its strip; tensors of more than 2048
 // channels make a thread take several column groups, one after the other.
-constexpr int WALK = 4, WALK_BWD = 2;      // pixels a thread has in flight
+// pixels a thread has in flight while it works on as many: 64 bytes (32 of each tensor backward), what the registers hold
+template <typename T> struct Depth { static constexpr int FWD = 16 / (int)sizeof(T) / 2, BWD = 1; };
 struct Walk { int ncg, lanes, pl, cg0, count; int64_t row0; };      // count pixels from row row0 on
 constexpr int WALK_CGS = 256;
 __device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip, int b) {
@@ -338,6 +339,7 @@ __device__ __forceinline__ void fold_pixel_lanes(float* s1, float* s2, int lanes
 
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
+  constexpr int WALK = Depth<T>::FWD;
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
   const Walk w = walk_of(p, strip, b);
@@ -409,6 +411,7 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
 
 template <typename T, int ACT, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
+  constexpr int WALK = Depth<T>::FWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   float* s_mean = reinterpret_cast<float*>(smem);
@@ -466,6 +469,7 @@ __global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
 // backward, first launch: channel sums of du and du xh over the strip, and the group sums of gamma times them
 template <typename T, int ACT, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
+  constexpr int WALK_BWD = Depth<T>::BWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
@@ -573,6 +577,7 @@ __global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int
 // backward, second launch: dx; the blocks behind the strips' fold dgamma and dbeta
 template <typename T, int ACT, bool DROP, bool WHOLE>
 __global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
+  constexpr int WALK_BWD = Depth<T>::BWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
   if ((int)blockIdx.x >= p.apply_blocks) {
