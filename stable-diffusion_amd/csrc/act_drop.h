@@ -76,16 +76,22 @@ __device__ __forceinline__ void drop8(float (&v)[8], const Keep8& k, unsigned th
 }
 
 // ---- activations ---------------------------------------------------------------------------------
-// fp32 tensors take the library functions; 16-bit ones the hardware exponential (relative error a few 2^-23, times
+// fp32 tensors take the library functions, or (sigmoid) as good as those; 16-bit ones the hardware exponential (relative error a few 2^-23, times
 // the exponent's size) and, for the normal distribution function of GELU, Abramowitz & Stegun 7.1.26
 // (|error| <= 1.5e-7), whose exponential also gives the density that the derivative needs.
-template <typename T> __device__ __forceinline__ float exp_for(float x) {
-  if constexpr (sizeof(T) == 4) return expf(x); else return __expf(x);
-}
-// e^-x reaches infinity below x = -88, where x / (1 + e^-x) is -0: the reciprocal of infinity is 0
+// e^-x reaches infinity below x = -88, where the reciprocal is 0
 template <typename T> __device__ __forceinline__ float sigmoid_for(float x) {
-  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
-  else return __builtin_amdgcn_rcpf(1.f + __expf(-x));
+  if constexpr (sizeof(T) == 4) {
+    // e^-x as 2^t (1 + r ln 2) with t + r = -x log2 e, r what the product's rounding and the constant's lose: an ulp or two
+    // for a handful of instructions.  x stops at +-88 (t and 2^t finite); a NaN passes through the selects
+    const float lo = x < -88.f ? -88.f : x, y = lo > 88.f ? 88.f : lo;
+    const float t = -y * 1.44269502162933349609375f;
+    const float r = fmaf(-y, 1.925963033500011e-08f, fmaf(-y, 1.44269502162933349609375f, -t));
+    const float p = __builtin_amdgcn_exp2f(t);
+    return __builtin_amdgcn_rcpf(1.f + fmaf(p, r * 0.693147182464599609375f, p));
+  } else {
+    return __builtin_amdgcn_rcpf(1.f + __expf(-x));
+  }
 }
 // Phi(z) and, on demand, the density phi(z)
 template <typename T> __device__ __forceinline__ float normal_cdf(float z, float* pdf) {

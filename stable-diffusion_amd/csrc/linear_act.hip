@@ -79,12 +79,44 @@ __device__ __forceinline__ void finish8(const Epilogue& e, unsigned k0, unsigned
 }
 
 // ---- the product -----------------------------------------------------------------------------------
+// Column sums of the bias gradient's strips; rides on the launch of a product, in blocks behind its own.
+struct DbFold { const float* partial = nullptr; int strips = 0, n = 0; float* db = nullptr; };
+constexpr int DB_COLS = 16;          // columns a block folds, by 16 lanes each
+__device__ __forceinline__ void fold_bias_gradient(const DbFold& f, int block, float* red) {
+  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, n = block * DB_COLS + cl;
+  float s = 0.f;
+  if (n < f.n && rl < 16) {
+    const float* src = f.partial + n;
+    int i = rl;
+    for (; i + 48 < f.strips; i += 64) {
+      const float a = src[(size_t)i * f.n], b = src[(size_t)(i + 16) * f.n], c = src[(size_t)(i + 32) * f.n],
+                  d = src[(size_t)(i + 48) * f.n];
+      s += (a + b) + (c + d);
+    }
+    for (; i < f.strips; i += 16) s += src[(size_t)i * f.n];
+  }
+  if (rl < 16) red[rl * 16 + cl] = s;
+  __syncthreads();
+  if (rl == 0 && n < f.n) {
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s += red[r * 16 + cl];
+    f.db[n] = s;
+  }
+}
+__global__ __launch_bounds__(256) void linear_db_kernel(DbFold f) {
+  __shared__ float red[256];
+  fold_bias_gradient(f, (int)blockIdx.x, red);
+}
+
 struct GemmParams {
   const char* q; const char* p;      // operands
+  const char* q2;                    // not null: a second Q, multiplied with the same P and added (low parts of Q)
   int64_t ldq, ldp;                  // elements from one stored row to the next
   int64_t K, k_per_split;            // contraction; a split's share is a multiple of the K-tile
   unsigned tiles_n, tiles, splits;
   float* partial;                    // [splits][M][N] fp32, or null: the kernel finishes the rows itself
+  DbFold fold;
   Epilogue e;
 };
 
@@ -177,6 +209,10 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
 
   // workgroup -> (split, tile): ids go round-robin over the 8 XCDs, so each XCD takes a contiguous run; column tiles
   // of one row block are neighbours and share its Q tile in the XCD's L2
+  if (blockIdx.x >= p.tiles * p.splits) {
+    fold_bias_gradient(p.fold, (int)(blockIdx.x - p.tiles * p.splits), reinterpret_cast<float*>(smem));
+    return;
+  }
   const unsigned total = p.tiles * p.splits, xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
   const unsigned id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
   const unsigned split = id / p.tiles, tile = id - split * p.tiles;
@@ -185,12 +221,14 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   const int n0 = (int)tn * BN;
   const int64_t kb = (int64_t)split * p.k_per_split;
   const int64_t ke = kb + p.k_per_split < p.K ? kb + p.k_per_split : p.K;
-  const int nk = (int)((ke - kb + KT - 1) / KT);
+  const int nk1 = (int)((ke - kb + KT - 1) / KT), nk = p.q2 ? 2 * nk1 : nk1;
 
   // Per-thread chunk sources: offsets from a uniform base that moves with the K-tile.  Output rows beyond the end repeat
   // the last ones (their results are not stored).  Chunk i of a thread lies i * NT chunks behind its first one.
-  const char* baseq = p.q + (QC ? kb * p.ldq + m0 : m0 * p.ldq + kb) * SZ;
-  const char* basep = p.p + (PC ? kb * p.ldp + n0 : (int64_t)n0 * p.ldp + kb) * SZ;
+  const int64_t startq = (QC ? kb * p.ldq + m0 : m0 * p.ldq + kb) * SZ;
+  const int64_t startp = (PC ? kb * p.ldp + n0 : (int64_t)n0 * p.ldp + kb) * SZ;
+  const char* baseq = p.q + startq;
+  const char* basep = p.p + startp;
   const int64_t stepq = QC ? (int64_t)KT * p.ldq * SZ : 128, stepp = PC ? (int64_t)KT * p.ldp * SZ : 128;
   const int64_t leftq = p.e.M - m0, leftp = (int64_t)p.e.N - n0;      // output rows / columns from this tile on
   auto place = [&](int i, bool isq, int& a, int& c) {
@@ -212,7 +250,8 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
 
   u32x4 reg[VEC ? 1 : NQ + NP];
   auto stage_in = [&](int t) {       // K-tile t: DMA into its stage, or loads into registers; called for t = 0, 1, 2, ...
-    const int64_t left = ke - kb - (int64_t)t * KT;
+    if (t == nk1) { baseq = p.q2 + startq; basep = p.p + startp; }      // once more, with the second Q
+    const int64_t left = ke - kb - (int64_t)(t < nk1 ? t : t - nk1) * KT;
     if constexpr (VEC) {
       char* buf = smem + (t % NST) * STAGE + wave * 1024;
       const auto rq = __builtin_amdgcn_make_buffer_rsrc((void*)baseq, 0, DMA_SPAN, 0x00020000);
@@ -432,50 +471,16 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
 
 // ---- joins -----------------------------------------------------------------------------------------
 // Sum of the splits in a fixed order, then the epilogue.  A group of eight columns is summed by LANES threads, each over
-// every LANES-th split (four loads in flight), and finished by the first of them.  The blocks behind the rows' fold the
-// bias gradient's strips.
+// every LANES-th split (four loads in flight), and finished by the first of them.
 struct JoinParams {
   const float* partial; unsigned splits;
   unsigned rows_per_y; FastDiv groups;
   Epilogue e;
-  const float* db_partial; int strips, db_n; float* db;
-  unsigned join_blocks;
 };
-
-__device__ __forceinline__ void fold_bias_gradient(const JoinParams& p, float (*red)[16]) {
-  // 16 columns x 16 lanes over the strips
-  const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4, n = (int)(blockIdx.x - p.join_blocks) * 16 + cl;
-  float s = 0.f;
-  if (n < p.db_n) {
-    const float* src = p.db_partial + n;
-    int i = rl;
-    for (; i + 48 < p.strips; i += 64) {
-      const float a = src[(size_t)i * p.db_n], b = src[(size_t)(i + 16) * p.db_n], c = src[(size_t)(i + 32) * p.db_n],
-                  d = src[(size_t)(i + 48) * p.db_n];
-      s += (a + b) + (c + d);
-    }
-    for (; i < p.strips; i += 16) s += src[(size_t)i * p.db_n];
-  }
-  red[rl][cl] = s;
-  __syncthreads();
-  if (rl == 0 && n < p.db_n) {
-    s = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s += red[r][cl];
-    p.db[n] = s;
-  }
-}
 
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
   __shared__ float red[LANES > 1 ? LANES - 1 : 1][256 / LANES][8];
-  if (blockIdx.x >= p.join_blocks) {
-    if (blockIdx.y == 0) {
-      __shared__ float db_red[16][16];
-      fold_bias_gradient(p, db_red);
-    }
-    return;
-  }
   constexpr unsigned GROUPS = 256 / LANES;
   const int64_t row_base = (int64_t)blockIdx.y * p.rows_per_y, left = p.e.M - row_base;
   const unsigned rows = left < (int64_t)p.rows_per_y ? (unsigned)left : p.rows_per_y;
@@ -532,6 +537,7 @@ struct DzParams {
   const void* dy; int64_t lddy;
   const float* preact;          // [M][N], null without an activation
   void* dz;                     // [M][N], null: only the sums are wanted
+  void* dz_lo;                  // [M][N] or null: what dz's rounding lost
   float* db_partial;            // [strips][N] or null
   int64_t M, rows_per_strip;
   int N, act, groups;
@@ -572,6 +578,12 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
         if (p.drop.thr) drop8(v[u], philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
         act_grad_n<T>(z[u], v[u], p.act);
         if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v[u]);
+        if (p.dz_lo) {
+          float lo[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lo[e] = v[u][e] - to_f32<T>(from_f32<T>(v[u][e]));
+          store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] += v[u][e];
       }
@@ -601,7 +613,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
 // round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
 // 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128 1.8, 64x64 0.48.
-struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; };
+struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; double us; };
+constexpr double SPLIT_US = 10.0;      // see bwd_layout
 
 enum Form { FORWARD, GRAD_X, GRAD_W };
 // sizes that are no whole 16-byte chunks stay off the large tiles
@@ -631,7 +644,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
       if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 4.0;
       if (us < best_us) {
         best_us = us;
-        best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt};
+        best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt, us};
       }
     }
   }
@@ -658,7 +671,7 @@ bool chunked(const void* p, int64_t ld, int64_t len, int esize) {
 
 template <typename T, bool QC, bool PC, bool VEC>
 void launch_tiles(const GemmParams& g, const Plan& pl, hipStream_t stream) {
-  const dim3 grid(g.tiles * g.splits);
+  const dim3 grid(g.tiles * g.splits + (g.fold.db ? (unsigned)(g.fold.n + DB_COLS - 1) / DB_COLS : 0));
   if constexpr (VEC && sizeof(T) == 2) {
     if (pl.bm == 256) {
       if constexpr (!QC) {
@@ -675,46 +688,40 @@ void launch_tiles(const GemmParams& g, const Plan& pl, hipStream_t stream) {
   else hipLaunchKernelGGL((linear_gemm_kernel<T, 2, 2, 2, 2, QC, PC, VEC, 0>), grid, dim3(256), 0, stream, g);
 }
 
-// db_*: a bias gradient to fold in the join's launch (or in one of its own)
-struct DbFold { const float* partial = nullptr; int strips = 0, n = 0; float* db = nullptr; };
-
 template <typename T>
-int launch_join(const float* partial, unsigned splits, const Epilogue& e, const DbFold& f, hipStream_t stream) {
+int launch_join(const float* partial, unsigned splits, const Epilogue& e, hipStream_t stream) {
   JoinParams j;
   j.partial = partial; j.splits = splits; j.e = e;
-  j.db_partial = f.partial; j.strips = f.strips; j.db_n = f.n; j.db = f.db;
   const unsigned groups = (unsigned)(e.N + 7) / 8;
-  j.groups = fast_div(groups ? groups : 1);
-  const int64_t cap = 0x08000000u / j.groups.d, rows = partial ? e.M : 0;
-  j.rows_per_y = (unsigned)(rows < cap ? rows : cap);
-  const unsigned ny = rows ? (unsigned)((rows + j.rows_per_y - 1) / j.rows_per_y) : 1u;
+  j.groups = fast_div(groups);
+  const int64_t cap = 0x08000000u / groups;
+  j.rows_per_y = (unsigned)(e.M < cap ? e.M : cap);
+  const unsigned ny = (unsigned)((e.M + j.rows_per_y - 1) / j.rows_per_y);
   // eight threads a group where there are that many splits to read and too few groups to fill the chip with one each
   const int lanes = splits >= 8 && e.M * (int64_t)groups < (1 << 18) ? 8 : 1;
-  j.join_blocks = partial ? (unsigned)(((uint64_t)j.rows_per_y * groups * lanes + 255) / 256) : 0;
-  const unsigned db_blocks = f.db ? (unsigned)(f.n + 15) / 16 : 0;
-  const dim3 grid(j.join_blocks + db_blocks, ny);
+  const dim3 grid((unsigned)(((uint64_t)j.rows_per_y * groups * lanes + 255) / 256), ny);
   if (lanes == 8) hipLaunchKernelGGL((linear_join_kernel<T, 8>), grid, dim3(256), 0, stream, j);
   else hipLaunchKernelGGL((linear_join_kernel<T, 1>), grid, dim3(256), 0, stream, j);
   SDMI_CHECK_HIP(hipGetLastError());
   return SDMI_OK;
 }
 
-// out[m][n] = epilogue(sum_k Q(m, k) P(n, k)); `fold` rides on the join if there is one (returns whether it did)
+// out[m][n] = epilogue(sum_k (Q + Q2)(m, k) P(n, k)); Q2 may be null
 template <typename T, bool QC, bool PC>
-int product(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e, float* partial,
-            const DbFold& fold, bool* folded, hipStream_t stream) {
+int product(const void* q, const void* q2, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e, float* partial,
+            const DbFold& fold, hipStream_t stream) {
   const int sz = (int)sizeof(T);
   Plan pl = plan_product(e.M, e.N, K, sz, QC ? GRAD_W : PC ? GRAD_X : FORWARD);
-  const bool vec = chunked(q, ldq, QC ? e.M : K, sz) && chunked(p, ldp, PC ? e.N : K, sz) && e.N % 8 == 0;
+  const bool vec = chunked(q, ldq, QC ? e.M : K, sz) && ((uintptr_t)q2 & 15) == 0 && chunked(p, ldp, PC ? e.N : K, sz) && e.N % 8 == 0;
   if (!vec && pl.bm == 256) {      // pointers or strides that the sizes do not tell; the splits (and the workspace) stay
     pl.bm = pl.bn = 128;
     pl.tiles_m = (unsigned)((e.M + 127) / 128); pl.tiles_n = (unsigned)((e.N + 127) / 128);
   }
   GemmParams g;
-  g.q = (const char*)q; g.p = (const char*)p; g.ldq = ldq; g.ldp = ldp; g.K = K; g.k_per_split = pl.k_per_split;
+  g.q = (const char*)q; g.q2 = (const char*)q2; g.p = (const char*)p; g.fold = fold; g.ldq = ldq; g.ldp = ldp; g.K = K; g.k_per_split = pl.k_per_split;
   g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.e = e;
   const uint64_t total = (uint64_t)pl.tiles_m * pl.tiles_n * pl.splits;
-  SDMI_REQUIRE(pl.bm && total < (1ull << 31), "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
+  SDMI_REQUIRE(pl.bm && total < (1ull << 30), "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
   g.tiles = pl.tiles_m * pl.tiles_n;
   g.partial = pl.splits > 1 ? partial : nullptr;
   {
@@ -726,18 +733,24 @@ int product(const void* q, int64_t ldq, const void* p, int64_t ldp, int64_t K, c
     SDMI_CHECK_HIP(hipGetLastError());
   }
   if (g.partial) {
-    SDMI_TRY(launch_join<T>(g.partial, g.splits, e, fold, stream));
-    if (folded) *folded = fold.db != nullptr;
+    SDMI_TRY(launch_join<T>(g.partial, g.splits, e, stream));
   }
   return SDMI_OK;
 }
 
-struct BwdLayout { size_t dz, dbp, px, pw, total; int strips, col_blocks, groups; int64_t rows_per_strip; bool need_dz; };
+struct BwdLayout { size_t dz, dz_lo, dbp, px, pw, total; int strips, col_blocks, groups; int64_t rows_per_strip; bool need_dz, split; };
 BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int esize) {
   BwdLayout w;
   size_t o = 0;
   w.need_dz = (act != ACT_NONE || drop) && (want & 3);
+  // With an activation dz = dy act'(z) does not fit the tensors' type, and rounded to it adds an error to dx and dw as
+  // large as the rounding of their own (error against 64 bits 1.41 times that of an unrounded dz, more where a few
+  // entries dominate).  Products whose time is mostly their launch's multiply what the rounding lost as well; the larger
+  // ones would take twice as long (4096x1280x5120 bf16 by about 130 us) and live with it.
+  const Plan px = plan_product(M, K, N, esize, GRAD_X), pw = plan_product(N, K, M, esize, GRAD_W);
+  w.split = w.need_dz && act != ACT_NONE && esize == 2 && px.us <= SPLIT_US && pw.us <= SPLIT_US;
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
+  w.dz_lo = o; o += w.split ? up256((size_t)M * N * esize) : 0;
   // column groups a block takes (all, or an even share), and strips of rows: about 1024 blocks, every row lane at
   // least four rows where there are that many
   const int ncg = (N + 7) / 8;
@@ -752,8 +765,8 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   w.rows_per_strip = (M + strips - 1) / strips;
   w.strips = w.rows_per_strip ? (int)((M + w.rows_per_strip - 1) / w.rows_per_strip) : 0;
   w.dbp = o; o += (want & 4) ? up256((size_t)w.strips * N * 4) : 0;
-  w.px = o; o += (want & 1) ? partial_bytes(plan_product(M, K, N, esize, GRAD_X), M, K) : 0;
-  w.pw = o; o += (want & 2) ? partial_bytes(plan_product(N, K, M, esize, GRAD_W), N, K) : 0;
+  w.px = o; o += (want & 1) ? partial_bytes(px, M, K) : 0;
+  w.pw = o; o += (want & 2) ? partial_bytes(pw, N, K) : 0;
   w.total = o;
   return w;
 }
@@ -778,6 +791,7 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
     DzParams d;
     d.dy = a.dy; d.lddy = a.lddy; d.preact = a.act != ACT_NONE ? a.preact : nullptr;
     d.dz = w.need_dz ? ws + w.dz : nullptr;
+    d.dz_lo = w.split ? ws + w.dz_lo : nullptr;
     d.db_partial = a.db ? (float*)(ws + w.dbp) : nullptr;
     d.M = a.rows; d.rows_per_strip = w.rows_per_strip; d.N = a.n; d.act = a.act; d.drop = drop; d.groups = w.groups;
     if (a.act == ACT_NONE) d.drop.scale = 1.f;
@@ -790,14 +804,21 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
     if (w.need_dz) { dz = d.dz; lddz = a.n; }
   }
   if (a.db) { fold.partial = (const float*)(ws + w.dbp); fold.strips = a.rows > 0 ? w.strips : 0; fold.n = a.n; fold.db = a.db; }
-  bool folded = false;
-  if (a.dw)
-    SDMI_TRY((product<T, true, true>(dz, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha), (float*)(ws + w.pw), fold,
-                                     &folded, s)));
-  if (a.dx && a.rows > 0)
-    SDMI_TRY((product<T, false, true>(dz, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha), (float*)(ws + w.px),
-                                      folded ? DbFold() : fold, folded ? nullptr : &folded, s)));
-  if (a.db && !folded) SDMI_TRY(launch_join<T>(nullptr, 0, plain_out(nullptr, 0, 0, 1.f), fold, s));
+  const void* dz_lo = a.rows > 0 && w.split ? ws + w.dz_lo : nullptr;
+  if (a.dw) {
+    SDMI_TRY((product<T, true, true>(dz, dz_lo, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha), (float*)(ws + w.pw),
+                                     fold, s)));
+    fold = DbFold();
+  }
+  if (a.dx && a.rows > 0) {
+    SDMI_TRY((product<T, false, true>(dz, dz_lo, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha), (float*)(ws + w.px),
+                                      fold, s)));
+    fold = DbFold();
+  }
+  if (fold.db) {
+    hipLaunchKernelGGL(linear_db_kernel, dim3((fold.n + DB_COLS - 1) / DB_COLS), dim3(256), 0, s, fold);
+    SDMI_CHECK_HIP(hipGetLastError());
+  }
   return SDMI_OK;
 }
 
@@ -831,8 +852,8 @@ int linear_act(const LinearActArgs& a, hipStream_t stream) {
   SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %lld bytes", (long long)need);
   e.bias = a.bias; e.resid = a.resid; e.ldr = a.ldr; e.out = a.out; e.ldo = a.n;
   e.alpha = 1.f; e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
-  SDMI_DISPATCH_DTYPE(a.dtype, T, return (product<T, false, false>(a.x, a.ldx, a.w, a.ldw, a.k, e, (float*)a.workspace,
-                                                                     DbFold(), nullptr, stream)));
+  SDMI_DISPATCH_DTYPE(a.dtype, T, return (product<T, false, false>(a.x, nullptr, a.ldx, a.w, a.ldw, a.k, e,
+                                                                     (float*)a.workspace, DbFold(), stream)));
   return SDMI_OK;
 }
 

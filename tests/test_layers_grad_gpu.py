@@ -441,3 +441,19 @@ def test_python_refusals_on_device_tensors():
     y, = torch.autograd.grad(ops.dropout(v, 0.5, 1).sum(), v, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y.sum(), v)                    # no second derivatives
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("m,k,n,act", [(1, 64, 24, "silu"), (5, 320, 640, "gelu"), (77, 768, 768, "quick_gelu"), (300, 33, 130, "silu")])
+def test_small_products_lose_nothing_but_their_own_rounding(m, k, n, act, dt):
+    """dx and dw of small layers with an activation are as far from 64 bits as their own rounding puts them: what dz
+    loses in the tensors' type is multiplied too.  An error of the same size on top would be 1.41 times as far."""
+    dt = DT[dt]
+    x, w = rand(m, k, dtype=dt, grad=True), rand(n, k, dtype=dt, seed=1, scale=k ** -0.5, grad=True)
+    dy = rand(m, n, dtype=dt, seed=4)
+    grads = torch.autograd.grad(ops.linear_act(x, w, act=act, p=0.1, seed=99), [x, w], dy)
+    ref = R.linear_ref(x, w, None, None, dy, act, 0.1, 99, 0, dt)
+    for got, name in zip(grads, ("dx", "dw")):
+        want = ref[name][0]
+        own = float((want.to(dt).double() - want).norm())
+        assert float((got.double().cpu() - want).norm()) < 1.05 * own, name
