@@ -9,9 +9,6 @@
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
-#ifdef SDMI_TUNE
-#include <stdlib.h>
-#endif
 
 namespace {
 
@@ -648,17 +645,6 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
       }
     }
   }
-#ifdef SDMI_TUNE
-  if (const char* ev = getenv("TILE")) {
-    int bm, bn, sp;
-    if (sscanf(ev, "%d,%d,%d", &bm, &bn, &sp) == 3) {
-      best.bm = bm; best.bn = bn; best.tiles_m = (unsigned)((M + bm - 1) / bm); best.tiles_n = (unsigned)((N + bn - 1) / bn);
-      if (sp > nkt) sp = (int)nkt;
-      const int64_t per2 = (nkt + sp - 1) / sp;
-      best.k_per_split = per2 * kt; best.splits = (unsigned)((nkt + per2 - 1) / per2);
-    }
-  }
-#endif
   return best;
 }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }

@@ -105,14 +105,15 @@ class DDIMSampler(object):
                                   log_every_t=log_every_t,
                                   unconditional_guidance_scale=unconditional_guidance_scale,
                                   unconditional_conditioning=unconditional_conditioning, verbose=verbose,
-                                  noise_fn=kwargs.get("noise_fn"), q_noise_fn=kwargs.get("q_noise_fn"))
+                                  noise_fn=kwargs.get("noise_fn"), q_noise_fn=kwargs.get("q_noise_fn"),
+                                  noise_dropout_seed=kwargs.get("noise_dropout_seed"))
 
     @torch.no_grad()
     def ddim_sampling(self, conditioning, shape, x_T=None, ddim_use_original_steps=False, callback=None,
                       timesteps=None, quantize_denoised=False, mask=None, x0=None, img_callback=None,
                       log_every_t=100, temperature=1., noise_dropout=0., score_corrector=None,
                       corrector_kwargs=None, unconditional_guidance_scale=1., unconditional_conditioning=None,
-                      verbose=True, noise_fn=None, q_noise_fn=None):
+                      verbose=True, noise_fn=None, q_noise_fn=None, noise_dropout_seed=None):
         device = self.model.device
         b = shape[0]
         img = torch.randn(shape, device=device) if x_T is None else x_T.to(device, torch.float32)
@@ -149,7 +150,7 @@ class DDIMSampler(object):
                               noise_dropout=noise_dropout, score_corrector=score_corrector,
                               corrector_kwargs=corrector_kwargs,
                               unconditional_guidance_scale=unconditional_guidance_scale, noise_fn=noise_fn,
-                              want_pred_x0=img_callback is not None)
+                              want_pred_x0=img_callback is not None, noise_dropout_seed=noise_dropout_seed)
             if callback:
                 callback(i)
             if img_callback:
@@ -194,7 +195,7 @@ class DDIMSampler(object):
 
         def step(self, cond, t_value, index, use_original_steps=False, quantize_denoised=False, temperature=1.,
                  noise_dropout=0., score_corrector=None, corrector_kwargs=None, unconditional_guidance_scale=1.,
-                 noise_fn=None, want_pred_x0=True):
+                 noise_fn=None, want_pred_x0=True, noise_dropout_seed=None):
             """One p_sample_ddim (:5338-5375).  ``t_value`` is the step's timestep for the whole batch (what the
             sampling loops pass, :5314) or a (b,) tensor of per-sample timesteps."""
             s = self.s
@@ -237,7 +238,7 @@ class DDIMSampler(object):
                 if noise_dropout > 0.:
                     # dropout(sigma * noise * temperature) (:5371-5373): the mask and its 1 / (1 - p) act on the noise
                     # term, whose other factors are scalars
-                    noise = torch.nn.functional.dropout(noise * temperature, p=noise_dropout)
+                    noise = ops.noise_dropout(noise * temperature, noise_dropout, noise_dropout_seed, index)
                     temperature = 1.
             from ._lib import lib, check, ptr, stream_ptr
             check(lib().sdmi_ddim_step(ptr(self.x_in), ptr(eps), 1 if combine else 0,
@@ -261,8 +262,10 @@ class DDIMSampler(object):
     @torch.no_grad()
     def p_sample_ddim(self, x, c, t, index, repeat_noise=False, use_original_steps=False, quantize_denoised=False,
                       temperature=1., noise_dropout=0., score_corrector=None, corrector_kwargs=None,
-                      unconditional_guidance_scale=1., unconditional_conditioning=True, noise=None):
-        """One step with the reference's signature; returns (x_prev, pred_x0)."""
+                      unconditional_guidance_scale=1., unconditional_conditioning=True, noise=None,
+                      noise_dropout_seed=None):
+        """One step with the reference's signature; returns (x_prev, pred_x0).  ``noise_dropout_seed``: the mask of
+        ``noise_dropout`` comes from (seed, index) instead of the device's random state."""
         doubled = bool(unconditional_conditioning) and unconditional_guidance_scale != 1.
         st = self._StepState(self, x, doubled)
         t = torch.as_tensor(t).reshape(-1)
@@ -273,7 +276,8 @@ class DDIMSampler(object):
                        quantize_denoised=quantize_denoised, temperature=temperature, noise_dropout=noise_dropout,
                        score_corrector=score_corrector, corrector_kwargs=corrector_kwargs,
                        unconditional_guidance_scale=unconditional_guidance_scale,
-                       noise_fn=(lambda shape: noise) if noise is not None else None)
+                       noise_fn=(lambda shape: noise) if noise is not None else None,
+                       noise_dropout_seed=noise_dropout_seed)
         return st.x().clone(), pred.clone()
 
     @torch.no_grad()

@@ -235,10 +235,11 @@ class LatentDiffusion:
     @torch.no_grad()
     def p_sample(self, x, c, t, clip_denoised=False, repeat_noise=False, return_codebook_ids=False,
                  quantize_denoised=False, return_x0=False, temperature=1., noise_dropout=0., score_corrector=None,
-                 corrector_kwargs=None, noise=None, _eps_out=None):
+                 corrector_kwargs=None, noise=None, _eps_out=None, noise_dropout_seed=None):
         """stable_diffusion.py:4693-4721.  One UNet call and one fused update kernel; ``noise`` may be
         injected (the reference draws it with torch.randn); ``_eps_out`` names the UNet's output buffer (the
-        sampling loops keep it, x and t at fixed addresses so that the UNet's launch graph is replayed)."""
+        sampling loops keep it, x and t at fixed addresses so that the UNet's launch graph is replayed);
+        ``noise_dropout_seed``: the mask of ``noise_dropout`` comes from (seed, first sample's t)."""
         if return_codebook_ids or quantize_denoised:
             raise NotImplementedError("VQ first stage options are not on this path")
         x = x.to(self.device, torch.float32).contiguous()
@@ -257,7 +258,7 @@ class LatentDiffusion:
                 noise = torch.randn(x.shape, device=self.device)
         noise = noise.to(self.device, torch.float32).contiguous()
         if noise_dropout > 0.:
-            noise = torch.nn.functional.dropout(noise * temperature, p=noise_dropout)
+            noise = ops.noise_dropout(noise * temperature, noise_dropout, noise_dropout_seed, int(tt[0]))
             temperature = 1.0
         x_prev, x0 = self._ddpm_update(x, model_out.contiguous(), tt, clip_denoised, noise, temperature, return_x0)
         return (x_prev, x0) if return_x0 else x_prev
@@ -326,7 +327,7 @@ class LatentDiffusion:
     def progressive_denoising(self, cond, shape, verbose=True, callback=None, quantize_denoised=False,
                               img_callback=None, mask=None, x0=None, temperature=1., noise_dropout=0.,
                               score_corrector=None, corrector_kwargs=None, batch_size=None, x_T=None, start_T=None,
-                              log_every_t=None):
+                              log_every_t=None, noise_dropout_seed=None):
         """stable_diffusion.py:4723-4777: the same loop, logging the x0 predictions; ``shape`` excludes the batch
         axis when ``batch_size`` is given."""
         if batch_size is not None:
@@ -342,7 +343,8 @@ class LatentDiffusion:
                                                         quantize_denoised=quantize_denoised, return_x0=True,
                                                         temperature=temps[i], noise_dropout=noise_dropout,
                                                         score_corrector=score_corrector,
-                                                        corrector_kwargs=corrector_kwargs, _eps_out=ebuf)
+                                                        corrector_kwargs=corrector_kwargs, _eps_out=ebuf,
+                                                        noise_dropout_seed=noise_dropout_seed)
         img = self._ancestral_loop(self._first_n(cond, b), img, steps, step, x0_log, log_every_t or self.log_every_t,
                                    mask, x0, callback, img_callback)
         return img, x0_log

@@ -442,6 +442,14 @@ def dropout(x, p, seed, offset=0, resid=None):
     return _dropout(x, resid, p, seed, seed_t, offset)
 
 
+def noise_dropout(noise, p, seed=None, step=0):
+    """The samplers' dropout of the noise term: torch's, drawn from the device's generator, or with ``seed`` the
+    counter-based mask of (seed, step), which does not depend on what was drawn before."""
+    if seed is None:
+        return torch.nn.functional.dropout(noise, p=p)
+    return dropout(noise, p, seed, step)
+
+
 def _workspace(nbytes, like):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 

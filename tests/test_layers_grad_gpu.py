@@ -457,3 +457,40 @@ def test_small_products_lose_nothing_but_their_own_rounding(m, k, n, act, dt):
         want = ref[name][0]
         own = float((want.to(dt).double() - want).norm())
         assert float((got.double().cpu() - want).norm()) < 1.05 * own, name
+
+
+# ---- the samplers' noise dropout ------------------------------------------------------------------------------
+
+def test_samplers_noise_dropout_by_seed():
+    """``noise_dropout_seed``: the same mask on every run whatever was drawn before, another one per step and seed, and
+    the one that ops.dropout gives for (seed, step)."""
+    from _util import device_latent_diffusion, synth
+    model = device_latent_diffusion(4, "crossattn", "fp32")
+    sampler = importlib.import_module("stable-diffusion_amd").DDIMSampler(model)
+    sampler.make_schedule(50, ddim_eta=0.5, verbose=False)
+    x = synth.normal(11, "psd.x", (2, 4, 16, 16)).cuda()
+    ctx = torch.cat([synth.normal(2, "psd.uc", (2, 77, 768)), synth.normal(1, "psd.c", (2, 77, 768))]).cuda()
+    noise = synth.normal(12, "psd.noise", (2, 4, 16, 16)).cuda()
+
+    def step(index, nz=noise, **kw):
+        st = sampler._StepState(sampler, x, True)
+        st.step(ctx, 20 * index + 1, index, unconditional_guidance_scale=7.5, noise_fn=lambda s: nz, **kw)
+        torch.rand(3, device="cuda")
+        return st.x().clone()
+
+    def t_step(**kw):
+        return model.p_sample(x, ctx[:2], torch.full((2,), 500), **kw)
+    a = step(49, noise_dropout=0.5, noise_dropout_seed=7)
+    assert torch.equal(a, step(49, noise_dropout=0.5, noise_dropout_seed=7))
+    assert torch.equal(a, step(49, ops.dropout(noise, 0.5, 7, 49)))
+    assert not torch.equal(a, step(49, noise_dropout=0.5, noise_dropout_seed=8))
+    b = t_step(noise=noise, noise_dropout=0.5, noise_dropout_seed=7)
+    assert torch.equal(b, t_step(noise=ops.dropout(noise, 0.5, 7, 500)))
+    assert not torch.equal(ops.dropout(noise, 0.5, 7, 49), ops.dropout(noise, 0.5, 7, 500))
+    lat, _ = sampler.sample(4, 2, (4, 16, 16), conditioning=ctx, eta=0.5, x_T=x, verbose=False, noise_dropout=0.3,
+                            unconditional_guidance_scale=7.5, unconditional_conditioning=True,
+                            noise_fn=lambda s: noise, noise_dropout_seed=1)
+    again, _ = sampler.sample(4, 2, (4, 16, 16), conditioning=ctx, eta=0.5, x_T=x, verbose=False, noise_dropout=0.3,
+                              unconditional_guidance_scale=7.5, unconditional_conditioning=True,
+                              noise_fn=lambda s: noise, noise_dropout_seed=1)
+    assert torch.equal(lat, again)
