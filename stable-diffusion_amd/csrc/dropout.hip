@@ -68,6 +68,7 @@ int launch_dropout(const DropoutArgs& a, const DropArgs& drop, hipStream_t strea
 
 int dropout(const DropoutArgs& a, hipStream_t stream) {
   SDMI_REQUIRE(a.rows >= 0 && a.cols >= 0, "dropout: negative size");
+  SDMI_REQUIRE(a.cols <= (1 << 30), "dropout: rows of %d columns are too long", a.cols);
   SDMI_REQUIRE(a.ldx >= 0 && a.ldr >= 0, "dropout: negative row stride");
   DropArgs drop;
   SDMI_TRY(drop_args(&drop, a.p, a.seed, a.seed_dev, a.offset, "dropout"));

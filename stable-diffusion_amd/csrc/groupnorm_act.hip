@@ -296,12 +296,12 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
 // pixels a thread has in flight while it works on as many: 64 bytes (32 of each tensor backward), what the registers hold
 template <typename T> struct Depth { static constexpr int FWD = 16 / (int)sizeof(T) / 2, BWD = 1; };
 struct Walk { int ncg, lanes, pl, cg0, count; int64_t row0; };      // count pixels from row row0 on
-constexpr int WALK_CGS = 256;
 __device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip, int b) {
   Walk w;
   w.ncg = (p.C + 7) >> 3;
-  const bool fits = w.ncg <= 256;
-  w.lanes = fits ? 256 / w.ncg : 1;
+  const int threads = (int)blockDim.x;
+  const bool fits = w.ncg <= threads;
+  w.lanes = fits ? threads / w.ncg : 1;
   w.pl = fits ? (int)threadIdx.x / w.ncg : 0;
   w.cg0 = fits ? (int)threadIdx.x - w.pl * w.ncg : (int)threadIdx.x;
   if (w.pl >= w.lanes) w.cg0 = w.ncg;                    // threads left over
@@ -319,7 +319,7 @@ __device__ __forceinline__ void fetch(const C& x, const Walk& w, int px, typenam
 // threads per group for folds over the groups: a power of two, at most a wave
 __device__ __forceinline__ int threads_per_group(int G) {
   int t = 64;
-  while (t > 1 && t * G > 256) t >>= 1;
+  while (t > 1 && t * G > (int)blockDim.x) t >>= 1;
   return t;
 }
 template <typename F> __device__ __forceinline__ F fold_lanes(F v, int tpg) {
@@ -329,7 +329,7 @@ template <typename F> __device__ __forceinline__ F fold_lanes(F v, int tpg) {
 // the strip's channel sums in LDS ([lanes][ncg * 8], two arrays) -> lane 0's row holds the totals
 __device__ __forceinline__ void fold_pixel_lanes(float* s1, float* s2, int lanes, int width) {
   __syncthreads();
-  for (int c = threadIdx.x; c < width; c += 256) {
+  for (int c = threadIdx.x; c < width; c += (int)blockDim.x) {
     float a = s1[c], q = s2[c];
     for (int l = 1; l < lanes; ++l) { a += s1[l * width + c]; q += s2[l * width + c]; }
     s1[c] = a; s2[c] = q;
@@ -338,7 +338,7 @@ __device__ __forceinline__ void fold_pixel_lanes(float* s1, float* s2, int lanes
 }
 
 template <typename T, bool WHOLE>
-__global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
+__global__ __launch_bounds__(1024) void gna_stats_kernel(GnaParams p) {
   constexpr int WALK = Depth<T>::FWD;
   extern __shared__ __align__(16) char smem[];
   const int strip = blockIdx.x, b = blockIdx.y;
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
   const int width = w.ncg * 8;
   float* s1 = reinterpret_cast<float*>(smem);
   float* s2 = s1 + w.lanes * width;
-  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
+  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
     const int c = cg * 8;
     const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
     float sh[8], s[8], q[8];
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
   }
   fold_pixel_lanes(s1, s2, w.lanes, width);
   const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
-  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {                // every lane goes round equally often (shuffles)
+  for (int g0 = 0; g0 < p.G; g0 += (int)blockDim.x / tpg) {                // every lane goes round equally often (shuffles)
     const int g = g0 + (int)threadIdx.x / tpg;
     float a = 0.f, q = 0.f;
     if (g < p.G)
@@ -389,7 +389,7 @@ __global__ __launch_bounds__(256) void gna_stats_kernel(GnaParams p) {
 // sums over the strips of sample b, per group, in double: fin(g, first sum, second sum) on one thread per group
 template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaParams& p, int b, Fn fin) {
   const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
-  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {
+  for (int g0 = 0; g0 < p.G; g0 += (int)blockDim.x / tpg) {
     const int g = g0 + (int)threadIdx.x / tpg;
     double a = 0.0, q = 0.0;
     if (g < p.G) {
@@ -410,7 +410,7 @@ template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaPara
 }
 
 template <typename T, int ACT, bool DROP, bool WHOLE>
-__global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
+__global__ __launch_bounds__(1024) void gna_apply_kernel(GnaParams p) {
   constexpr int WALK = Depth<T>::FWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
@@ -435,7 +435,7 @@ __global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
   __syncthreads();
   unsigned k0 = 0, k1 = 0;
   if (DROP) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
+  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
     const int c = cg * 8;
     const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), y(p.out0, p.out0, p.C, 0, c, w.row0);
     if (cg != w.cg0) fetch(x, w, w.pl, r);
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256, 4) void gna_apply_kernel(GnaParams p) {
 
 // backward, first launch: channel sums of du and du xh over the strip, and the group sums of gamma times them
 template <typename T, int ACT, bool DROP, bool WHOLE>
-__global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
+__global__ __launch_bounds__(1024) void gna_grad_sums_kernel(GnaParams p) {
   constexpr int WALK_BWD = Depth<T>::BWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
   float* s2 = s1 + w.lanes * width;
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
+  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
     const int c = cg * 8;
     const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0);
     typename C::Raw rx[WALK_BWD], rd[WALK_BWD];
@@ -532,10 +532,10 @@ __global__ __launch_bounds__(256, 4) void gna_grad_sums_kernel(GnaParams p) {
   fold_pixel_lanes(s1, s2, w.lanes, width);
   if (p.dgamma || p.dbeta) {
     float* cp = p.cpart + ((size_t)b * p.strips + strip) * 2 * p.C;
-    for (int c = threadIdx.x; c < p.C; c += 256) { cp[c] = s1[c]; cp[p.C + c] = s2[c]; }
+    for (int c = threadIdx.x; c < p.C; c += (int)blockDim.x) { cp[c] = s1[c]; cp[p.C + c] = s2[c]; }
   }
   const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
-  for (int g0 = 0; g0 < p.G; g0 += 256 / tpg) {
+  for (int g0 = 0; g0 < p.G; g0 += (int)blockDim.x / tpg) {
     const int g = g0 + (int)threadIdx.x / tpg;
     float a = 0.f, q = 0.f;
     if (g < p.G)
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int
 
 // backward, second launch: dx; the blocks behind the strips' fold dgamma and dbeta
 template <typename T, int ACT, bool DROP, bool WHOLE>
-__global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
+__global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
   constexpr int WALK_BWD = Depth<T>::BWD;
   const int act = ACT < 0 ? p.act : ACT;
   extern __shared__ __align__(16) char smem[];
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(256, 4) void gna_grad_apply_kernel(GnaParams p) {
   __syncthreads();
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += WALK_CGS) {
+  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
     const int c = cg * 8;
     const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0), dx(p.out0, p.out1, p.c0, p.c1, c, w.row0);
     if (cg != w.cg0) {
@@ -656,7 +656,7 @@ struct GnaPlan {
   int slice;                    // 1: one workgroup per (sample, group)
   int w;                        // ... columns per access
   int lds;
-  int strips; int64_t px_per_strip;
+  int threads, strips; int64_t px_per_strip;
   size_t part, cpart, total;    // workspace offsets
 };
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -669,19 +669,33 @@ GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backwa
   pl.w = 1;
   for (int w = 8; w > 1; w >>= 1)
     if (cpg % w == 0 && c0 % w == 0) { pl.w = w; break; }
-  if (HW <= (1 << 20) && (size_t)HW * cpg * per <= 60 * 1024) {
+  // beyond 8192 accesses a slice keeps its workgroup longer than two launches over strips take (bf16, us forward:
+  // 3x37x53x480, 15 channels a group one by one, 37 against 15; 16x32x32x960 in pairs 37 against 28; but 16x32x32x640 in
+  // fours 18 against 21)
+  if (HW * (cpg / pl.w) <= 8192 && (size_t)HW * cpg * per <= 60 * 1024) {
     pl.slice = 1;
     pl.lds = (int)((size_t)HW * cpg * per);
     pl.cpart = 0;
     pl.total = backward && B > 1 ? up256((size_t)B * 2 * C * 4) : 0;
     return pl;
   }
-  const int ncg = (C + 7) / 8, lanes = ncg <= 256 ? 256 / ncg : 1;
-  // about four workgroups per CU, every pixel lane at least four pixels, and no more strips than a fold likes to read
-  int64_t strips = (1024 + B - 1) / B;
-  const int64_t by_work = (HW + 4 * lanes - 1) / (4 * lanes);
-  if (strips > by_work) strips = by_work;
-  if (strips > 256) strips = 256;
+  // About 1024 waves' worth of threads on the chip at a time (128 registers each): 512 blocks of 512, every pixel lane at
+  // least four pixels.  Every block of the second launch folds its sample's strips, so where few samples would get more
+  // than 128 strips each, and where a row alone takes half a block, it is 256 blocks of 1024.  Forward + backward, bf16,
+  // us: 16x64x64x320 84 (92 with the large blocks), 2x64x64x320 34 (44), 1x256x256x256 75 (93 with the small ones),
+  // 1x40x30x2560 45 (58).  A lane adds at most 512 values one after the other.
+  const int ncg = (C + 7) / 8;
+  int lanes;
+  int64_t strips;
+  for (pl.threads = 512;; pl.threads = 1024) {
+    lanes = ncg <= pl.threads ? pl.threads / ncg : 1;
+    const int64_t by_work = (HW + 4 * lanes - 1) / (4 * lanes);
+    strips = ((1 << 18) / pl.threads + B - 1) / B;
+    if (strips > by_work) strips = by_work;
+    if (pl.threads == 1024 || (strips <= 128 && ncg <= 256)) break;
+  }
+  const int64_t by_sum = (HW + 512 * lanes - 1) / (512 * lanes);
+  if (strips < by_sum) strips = by_sum;
   if (strips < 1) strips = 1;
   pl.px_per_strip = (HW + strips - 1) / strips;
   pl.px_per_strip = (pl.px_per_strip + 4 * lanes - 1) / (4 * lanes) * (4 * lanes);      // whole walks of every lane
@@ -726,7 +740,7 @@ int slice_threads(const GnaPlan& pl, const GnaParams& p) {
 }
 
 // the kernels over strips with SiLU (others by a branch), dropout and whole column groups compiled in
-#define GNA_LAUNCH(K, A, D, W, GRID, LDS) hipLaunchKernelGGL((K<T, A, D, W>), GRID, dim3(256), LDS, s, p)
+#define GNA_LAUNCH(K, A, D, W, GRID, LDS) hipLaunchKernelGGL((K<T, A, D, W>), GRID, dim3(pl.threads), LDS, s, p)
 #define GNA_VARIANTS_W(K, W, GRID, LDS)                                   \
   {                                                                       \
     if (p.drop.thr) {                                                     \
@@ -763,8 +777,8 @@ int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
   } else {
     const dim3 grid(pl.strips, p.B);
     const bool whole = gna_whole(p);
-    if (whole) hipLaunchKernelGGL((gna_stats_kernel<T, true>), grid, dim3(256), pl.lds, s, p);
-    else hipLaunchKernelGGL((gna_stats_kernel<T, false>), grid, dim3(256), pl.lds, s, p);
+    if (whole) hipLaunchKernelGGL((gna_stats_kernel<T, true>), grid, dim3(pl.threads), pl.lds, s, p);
+    else hipLaunchKernelGGL((gna_stats_kernel<T, false>), grid, dim3(pl.threads), pl.lds, s, p);
     GNA_VARIANTS(gna_apply_kernel, grid, 2 * p.G * 4)
   }
   SDMI_CHECK_HIP(hipGetLastError());

@@ -812,6 +812,7 @@ int check_common(const LinearActArgs& a, const char* who) {
   SDMI_REQUIRE(a.dtype >= 0 && a.dtype <= 2, "%s: bad dtype %d", who, a.dtype);
   SDMI_REQUIRE(a.rows >= 0 && a.k > 0 && a.n > 0, "%s: bad size (%lld rows, %d inputs, %d outputs)", who,
                (long long)a.rows, a.k, a.n);
+  SDMI_REQUIRE(a.k <= (1 << 30) && a.n <= (1 << 30), "%s: %d inputs, %d outputs are too many", who, a.k, a.n);
   SDMI_REQUIRE(a.act >= 0 && a.act < ACT_COUNT, "%s: unknown activation %d", who, a.act);
   SDMI_REQUIRE(a.ldx >= 0 && a.ldw >= 0 && a.ldr >= 0 && a.lddy >= 0, "%s: negative row stride", who);
   return SDMI_OK;

@@ -358,6 +358,12 @@ def _check_input(what, x):
         raise ValueError(f"{what} is {x.dtype}, expected float32, float16 or bfloat16")
 
 
+def _check_columns(*counts):
+    for n in counts:
+        if n > 1 << 30:
+            raise ValueError(f"rows of {n} columns are too long: at most 2^30")
+
+
 def _drop_state(p, seed, offset, device):
     """(p, host seed, seed tensor or None, offset), checked."""
     p, offset = float(p), int(offset)
@@ -434,6 +440,7 @@ def dropout(x, p, seed, offset=0, resid=None):
     (read when the kernel runs); ``offset``: one number per layer or call, below 2^32.  ``p`` counts in steps of
     2^-16, and the scale is that of the probability used.  Dropped elements are 0 whatever they held."""
     _check_input("x", x)
+    _check_columns(*x.shape[-1:])
     p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
     if resid is not None:
         _check_like("resid", resid, x.device, x.dtype, x.shape)
@@ -519,6 +526,7 @@ def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or 0 in w.shape:
         raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (..., K) and (N, K)")
     _check_like("w", w, x.device, x.dtype)
+    _check_columns(*w.shape)
     n = w.shape[0]
     if bias is not None:
         _check_like("bias", bias, x.device, torch.float32, (n,))
@@ -596,6 +604,8 @@ def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.
     groups = int(groups)
     if c == 0 or x.shape[-1] == 0 or groups < 1 or c % groups:
         raise ValueError(f"{c} channels do not split into {groups} groups")
+    if c > 8192 or x.shape[0] > 65535:
+        raise ValueError(f"batch {x.shape[0]} of {c} channels: at most 65535 and 8192 are supported")
     _check_like("gamma", gamma, x.device, torch.float32, (c,))
     _check_like("beta", beta, x.device, torch.float32, (c,))
     x, gamma, beta, eps = x.contiguous(), gamma.contiguous(), beta.contiguous(), float(eps)

@@ -53,12 +53,16 @@ def test_library_refuses_bad_calls():
     assert "negative" in _refused("sdmi_dropout", *drop(rows=-1))
     assert "negative" in _refused("sdmi_dropout", *drop(ld=-8))
     assert "null" in _refused("sdmi_dropout", *drop(x=None))
+    assert "too long" in _refused("sdmi_dropout", *drop(cols=(1 << 30) + 8))
+    assert "too many" in _refused("sdmi_dropout", *drop(rows=1 << 50, cols=1 << 10))
     assert "aligned" in _refused("sdmi_dropout", *drop(sd=ctypes.c_void_p(4100)))
 
     lin = lambda rows=4, k=8, n=8, act=0, dt=1, w=D, ws=None: (D, k, w, k, None, None, 0, D, None, rows, k, n, act, 0.0, 0,
                                                              None, 0, ws, dt, None)
     assert "size" in _refused("sdmi_linear_act", *lin(k=0))
     assert "size" in _refused("sdmi_linear_act", *lin(rows=-1))
+    assert "too many" in _refused("sdmi_linear_act", *lin(n=(1 << 30) + 1))
+    assert "too many" in _refused("sdmi_linear_act", *lin(rows=1 << 50))
     assert "activation" in _refused("sdmi_linear_act", *lin(act=4))
     assert "dtype" in _refused("sdmi_linear_act", *lin(dt=-1))
     assert "null" in _refused("sdmi_linear_act", *lin(w=None))
@@ -122,5 +126,7 @@ def test_python_refuses_cpu_tensors_and_bad_arguments():
         ops._drop_state(0.5, torch.zeros(1), 0, dev)
     with pytest.raises(ValueError, match="one"):
         ops._drop_state(0.5, torch.zeros(2, dtype=torch.int64), 0, dev)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops._check_columns(8, (1 << 30) + 1)
     with pytest.raises(ValueError, match="activation"):
         ops._act_code("relu")
