@@ -245,9 +245,28 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
     }
   }
 
+  const T* src[VEC ? 1 : NQ + NP];   // register staging: any stride, so whole addresses
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int i = 0; i < NQ + NP; ++i) {
+      const bool isq = i < NQ, cols = isq ? QC : PC;
+      const int64_t ld = isq ? p.ldq : p.ldp, left = isq ? leftq : leftp;
+      int a, c;
+      place(isq ? i : i - NQ, isq, a, c);
+      src[i] = reinterpret_cast<const T*>(isq ? baseq : basep) + (cols || a < left ? a : left - 1) * ld + c * EPC;
+    }
+  }
+
   u32x4 reg[VEC ? 1 : NQ + NP];
   auto stage_in = [&](int t) {       // K-tile t: DMA into its stage, or loads into registers; called for t = 0, 1, 2, ...
-    if (t == nk1) { baseq = p.q2 + startq; basep = p.p + startp; }      // once more, with the second Q
+    if (t == nk1) {                  // once more, with the second Q
+      if constexpr (VEC) { baseq = p.q2 + startq; basep = p.p + startp; }
+      else {
+        const int64_t backq = (p.q2 - p.q) - nk1 * stepq, backp = -nk1 * stepp;
+#pragma unroll
+        for (int i = 0; i < NQ + NP; ++i) src[i] = reinterpret_cast<const T*>(reinterpret_cast<const char*>(src[i]) + (i < NQ ? backq : backp));
+      }
+    }
     const int64_t left = ke - kb - (int64_t)(t < nk1 ? t : t - nk1) * KT;
     if constexpr (VEC) {
       char* buf = smem + (t % NST) * STAGE + wave * 1024;
@@ -268,26 +287,31 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
     } else {
       typedef typename Frag<T>::type F;
       typedef F Fu __attribute__((aligned(sizeof(T))));
+      if (left >= KT && (!QC || leftq >= BM) && (!PC || leftp >= BN)) {      // every chunk is whole
 #pragma unroll
-      for (int i = 0; i < NQ + NP; ++i) {
-        const bool isq = i < NQ, cols = isq ? QC : PC;
-        const int64_t ld = isq ? p.ldq : p.ldp, out = isq ? leftq : leftp;
-        int a, c;
-        place(isq ? i : i - NQ, isq, a, c);
-        // elements of the chunk that are there
-        const int64_t have = cols ? (a < left ? out - c * EPC : 0) : left - c * EPC;
-        const int n = have <= 0 ? 0 : (have < EPC ? (int)have : EPC);
-        const T* src = reinterpret_cast<const T*>(isq ? baseq : basep) +
-                       (cols ? a * ld + c * EPC : (a < out ? a : out - 1) * ld + c * EPC);
-        F f;
-        if (n == EPC) {
-          f = *reinterpret_cast<const Fu*>(src);
-        } else {
-#pragma unroll
-          for (int e = 0; e < EPC; ++e) f[e] = e < n ? src[e] : (T)0.f;
+        for (int i = 0; i < NQ + NP; ++i) {
+          reg[i] = __builtin_bit_cast(u32x4, (F)*reinterpret_cast<const Fu*>(src[i]));
         }
-        reg[i] = __builtin_bit_cast(u32x4, f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NQ + NP; ++i) {
+          const bool cols = i < NQ ? QC : PC;
+          int a, c;
+          place(i < NQ ? i : i - NQ, i < NQ, a, c);
+          // elements of the chunk that are there
+          const int64_t have = cols ? (a < left ? (i < NQ ? leftq : leftp) - c * EPC : 0) : left - c * EPC;
+          F f;
+          if (have >= EPC) {
+            f = *reinterpret_cast<const Fu*>(src[i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < EPC; ++e) f[e] = e < have ? src[i][e] : (T)0.f;
+          }
+          reg[i] = __builtin_bit_cast(u32x4, f);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < NQ + NP; ++i) src[i] = reinterpret_cast<const T*>(reinterpret_cast<const char*>(src[i]) + (i < NQ ? stepq : stepp));
     }
     baseq += stepq;
     basep += stepp;
@@ -609,7 +633,8 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // (1.72 with column operands), 128x128 0.55 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone).  What the choice is
 // worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
 // round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
-// 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128 1.8, 64x64 0.48.
+// 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128
+// 2.3, 64x64 0.56.
 struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; double us; };
 constexpr double SPLIT_US = 10.0;      // see bwd_layout
 
@@ -621,8 +646,8 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
   const int64_t nkt = (K + kt - 1) / kt;
   const bool whole = esize == 2 && N % 8 == 0 && (form == GRAD_W ? M : K) % 8 == 0;
   struct Opt { int bm, bn; double step, alone; };
-  const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.48, esize == 2 ? 0.35 : 0.48},
-                       {128, 128, esize == 2 ? 0.55 : 1.8, esize == 2 ? 0.8 : 1.8},
+  const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.56, esize == 2 ? 0.35 : 0.56},
+                       {128, 128, esize == 2 ? 0.55 : 2.3, esize == 2 ? 0.8 : 2.3},
                        {256, 256, forward ? 1.55 : 1.72, 0.0},
                        {256, 320, forward ? 1.85 : 2.6, 0.0}};
   Plan best = {};
