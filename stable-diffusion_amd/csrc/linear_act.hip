@@ -628,7 +628,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // ---- host ------------------------------------------------------------------------------------------
 // Tile and split of a product: the least of an estimate in microseconds.  A CU works through ceil(workgroups / 256) of
 // them, each costing `step` per K-tile of 128 bytes and its stores (a CU's share of HBM, 20 KB a microsecond); a split
-// contraction stores fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.6
+// contraction stores fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.8
 // with a column operand, not for two: their addresses do not fit the registers beside 160 accumulators), 256x256 1.55
 // (1.72 with column operands), 128x128 0.55 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone).  What the choice is
 // worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
@@ -649,7 +649,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
   const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.56, esize == 2 ? 0.35 : 0.56},
                        {128, 128, esize == 2 ? 0.55 : 2.3, esize == 2 ? 0.8 : 2.3},
                        {256, 256, forward ? 1.55 : 1.72, 0.0},
-                       {256, 320, forward ? 1.85 : 2.6, 0.0}};
+                       {256, 320, forward ? 1.85 : 2.8, 0.0}};
   Plan best = {};
   double best_us = 1e30;
   const double out = (double)M * N;

@@ -343,8 +343,8 @@ def _first_derivative(backward):
 
 
 def _check_like(what, t, device, dtype, shape=None):
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, expected cuda:{device}")
     if t.dtype != dtype:
         raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
     if shape is not None and t.shape != shape:
@@ -352,10 +352,14 @@ def _check_like(what, t, device, dtype, shape=None):
 
 
 def _check_input(what, x):
-    if not x.is_cuda:
+    """Device number and dtype code of a differentiable call's input."""
+    device = x.get_device()
+    if device < 0:
         raise ValueError(f"{what} is on {x.device}: there is no CPU path")
-    if x.dtype not in _CODES:
+    code = _CODES.get(x.dtype)
+    if code is None:
         raise ValueError(f"{what} is {x.dtype}, expected float32, float16 or bfloat16")
+    return device, code
 
 
 def _check_columns(*counts):
@@ -365,25 +369,25 @@ def _check_columns(*counts):
 
 
 def _drop_state(p, seed, offset, device):
-    """(p, host seed, seed tensor or None, offset), checked."""
+    """((p, host seed, offset), seed tensor or None), checked."""
     p, offset = float(p), int(offset)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability {p} is not in [0, 1]")
     if not 0 <= offset < 1 << 32:
         raise ValueError(f"dropout offset {offset} does not fit 32 bits")
     if p == 0.0:
-        return 0.0, 0, None, 0
+        return (0.0, 0, 0), None
     if seed is None:
         raise ValueError("dropout needs a seed")
     if torch.is_tensor(seed):
         _check_like("seed", seed, device, torch.int64)
         if seed.numel() != 1:
             raise ValueError(f"seed holds {seed.numel()} numbers, expected one")
-        return p, 0, seed, offset
+        return (p, 0, offset), seed
     seed = int(seed)
     if not -(1 << 63) <= seed < 1 << 64:
         raise ValueError(f"seed {seed} does not fit 64 bits")
-    return p, seed, None, offset
+    return (p, seed, offset), None
 
 
 def _rows(t, cols):
@@ -397,38 +401,41 @@ def _rows(t, cols):
     return t, (t.stride(0) if rows > 1 else cols), rows
 
 
-def _dropout(x, resid, p, seed, seed_t, offset):
-    cols = x.shape[-1] if x.dim() else 1
-    out = x.new_empty(x.shape)
-    x2, ldx, rows = _rows(x, cols)
-    r2, ldr = (None, 0) if resid is None else _rows(resid, cols)[:2]
-    _run(x.get_device(), "sdmi_dropout", x2.data_ptr(), ldx, _p(r2), ldr, out.data_ptr(), rows, cols, p, seed, _p(seed_t),
-         offset, _CODES[x.dtype])
-    return out
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, resid, seed_t, p, seed, offset):
-        if seed_t is not None:
-            ctx.save_for_backward(seed_t)
-        ctx.args = (p, seed, offset, seed_t is not None) + ctx.needs_input_grad[:2]
-        return _dropout(x, resid, p, seed, seed_t, offset)
-
-    @staticmethod
-    @_first_derivative
-    def backward(ctx, dy):
-        p, seed, offset, seeded, need_x, need_r = ctx.args
-        dx = _dropout(dy, None, p, seed, ctx.saved_tensors[0] if seeded else None, offset) if need_x else None
-        return dx, (dy if need_r else None), None, None, None, None
-
-
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _dropout(x, resid, seed_t, args):
+    (p, seed, offset), device, dt = args
+    cols = x.shape[-1] if x.dim() else 1
+    out = x.new_empty(x.shape)
+    x2, ldx, rows = _rows(x, cols)
+    rp, ldr = None, 0
+    if resid is not None:
+        resid, ldr, _ = _rows(resid, cols)
+        rp = resid.data_ptr()
+    _run(device, "sdmi_dropout", x2.data_ptr(), ldx, rp, ldr, out.data_ptr(), rows, cols, p, seed, _p(seed_t), offset, dt)
+    return out
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, resid, seed_t, args):
+        if seed_t is not None:
+            ctx.save_for_backward(seed_t)
+        ctx.args = (args, seed_t is not None) + ctx.needs_input_grad[:2]
+        return _dropout(x, resid, seed_t, args)
+
+    @staticmethod
+    @_first_derivative
+    def backward(ctx, dy):
+        args, seeded, need_x, need_r = ctx.args
+        dx = _dropout(dy, None, ctx.saved_tensors[0] if seeded else None, args) if need_x else None
+        return dx, (dy if need_r else None), None, None
 
 
 def dropout(x, p, seed, offset=0, resid=None):
@@ -439,14 +446,15 @@ def dropout(x, p, seed, offset=0, resid=None):
     offset drop the same elements.  ``seed``: an integer of 64 bits, or a one-element int64 tensor on ``x``'s device
     (read when the kernel runs); ``offset``: one number per layer or call, below 2^32.  ``p`` counts in steps of
     2^-16, and the scale is that of the probability used.  Dropped elements are 0 whatever they held."""
-    _check_input("x", x)
+    device, dt = _check_input("x", x)
     _check_columns(*x.shape[-1:])
-    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
+    drop, seed_t = _drop_state(p, seed, offset, device)
     if resid is not None:
-        _check_like("resid", resid, x.device, x.dtype, x.shape)
+        _check_like("resid", resid, device, x.dtype, x.shape)
+    args = (drop, device, dt)
     if _wants_grad(x, resid):
-        return _DropoutFn.apply(x, resid, seed_t, p, seed, offset)
-    return _dropout(x, resid, p, seed, seed_t, offset)
+        return _DropoutFn.apply(x, resid, seed_t, args)
+    return _dropout(x, resid, seed_t, args)
 
 
 def noise_dropout(noise, p, seed=None, step=0):
@@ -461,39 +469,41 @@ def _workspace(nbytes, like):
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-def _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, want_preact):
+def _linear_act(x, w, bias, resid, seed_t, args, want_preact):
+    (p, seed, offset), device, dt, act = args
     n, k = w.shape
-    dt = _CODES[x.dtype]
     out = x.new_empty(x.shape[:-1] + (n,))
-    x2, ldx, rows = _rows(x, k)
-    w2, ldw, _ = _rows(w, k)
-    r2, ldr = (None, 0) if resid is None else _rows(resid, n)[:2]
+    x, ldx, rows = _rows(x, k)
+    w, ldw, _ = _rows(w, k)
+    rp, ldr = None, 0
+    if resid is not None:
+        resid, ldr, _ = _rows(resid, n)
+        rp = resid.data_ptr()
     preact = x.new_empty((rows, n), dtype=torch.float32) if want_preact else None
     ws = _workspace(_entry("sdmi_linear_act_workspace_bytes")(rows, k, n, dt), x)
-    _run(x.get_device(), "sdmi_linear_act", x2.data_ptr(), ldx, w2.data_ptr(), ldw, _p(bias), _p(r2), ldr, out.data_ptr(),
-         _p(preact), rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
+    _run(device, "sdmi_linear_act", x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), rp, ldr, out.data_ptr(), _p(preact),
+         rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
     return out, preact
 
 
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, resid, seed_t, act, p, seed, offset):
-        need_x, need_w, need_b, need_r = need = ctx.needs_input_grad[:4]
+    def forward(ctx, x, w, bias, resid, seed_t, args):
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         want = (1 if need_x else 0) | (2 if need_w else 0) | (4 if need_b else 0)
-        out, preact = _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, act != 0 and want != 0)
+        out, preact = _linear_act(x, w, bias, resid, seed_t, args, args[3] != 0 and want != 0)
         if want:
             ctx.save_for_backward(x if need_w else None, w if need_x else None, preact, seed_t)
-        ctx.args = (want, need_r, w.shape, x.shape, act, p, seed, offset)
+        ctx.args = (args, want, need_r, w.shape, x.shape)
         return out
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
-        want, need_r, (n, k), xshape, act, p, seed, offset = ctx.args
+        ((p, seed, offset), device, dt, act), want, need_r, (n, k), xshape = ctx.args
         dx = dw = db = None
         if want:
             x, w, preact, seed_t = ctx.saved_tensors
-            dt = _CODES[dy.dtype]
             d2, ldd, rows = _rows(dy, n)
             xp = wp = dxp = dwp = dbp = None
             ldx = ldw = 0
@@ -509,9 +519,9 @@ class _LinearActFn(torch.autograd.Function):
                 db = dy.new_empty((n,), dtype=torch.float32)
                 dbp = db.data_ptr()
             ws = _workspace(_entry("sdmi_linear_act_backward_workspace_bytes")(rows, k, n, act, p, want, dt), dy)
-            _run(dy.get_device(), "sdmi_linear_act_backward", d2.data_ptr(), ldd, _p(preact), xp, ldx, wp, ldw, dxp, dwp, dbp,
-                 rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
-        return dx, dw, db, (dy if need_r else None), None, None, None, None, None
+            _run(device, "sdmi_linear_act_backward", d2.data_ptr(), ldd, _p(preact), xp, ldx, wp, ldw, dxp, dwp, dbp, rows, k, n,
+                 act, p, seed, _p(seed_t), offset, _p(ws), dt)
+        return dx, dw, db, (dy if need_r else None), None, None
 
 
 def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0):
@@ -520,69 +530,63 @@ def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0
     x (..., K), w (N, K) and resid (..., N) in one dtype (fp32, fp16, bf16), bias fp32 (N,).  act: None, "silu",
     "gelu" (erf) or "quick_gelu" (z sigmoid(1.702 z)); p, seed, offset as in ``dropout``.  With an activation a
     training call keeps x w^T + bias in fp32.  Any sizes from one on; rows of whole 16-byte pieces are fastest."""
-    _check_input("x", x)
+    device, dt = _check_input("x", x)
     act = _act_code(act)
-    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
+    drop, seed_t = _drop_state(p, seed, offset, device)
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or 0 in w.shape:
         raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (..., K) and (N, K)")
-    _check_like("w", w, x.device, x.dtype)
+    _check_like("w", w, device, x.dtype)
     _check_columns(*w.shape)
     n = w.shape[0]
     if bias is not None:
-        _check_like("bias", bias, x.device, torch.float32, (n,))
+        _check_like("bias", bias, device, torch.float32, (n,))
         bias = bias.contiguous()
     if resid is not None:
-        _check_like("resid", resid, x.device, x.dtype, x.shape[:-1] + (n,))
+        _check_like("resid", resid, device, x.dtype, x.shape[:-1] + (n,))
+    args = (drop, device, dt, act)
     if _wants_grad(x, w, bias, resid):
-        return _LinearActFn.apply(x, w, bias, resid, seed_t, act, p, seed, offset)
-    return _linear_act(x, w, bias, resid, act, p, seed, seed_t, offset, False)[0]
+        return _LinearActFn.apply(x, w, bias, resid, seed_t, args)
+    return _linear_act(x, w, bias, resid, seed_t, args, False)[0]
 
 
-def _gn_sizes(x, x1):
-    b, hw = x.shape[0], 1
-    for s in x.shape[1:-1]:
-        hw *= s
-    return b, hw, x.shape[-1], 0 if x1 is None else x1.shape[-1]
-
-
-def _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset):
-    b, hw, c0, c1 = _gn_sizes(x, x1)
-    dt = _CODES[x.dtype]
-    out = x.new_empty(x.shape[:-1] + (c0 + c1,))
-    stats = x.new_empty((b, groups, 2), dtype=torch.float32)
+def _groupnorm_act(x, x1, gamma, beta, seed_t, args):
+    (p, seed, offset), device, dt, act, eps, groups, sizes, shape = args
+    b, hw, c0, c1 = sizes
+    out = x.new_empty(shape)
+    stats = gamma.new_empty((b, groups, 2))
     ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 0), x)
-    _run(x.get_device(), "sdmi_groupnorm_act", x.data_ptr(), c0, _p(x1), c1, b, hw, groups, eps, gamma.data_ptr(),
-         beta.data_ptr(), act, p, seed, _p(seed_t), offset, out.data_ptr(), stats.data_ptr(), _p(ws), dt)
+    _run(device, "sdmi_groupnorm_act", x.data_ptr(), c0, _p(x1), c1, b, hw, groups, eps, gamma.data_ptr(), beta.data_ptr(), act,
+         p, seed, _p(seed_t), offset, out.data_ptr(), stats.data_ptr(), _p(ws), dt)
     return out, stats
 
 
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, x1, gamma, beta, seed_t, eps, act, groups, p, seed, offset):
-        out, stats = _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset)
+    def forward(ctx, x, x1, gamma, beta, seed_t, args):
+        out, stats = _groupnorm_act(x, x1, gamma, beta, seed_t, args)
         ctx.save_for_backward(x, x1, gamma, beta, stats, seed_t)
-        ctx.args = (act, groups, p, seed, offset) + ctx.needs_input_grad[:4]
+        ctx.args = (args,) + ctx.needs_input_grad[:4]
         return out
 
     @staticmethod
     @_first_derivative
     def backward(ctx, dy):
+        args, need_x, need_x1, need_g, need_b = ctx.args
+        (p, seed, offset), device, dt, act, _, groups, (b, hw, c0, c1), _ = args
         x, x1, gamma, beta, stats, seed_t = ctx.saved_tensors
-        act, groups, p, seed, offset, need_x, need_x1, need_g, need_b = ctx.args
-        b, hw, c0, c1 = _gn_sizes(x, x1)
-        dt = _CODES[x.dtype]
         dy = dy.contiguous()
-        dx = dx1 = None
+        dx = dx1 = dgamma = dbeta = None
         if need_x or need_x1:
             dx = torch.empty_like(x)
             dx1 = None if x1 is None else torch.empty_like(x1)
-        dgamma = torch.empty_like(gamma) if need_g else None
-        dbeta = torch.empty_like(beta) if need_b else None
+        if need_g:
+            dgamma = torch.empty_like(gamma)
+        if need_b:
+            dbeta = torch.empty_like(beta)
         ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 1), x)
-        _run(x.get_device(), "sdmi_groupnorm_act_backward", dy.data_ptr(), x.data_ptr(), c0, _p(x1), c1, b, hw, groups,
-             gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1),
-             _p(dgamma), _p(dbeta), _p(ws), dt)
-        return (dx if need_x else None, dx1 if need_x1 else None, dgamma, dbeta, None, None, None, None, None, None, None)
+        _run(device, "sdmi_groupnorm_act_backward", dy.data_ptr(), x.data_ptr(), c0, _p(x1), c1, b, hw, groups, gamma.data_ptr(),
+             beta.data_ptr(), stats.data_ptr(), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1), _p(dgamma), _p(dbeta), _p(ws), dt)
+        return (dx if need_x else None), (dx1 if need_x1 else None), dgamma, dbeta, None, None
 
 
 def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.0, seed=None, offset=0):
@@ -591,24 +595,29 @@ def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.
     x (B, ..., C0) [and x1 (B, ..., C1), concatenated behind it] -> (B, ..., C0 + C1); gamma, beta fp32 (C0 + C1,).
     act as in ``linear_act``, p / seed / offset as in ``dropout`` (a pixel is a row).  Any number of channels per
     group (8192 channels in all at most) and any image size; ``groupnorm`` is the inference path's own kernel."""
-    _check_input("x", x)
+    device, dt = _check_input("x", x)
     act = _act_code(act)
-    p, seed, seed_t, offset = _drop_state(p, seed, offset, x.device)
-    if x.dim() < 2:
-        raise ValueError(f"x {tuple(x.shape)} has no batch and channel dimension")
-    c = x.shape[-1]
+    drop, seed_t = _drop_state(p, seed, offset, device)
+    shape, groups = x.shape, int(groups)
+    if len(shape) < 2:
+        raise ValueError(f"x {tuple(shape)} has no batch and channel dimension")
+    b, c0, c1 = shape[0], shape[-1], 0
     if x1 is not None:
-        _check_like("x1", x1, x.device, x.dtype, x.shape[:-1] + (x1.shape[-1] if x1.dim() else 0,))
-        c += x1.shape[-1]
-        x1 = x1.contiguous() if x1.shape[-1] else None
-    groups = int(groups)
-    if c == 0 or x.shape[-1] == 0 or groups < 1 or c % groups:
+        c1 = x1.shape[-1] if x1.dim() else 0
+        _check_like("x1", x1, device, x.dtype, shape[:-1] + (c1,))
+        x1 = x1.contiguous() if c1 else None
+    c = c0 + c1
+    if c0 == 0 or groups < 1 or c % groups:
         raise ValueError(f"{c} channels do not split into {groups} groups")
-    if c > 8192 or x.shape[0] > 65535:
-        raise ValueError(f"batch {x.shape[0]} of {c} channels: at most 65535 and 8192 are supported")
-    _check_like("gamma", gamma, x.device, torch.float32, (c,))
-    _check_like("beta", beta, x.device, torch.float32, (c,))
-    x, gamma, beta, eps = x.contiguous(), gamma.contiguous(), beta.contiguous(), float(eps)
+    if c > 8192 or b > 65535:
+        raise ValueError(f"batch {b} of {c} channels: at most 65535 and 8192 are supported")
+    _check_like("gamma", gamma, device, torch.float32, (c,))
+    _check_like("beta", beta, device, torch.float32, (c,))
+    hw = 1
+    for s in shape[1:-1]:
+        hw *= s
+    x, gamma, beta = x.contiguous(), gamma.contiguous(), beta.contiguous()
+    args = (drop, device, dt, act, float(eps), groups, (b, hw, c0, c1), shape if c1 == 0 else shape[:-1] + (c,))
     if _wants_grad(x, x1, gamma, beta):
-        return _GroupNormActFn.apply(x, x1, gamma, beta, seed_t, eps, act, groups, p, seed, offset)
-    return _groupnorm_act(x, x1, gamma, beta, eps, act, groups, p, seed, seed_t, offset)[0]
+        return _GroupNormActFn.apply(x, x1, gamma, beta, seed_t, args)
+    return _groupnorm_act(x, x1, gamma, beta, seed_t, args)[0]

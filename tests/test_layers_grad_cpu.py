@@ -112,7 +112,7 @@ def test_python_refuses_cpu_tensors_and_bad_arguments():
         ops.linear_act(x, w)
     with pytest.raises(ValueError, match="CPU"):
         ops.groupnorm_act(x.view(1, 4, 8), torch.ones(8), torch.zeros(8), groups=2)
-    dev = torch.device("cpu")
+    dev = -1                                # a CPU tensor's device number
     for p in (-0.1, 1.1, float("nan")):
         with pytest.raises(ValueError, match="probability"):
             ops._drop_state(p, 1, 0, dev)
