@@ -490,6 +490,73 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   }
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------
+// Forward for a handful of tokens: the weights pass through once and nothing is shared, so nothing goes through LDS on
+// the way.  A workgroup takes 16 columns; its eight waves share the contraction in steps of one fragment, four steps' loads
+// in flight each, and meet in LDS.  One launch, no workspace.
+template <typename T, int FQ>
+__global__ __launch_bounds__(512) void linear_few_kernel(GemmParams p) {
+  typedef typename Frag<T>::type F;
+  typedef F Fu __attribute__((aligned(sizeof(T))));
+  constexpr int EPC = 16 / (int)sizeof(T), STEP = 4 * EPC, NW = 8, U = 4, PITCH = 20;
+  __shared__ __align__(16) float red[NW][16 * FQ][PITCH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int n0 = (int)blockIdx.x * 16, M = (int)p.e.M;
+  const T* wrow = reinterpret_cast<const T*>(p.p) + (int64_t)(n0 + r < p.e.N ? n0 + r : p.e.N - 1) * p.ldp;
+  const T* xrow[FQ];
+#pragma unroll
+  for (int j = 0; j < FQ; ++j) xrow[j] = reinterpret_cast<const T*>(p.q) + (int64_t)min(j * 16 + r, M - 1) * p.ldq;
+  f32x4 acc[FQ];
+#pragma unroll
+  for (int j = 0; j < FQ; ++j) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  auto chunk = [&](const T* row, int64_t k) -> F {       // indices k .. k + EPC - 1, zeros beyond the end
+    if (k + EPC <= p.K) return *reinterpret_cast<const Fu*>(row + k);
+    F f;
+#pragma unroll
+    for (int e = 0; e < EPC; ++e) f[e] = k + e < p.K ? row[k + e] : (T)0.f;
+    return f;
+  };
+  const int64_t whole = p.K - p.K % STEP;                // steps without an end in them
+  int64_t k = (int64_t)wave * STEP + g * EPC;
+  for (; k - g * EPC + (U - 1) * NW * STEP < whole; k += U * NW * STEP) {
+    F w[U], x[U][FQ];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = *reinterpret_cast<const Fu*>(wrow + k + u * NW * STEP);
+#pragma unroll
+      for (int j = 0; j < FQ; ++j) x[u][j] = *reinterpret_cast<const Fu*>(xrow[j] + k + u * NW * STEP);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < FQ; ++j) acc[j] = mma(w[u], x[u][j], acc[j]);
+  }
+  for (; k - g * EPC < p.K; k += NW * STEP) {
+    const F w = chunk(wrow, k);
+#pragma unroll
+    for (int j = 0; j < FQ; ++j) acc[j] = mma(w, chunk(xrow[j], k), acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < FQ; ++j) *reinterpret_cast<f32x4*>(&red[wave][j * 16 + r][g * 4]) = acc[j];
+  __syncthreads();
+  const int row = threadIdx.x >> 1, n = n0 + (threadIdx.x & 1) * 8;
+  if (row >= M || n >= p.e.N) return;
+  float v[8], res[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < NW; ++s) v[e] += red[s][row][(threadIdx.x & 1) * 8 + e];
+  }
+  unsigned k0 = 0, k1 = 0;
+  if (p.e.drop.thr) drop_key(p.e.drop, k0, k1);
+  if (p.e.resid) load8<T>((const T*)p.e.resid + row * p.e.ldr + n, p.e.N - n, res);
+  finish8<T, true>(p.e, k0, k1, row, n, res, v);
+}
+// where it beats the tiles (us, replayed, few / tiles): fp16 32x1280x1280 5.8 / 9.0, 16x2560x640 6.8 / 6.8,
+// 8x5120x1280 9.6 / 8.0; fp32 2x1280x1280 5.8 / 8.6, 16x2560x640 11.3 / 9.3
+bool few_rows(int64_t rows, int64_t k, int esize) { return rows <= 32 && k * esize * (8 + rows) <= (128 << 10); }
+
 // ---- joins -----------------------------------------------------------------------------------------
 // Sum of the splits in a fixed order, then the epilogue.  A group of eight columns is summed by LANES threads, each over
 // every LANES-th split (four loads in flight), and finished by the first of them.
@@ -663,7 +730,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
       const double load = (double)((tiles * used + 255) / 256);
       double us = load * t.step > t.alone ? load * t.step : t.alone;
       us = us * per + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
-      if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 4.0;
+      if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 6.0;
       if (us < best_us) {
         best_us = us;
         best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt, us};
@@ -833,6 +900,20 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
   return SDMI_OK;
 }
 
+template <typename T>
+int linear_few(const LinearActArgs& a, const Epilogue& e, hipStream_t s) {
+  GemmParams g = {};
+  g.q = (const char*)a.x; g.p = (const char*)a.w; g.ldq = a.ldx; g.ldp = a.ldw; g.K = a.k; g.e = e;
+  char label[96];
+  snprintf(label, sizeof(label), "linear M%lld N%d K%d", (long long)a.rows, a.n, a.k);
+  ProfScope prof(PROF_OTHER, s, 2.0 * a.rows * (double)a.n * a.k, (double)a.n * a.k * sizeof(T), label);
+  const dim3 grid((unsigned)(a.n + 15) / 16);
+  if (a.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, dim3(512), 0, s, g);
+  SDMI_CHECK_HIP(hipGetLastError());
+  return SDMI_OK;
+}
+
 int check_common(const LinearActArgs& a, const char* who) {
   SDMI_REQUIRE(a.dtype >= 0 && a.dtype <= 2, "%s: bad dtype %d", who, a.dtype);
   SDMI_REQUIRE(a.rows >= 0 && a.k > 0 && a.n > 0, "%s: bad size (%lld rows, %d inputs, %d outputs)", who,
@@ -846,7 +927,7 @@ int check_common(const LinearActArgs& a, const char* who) {
 }  // namespace
 
 int64_t linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype) {
-  if (rows <= 0 || k <= 0 || n <= 0) return 0;
+  if (rows <= 0 || k <= 0 || n <= 0 || few_rows(rows, k, (int)sdmi_dtype_size(dtype))) return 0;
   return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype), FORWARD), rows, n);
 }
 int64_t linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype) {
@@ -864,6 +945,7 @@ int linear_act(const LinearActArgs& a, hipStream_t stream) {
   SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %lld bytes", (long long)need);
   e.bias = a.bias; e.resid = a.resid; e.ldr = a.ldr; e.out = a.out; e.ldo = a.n;
   e.alpha = 1.f; e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
+  if (few_rows(a.rows, a.k, (int)sdmi_dtype_size(a.dtype))) { SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_few<T>(a, e, stream)); }
   SDMI_DISPATCH_DTYPE(a.dtype, T, return (product<T, false, false>(a.x, nullptr, a.ldx, a.w, a.ldw, a.k, e,
                                                                      (float*)a.workspace, DbFold(), stream)));
   return SDMI_OK;

@@ -97,6 +97,9 @@ LINEAR = [  # m, k, n, act, bias, resid, p
     (300, 2048, 64, "gelu", True, True, 0.1),
     (1000, 520, 264, "gelu", True, True, 0.1),
     (4096, 40, 24, None, True, False, 0.3),
+    (31, 1000, 77, "gelu", True, True, 0.2),
+    (9, 3, 1000, None, True, True, 0.5),
+    (32, 4000, 17, "silu", False, True, 0.0),
     (2100, 320, 1288, "silu", True, False, 0.1),
 ]
 
