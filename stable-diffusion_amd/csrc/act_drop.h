@@ -7,8 +7,8 @@
 // offset).  One call gives four 32-bit words = eight 16-bit numbers, one per column 8 j .. 8 j + 7, low half first.
 // Element kept if its number >= thr = round(p 65536); kept values are scaled by 65536 / (65536 - thr), the reciprocal
 // of the probability that is really used, so the expectation is exact.  16 bits per element keep the generator
-// below the memory time: a call costs about 20 quarter-rate multiplies, a third of the time that a wave's eight
-// elements per lane take to come from and go to HBM.
+// below the memory time: a call is about 480 cycles of a wave (20 quarter-rate multiplies, 20 three-input XORs), half of
+// what eight 16-bit elements per lane take to come from and go to HBM; 32 bits per element would take as long as they do.
 #pragma once
 #include "common.h"
 

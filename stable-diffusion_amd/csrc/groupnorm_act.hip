@@ -9,6 +9,12 @@
 // the first leaves per-strip sums, the second folds them in double and finishes the strip.  Every sum is taken in a
 // fixed order.  Statistics are taken about a value of the group (its first one), so that a common offset does not
 // cancel in E[x^2] - E[x]^2.
+//
+// Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 12 us (HBM: 8), apply 23, gradient
+// sums 23, gradient apply 25 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
+// (480) and the SiLU (its exponential and reciprocal at a quarter of the rate) of 512 elements, 20 us in all, where HBM
+// would take 16, 16 and 24.  3x37x53x480 fp32: 7, 9, 9 and 9 us, launches and the fold of the strips.  One workgroup per
+// slice: 2x8x8x1280 fp16 forward 5.6 us, 16x16x16x1280 bf16 12 forward, 23 backward.
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
