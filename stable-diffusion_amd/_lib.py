@@ -6,9 +6,11 @@ raises.  ``build()`` compiles the library in-tree with hipcc for gfx950.
 import ctypes
 import os
 import subprocess
+import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SDMI_LIB") or os.path.join(_HERE, "libsdmi.so")
+LAYERS_PATH = os.path.join(_HERE, "sdmi_layers.so")
 CSRC = os.path.join(_HERE, "csrc")
 
 c_void_p, c_int, c_float, c_int64, c_char_p = (ctypes.c_void_p, ctypes.c_int, ctypes.c_float,
@@ -145,13 +147,13 @@ _lib = None
 
 
 def build(verbose=False, jobs=8):
-    """Compile libsdmi.so in-tree (hipcc, --offload-arch=gfx950)."""
-    cmd = ["make", "-C", CSRC, f"-j{jobs}"]
+    """Compile libsdmi.so (hipcc, --offload-arch=gfx950) and sdmi_layers.so in-tree."""
+    cmd = ["make", "-C", CSRC, f"-j{jobs}", f"PYTHON={sys.executable or 'python3'}"]
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout)
     if res.returncode != 0:
-        raise RuntimeError("building libsdmi.so failed (see output above)")
+        raise RuntimeError("building libsdmi.so and sdmi_layers.so failed (see output above)")
     return LIB_PATH
 
 
@@ -171,6 +173,27 @@ def lib():
             fn.argtypes = args
         _lib = l
     return _lib
+
+
+_layers = None
+
+
+def layers():
+    """The torch side of the layers with gradients (csrc/torch_layers.cpp), bound to the loaded library."""
+    global _layers
+    if _layers is None:
+        import importlib.util
+        import torch  # noqa: F401  (its libraries are what the module links against)
+        if not os.path.exists(LAYERS_PATH):
+            raise RuntimeError(f"{LAYERS_PATH} is missing: build it with `make -C {CSRC}`")
+        spec = importlib.util.spec_from_file_location("sdmi_layers", LAYERS_PATH)
+        m = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(m)
+        l = lib()
+        m.bind({n: ctypes.cast(getattr(l, n), c_void_p).value for n in SIGNATURES
+                if n == "sdmi_last_error" or n.startswith(("sdmi_dropout", "sdmi_linear_act", "sdmi_groupnorm_act"))})
+        _layers = m
+    return _layers
 
 
 def check(code, what=""):

@@ -293,151 +293,6 @@ def inpaint_composite(image, mask, predicted):
 # there a `seed` in device memory makes every replay draw anew.  Capture a backward pass together with its forward
 # pass, and with no eager graph of the same leaves alive (torch joins the streams of a leaf's graphs).
 
-_ACTS = {None: 0, "silu": 1, "gelu": 2, "quick_gelu": 3}
-
-
-def _act_code(act):
-    if act not in _ACTS:
-        raise ValueError(f"unknown activation {act!r}: one of {list(_ACTS)}")
-    return _ACTS[act]
-
-
-# The wrappers below cost as much as the kernels of a small call, and backward passes run in a thread of torch's own, on
-# cold caches: hence the table of entry points, the raw device and stream queries (the Stream object that
-# torch.cuda.current_stream builds costs 3 us, and 16 us there) and what forward leaves ready in ctx.
-_CODES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
-_ENTRIES = {}
-
-
-def _entry(name):
-    fn = _ENTRIES.get(name)
-    if fn is None:
-        fn = _ENTRIES[name] = getattr(_lib.lib(), name)
-    return fn
-
-
-def _run(device, name, *args):
-    """One call of the library on the current stream of device number ``device``."""
-    fn = _ENTRIES.get(name) or _entry(name)
-    if device == torch._C._cuda_getDevice():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(device))
-    if code:
-        check(code, name)
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
-
-
-def _first_derivative(backward):
-    """A backward pass whose results carry no graph: torch's once_differentiable where a graph is wanted of it (it
-    then raises when that graph is used), the plain function otherwise (the wrapper costs 25 us a call)."""
-    once = torch.autograd.function.once_differentiable(backward)
-
-    def call(ctx, dy):
-        return once(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
-    return call
-
-
-def _check_like(what, t, device, dtype, shape=None):
-    if t.get_device() != device:
-        raise ValueError(f"{what} is on {t.device}, expected cuda:{device}")
-    if t.dtype != dtype:
-        raise ValueError(f"{what} is {t.dtype}, expected {dtype}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-
-
-def _check_input(what, x):
-    """Device number and dtype code of a differentiable call's input."""
-    device = x.get_device()
-    if device < 0:
-        raise ValueError(f"{what} is on {x.device}: there is no CPU path")
-    code = _CODES.get(x.dtype)
-    if code is None:
-        raise ValueError(f"{what} is {x.dtype}, expected float32, float16 or bfloat16")
-    return device, code
-
-
-def _check_columns(*counts):
-    for n in counts:
-        if n > 1 << 30:
-            raise ValueError(f"rows of {n} columns are too long: at most 2^30")
-
-
-def _drop_state(p, seed, offset, device):
-    """((p, host seed, offset), seed tensor or None), checked."""
-    p, offset = float(p), int(offset)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"dropout probability {p} is not in [0, 1]")
-    if not 0 <= offset < 1 << 32:
-        raise ValueError(f"dropout offset {offset} does not fit 32 bits")
-    if p == 0.0:
-        return (0.0, 0, 0), None
-    if seed is None:
-        raise ValueError("dropout needs a seed")
-    if torch.is_tensor(seed):
-        _check_like("seed", seed, device, torch.int64)
-        if seed.numel() != 1:
-            raise ValueError(f"seed holds {seed.numel()} numbers, expected one")
-        return (p, 0, offset), seed
-    seed = int(seed)
-    if not -(1 << 63) <= seed < 1 << 64:
-        raise ValueError(f"seed {seed} does not fit 64 bits")
-    return (p, seed, offset), None
-
-
-def _rows(t, cols):
-    """``t`` as (rows, cols) with unit column stride (a view where the strides allow it), its row stride, rows."""
-    if t.is_contiguous():
-        return t, cols, t.numel() // cols if cols else 0
-    rows = t.numel() // cols
-    t = t.reshape(rows, cols)
-    if cols > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else cols), rows
-
-
-def _wants_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-def _dropout(x, resid, seed_t, args):
-    (p, seed, offset), device, dt = args
-    cols = x.shape[-1] if x.dim() else 1
-    out = x.new_empty(x.shape)
-    x2, ldx, rows = _rows(x, cols)
-    rp, ldr = None, 0
-    if resid is not None:
-        resid, ldr, _ = _rows(resid, cols)
-        rp = resid.data_ptr()
-    _run(device, "sdmi_dropout", x2.data_ptr(), ldx, rp, ldr, out.data_ptr(), rows, cols, p, seed, _p(seed_t), offset, dt)
-    return out
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, resid, seed_t, args):
-        if seed_t is not None:
-            ctx.save_for_backward(seed_t)
-        ctx.args = (args, seed_t is not None) + ctx.needs_input_grad[:2]
-        return _dropout(x, resid, seed_t, args)
-
-    @staticmethod
-    @_first_derivative
-    def backward(ctx, dy):
-        args, seeded, need_x, need_r = ctx.args
-        dx = _dropout(dy, None, ctx.saved_tensors[0] if seeded else None, args) if need_x else None
-        return dx, (dy if need_r else None), None, None
-
-
 def dropout(x, p, seed, offset=0, resid=None):
     """Dropout with a counter-based mask that is never stored: ``[resid +] keep * x / (1 - p)``, differentiable.
 
@@ -446,15 +301,7 @@ def dropout(x, p, seed, offset=0, resid=None):
     offset drop the same elements.  ``seed``: an integer of 64 bits, or a one-element int64 tensor on ``x``'s device
     (read when the kernel runs); ``offset``: one number per layer or call, below 2^32.  ``p`` counts in steps of
     2^-16, and the scale is that of the probability used.  Dropped elements are 0 whatever they held."""
-    device, dt = _check_input("x", x)
-    _check_columns(*x.shape[-1:])
-    drop, seed_t = _drop_state(p, seed, offset, device)
-    if resid is not None:
-        _check_like("resid", resid, device, x.dtype, x.shape)
-    args = (drop, device, dt)
-    if _wants_grad(x, resid):
-        return _DropoutFn.apply(x, resid, seed_t, args)
-    return _dropout(x, resid, seed_t, args)
+    return _lib.layers().dropout(x, p, seed, offset, resid)
 
 
 def noise_dropout(noise, p, seed=None, step=0):
@@ -465,128 +312,13 @@ def noise_dropout(noise, p, seed=None, step=0):
     return dropout(noise, p, seed, step)
 
 
-def _workspace(nbytes, like):
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-
-
-def _linear_act(x, w, bias, resid, seed_t, args, want_preact):
-    (p, seed, offset), device, dt, act = args
-    n, k = w.shape
-    out = x.new_empty(x.shape[:-1] + (n,))
-    x, ldx, rows = _rows(x, k)
-    w, ldw, _ = _rows(w, k)
-    rp, ldr = None, 0
-    if resid is not None:
-        resid, ldr, _ = _rows(resid, n)
-        rp = resid.data_ptr()
-    preact = x.new_empty((rows, n), dtype=torch.float32) if want_preact else None
-    ws = _workspace(_entry("sdmi_linear_act_workspace_bytes")(rows, k, n, dt), x)
-    _run(device, "sdmi_linear_act", x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), rp, ldr, out.data_ptr(), _p(preact),
-         rows, k, n, act, p, seed, _p(seed_t), offset, _p(ws), dt)
-    return out, preact
-
-
-class _LinearActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, bias, resid, seed_t, args):
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        want = (1 if need_x else 0) | (2 if need_w else 0) | (4 if need_b else 0)
-        out, preact = _linear_act(x, w, bias, resid, seed_t, args, args[3] != 0 and want != 0)
-        if want:
-            ctx.save_for_backward(x if need_w else None, w if need_x else None, preact, seed_t)
-        ctx.args = (args, want, need_r, w.shape, x.shape)
-        return out
-
-    @staticmethod
-    @_first_derivative
-    def backward(ctx, dy):
-        ((p, seed, offset), device, dt, act), want, need_r, (n, k), xshape = ctx.args
-        dx = dw = db = None
-        if want:
-            x, w, preact, seed_t = ctx.saved_tensors
-            d2, ldd, rows = _rows(dy, n)
-            xp = wp = dxp = dwp = dbp = None
-            ldx = ldw = 0
-            if want & 1:
-                w, ldw, _ = _rows(w, k)
-                dx = dy.new_empty(xshape)
-                wp, dxp = w.data_ptr(), dx.data_ptr()
-            if want & 2:
-                x, ldx, _ = _rows(x, k)
-                dw = dy.new_empty((n, k))
-                xp, dwp = x.data_ptr(), dw.data_ptr()
-            if want & 4:
-                db = dy.new_empty((n,), dtype=torch.float32)
-                dbp = db.data_ptr()
-            ws = _workspace(_entry("sdmi_linear_act_backward_workspace_bytes")(rows, k, n, act, p, want, dt), dy)
-            _run(device, "sdmi_linear_act_backward", d2.data_ptr(), ldd, _p(preact), xp, ldx, wp, ldw, dxp, dwp, dbp, rows, k, n,
-                 act, p, seed, _p(seed_t), offset, _p(ws), dt)
-        return dx, dw, db, (dy if need_r else None), None, None
-
-
 def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0):
     """``[resid +] dropout(act(x w^T + bias))``, differentiable in x, w, bias and resid.
 
     x (..., K), w (N, K) and resid (..., N) in one dtype (fp32, fp16, bf16), bias fp32 (N,).  act: None, "silu",
     "gelu" (erf) or "quick_gelu" (z sigmoid(1.702 z)); p, seed, offset as in ``dropout``.  With an activation a
     training call keeps x w^T + bias in fp32.  Any sizes from one on; rows of whole 16-byte pieces are fastest."""
-    device, dt = _check_input("x", x)
-    act = _act_code(act)
-    drop, seed_t = _drop_state(p, seed, offset, device)
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1] or 0 in w.shape:
-        raise ValueError(f"x {tuple(x.shape)} and w {tuple(w.shape)} do not fit (..., K) and (N, K)")
-    _check_like("w", w, device, x.dtype)
-    _check_columns(*w.shape)
-    n = w.shape[0]
-    if bias is not None:
-        _check_like("bias", bias, device, torch.float32, (n,))
-        bias = bias.contiguous()
-    if resid is not None:
-        _check_like("resid", resid, device, x.dtype, x.shape[:-1] + (n,))
-    args = (drop, device, dt, act)
-    if _wants_grad(x, w, bias, resid):
-        return _LinearActFn.apply(x, w, bias, resid, seed_t, args)
-    return _linear_act(x, w, bias, resid, seed_t, args, False)[0]
-
-
-def _groupnorm_act(x, x1, gamma, beta, seed_t, args):
-    (p, seed, offset), device, dt, act, eps, groups, sizes, shape = args
-    b, hw, c0, c1 = sizes
-    out = x.new_empty(shape)
-    stats = gamma.new_empty((b, groups, 2))
-    ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 0), x)
-    _run(device, "sdmi_groupnorm_act", x.data_ptr(), c0, _p(x1), c1, b, hw, groups, eps, gamma.data_ptr(), beta.data_ptr(), act,
-         p, seed, _p(seed_t), offset, out.data_ptr(), stats.data_ptr(), _p(ws), dt)
-    return out, stats
-
-
-class _GroupNormActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, x1, gamma, beta, seed_t, args):
-        out, stats = _groupnorm_act(x, x1, gamma, beta, seed_t, args)
-        ctx.save_for_backward(x, x1, gamma, beta, stats, seed_t)
-        ctx.args = (args,) + ctx.needs_input_grad[:4]
-        return out
-
-    @staticmethod
-    @_first_derivative
-    def backward(ctx, dy):
-        args, need_x, need_x1, need_g, need_b = ctx.args
-        (p, seed, offset), device, dt, act, _, groups, (b, hw, c0, c1), _ = args
-        x, x1, gamma, beta, stats, seed_t = ctx.saved_tensors
-        dy = dy.contiguous()
-        dx = dx1 = dgamma = dbeta = None
-        if need_x or need_x1:
-            dx = torch.empty_like(x)
-            dx1 = None if x1 is None else torch.empty_like(x1)
-        if need_g:
-            dgamma = torch.empty_like(gamma)
-        if need_b:
-            dbeta = torch.empty_like(beta)
-        ws = _workspace(_entry("sdmi_groupnorm_act_workspace_bytes")(b, hw, c0, c1, groups, dt, 1), x)
-        _run(device, "sdmi_groupnorm_act_backward", dy.data_ptr(), x.data_ptr(), c0, _p(x1), c1, b, hw, groups, gamma.data_ptr(),
-             beta.data_ptr(), stats.data_ptr(), act, p, seed, _p(seed_t), offset, _p(dx), _p(dx1), _p(dgamma), _p(dbeta), _p(ws), dt)
-        return (dx if need_x else None), (dx1 if need_x1 else None), dgamma, dbeta, None, None
+    return _lib.layers().linear_act(x, w, bias, act, resid, p, seed, offset)
 
 
 def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.0, seed=None, offset=0):
@@ -595,29 +327,4 @@ def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.
     x (B, ..., C0) [and x1 (B, ..., C1), concatenated behind it] -> (B, ..., C0 + C1); gamma, beta fp32 (C0 + C1,).
     act as in ``linear_act``, p / seed / offset as in ``dropout`` (a pixel is a row).  Any number of channels per
     group (8192 channels in all at most) and any image size; ``groupnorm`` is the inference path's own kernel."""
-    device, dt = _check_input("x", x)
-    act = _act_code(act)
-    drop, seed_t = _drop_state(p, seed, offset, device)
-    shape, groups = x.shape, int(groups)
-    if len(shape) < 2:
-        raise ValueError(f"x {tuple(shape)} has no batch and channel dimension")
-    b, c0, c1 = shape[0], shape[-1], 0
-    if x1 is not None:
-        c1 = x1.shape[-1] if x1.dim() else 0
-        _check_like("x1", x1, device, x.dtype, shape[:-1] + (c1,))
-        x1 = x1.contiguous() if c1 else None
-    c = c0 + c1
-    if c0 == 0 or groups < 1 or c % groups:
-        raise ValueError(f"{c} channels do not split into {groups} groups")
-    if c > 8192 or b > 65535:
-        raise ValueError(f"batch {b} of {c} channels: at most 65535 and 8192 are supported")
-    _check_like("gamma", gamma, device, torch.float32, (c,))
-    _check_like("beta", beta, device, torch.float32, (c,))
-    hw = 1
-    for s in shape[1:-1]:
-        hw *= s
-    x, gamma, beta = x.contiguous(), gamma.contiguous(), beta.contiguous()
-    args = (drop, device, dt, act, float(eps), groups, (b, hw, c0, c1), shape if c1 == 0 else shape[:-1] + (c,))
-    if _wants_grad(x, x1, gamma, beta):
-        return _GroupNormActFn.apply(x, x1, gamma, beta, seed_t, args)
-    return _groupnorm_act(x, x1, gamma, beta, seed_t, args)[0]
+    return _lib.layers().groupnorm_act(x, gamma, beta, eps, act, x1, groups, p, seed, offset)

@@ -112,21 +112,37 @@ def test_python_refuses_cpu_tensors_and_bad_arguments():
         ops.linear_act(x, w)
     with pytest.raises(ValueError, match="CPU"):
         ops.groupnorm_act(x.view(1, 4, 8), torch.ones(8), torch.zeros(8), groups=2)
-    dev = -1                                # a CPU tensor's device number
-    for p in (-0.1, 1.1, float("nan")):
-        with pytest.raises(ValueError, match="probability"):
-            ops._drop_state(p, 1, 0, dev)
-    with pytest.raises(ValueError, match="needs a seed"):
-        ops._drop_state(0.5, None, 0, dev)
-    with pytest.raises(ValueError, match="offset"):
-        ops._drop_state(0.5, 1, 1 << 32, dev)
-    with pytest.raises(ValueError, match="64 bits"):
-        ops._drop_state(0.5, 1 << 64, 0, dev)
-    with pytest.raises(ValueError, match="int64"):
-        ops._drop_state(0.5, torch.zeros(1), 0, dev)
-    with pytest.raises(ValueError, match="one"):
-        ops._drop_state(0.5, torch.zeros(2, dtype=torch.int64), 0, dev)
-    with pytest.raises(ValueError, match="2\\^30"):
-        ops._check_columns(8, (1 << 30) + 1)
     with pytest.raises(ValueError, match="activation"):
-        ops._act_code("relu")
+        ops.linear_act(x, w, act="relu")
+    with pytest.raises(ValueError, match="do not fit"):
+        ops.linear_act(x, w[:, :7])
+    with pytest.raises(ValueError, match="do not fit"):
+        ops.linear_act(x, w[:0])
+    calls = [lambda **kw: ops.dropout(x, **kw), lambda **kw: ops.linear_act(x, w, **kw),
+             lambda **kw: ops.groupnorm_act(x.view(1, 4, 8), torch.ones(8), torch.zeros(8), groups=2, **kw)]
+    for call in calls:
+        for p in (-0.1, 1.1, float("nan")):
+            with pytest.raises(ValueError, match="probability"):
+                call(p=p, seed=1)
+        with pytest.raises(ValueError, match="needs a seed"):
+            call(p=0.5, seed=None)
+        with pytest.raises(ValueError, match="offset"):
+            call(p=0.5, seed=1, offset=1 << 32)
+        with pytest.raises(ValueError, match="offset"):
+            call(p=0.5, seed=1, offset=-1)
+        for seed in (1 << 64, -(1 << 63) - 1):
+            with pytest.raises(ValueError, match="64 bits"):
+                call(p=0.5, seed=seed)
+        with pytest.raises(ValueError, match="float32, expected int64"):
+            call(p=0.5, seed=torch.zeros(1))
+        with pytest.raises(ValueError, match="one"):
+            call(p=0.5, seed=torch.zeros(2, dtype=torch.int64))
+        with pytest.raises(TypeError):
+            call(p=0.5, seed="7")
+        for seed in (-(1 << 63), (1 << 64) - 1, np.int64(3), torch.zeros((), dtype=torch.int64)):
+            with pytest.raises(ValueError, match="CPU"):             # a seed like that is none of its refusals
+                call(p=0.5, seed=seed)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.dropout(x[0, :1].expand((1 << 30) + 1), 0.5, 1)
+    with pytest.raises(ValueError, match="2\\^30"):
+        ops.linear_act(x[:, :1], w[:1, :1].expand((1 << 30) + 1, 1))

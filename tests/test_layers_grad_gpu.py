@@ -497,3 +497,63 @@ def test_samplers_noise_dropout_by_seed():
                               unconditional_guidance_scale=7.5, unconditional_conditioning=True,
                               noise_fn=lambda s: noise, noise_dropout_seed=1)
     assert torch.equal(lat, again)
+
+
+def _layer_calls():
+    x, w, b, g, h = rand(6, 16, grad=True), rand(24, 16, grad=True), rand(24), rand(16), rand(16)
+    return x, {"dropout": lambda: ops.dropout(x, 0.5, 3),
+               "linear": lambda: ops.linear_act(x, w, b, act="gelu", p=0.25, seed=3),
+               "groupnorm": lambda: ops.groupnorm_act(x.view(2, 3, 16), g, h, groups=4, p=0.25, seed=3)}
+
+
+@pytest.mark.parametrize("layer", ["dropout", "linear", "groupnorm"])
+def test_autograd_refuses_what_the_layers_have_not(layer):
+    x, calls = _layer_calls()
+    call = calls[layer]
+    g, = torch.autograd.grad(call().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        g.sum().backward()
+    if layer != "dropout":                                  # (dropout keeps nothing that a first pass could free)
+        y = call().sum()
+        y.backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            y.backward()
+        y = call().sum()
+        with torch.no_grad():
+            x.mul_(1.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        t = fw.make_dual(x.detach(), torch.ones_like(x))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            if layer == "dropout":
+                ops.dropout(t, 0.5, 3)
+            elif layer == "linear":
+                ops.linear_act(t, rand(24, 16))
+            else:
+                ops.groupnorm_act(t.view(2, 3, 16), rand(16), rand(16), groups=4)
+    torch.cuda.synchronize()
+
+
+def test_recomputation_gives_the_same_gradients():
+    """Activation checkpointing runs the forward pass a second time from inside the backward pass: the masks are the
+    same ones, and so are the gradients, bit by bit."""
+    from torch.utils.checkpoint import checkpoint
+    x, w, b = rand(20, 64, grad=True), rand(64, 64, grad=True), rand(64, grad=True)
+
+    def block(t):
+        u = ops.groupnorm_act(t.view(4, 5, 64), torch.ones_like(b), b, groups=8, p=0.3, seed=9, offset=0)
+        u = ops.linear_act(u.reshape(20, 64), w, b, act="silu", p=0.3, seed=9, offset=1)
+        return ops.dropout(u, 0.3, 9, offset=2, resid=t)
+    want = torch.autograd.grad(block(x).square().sum(), (x, w, b))
+    for reentrant in (False, True):
+        got = torch.autograd.grad(checkpoint(block, x, use_reentrant=False).square().sum(), (x, w, b)) if not reentrant \
+            else None
+        if reentrant:
+            for t in (x, w, b):
+                t.grad = None
+            checkpoint(block, x, use_reentrant=True).square().sum().backward()
+            got = (x.grad, w.grad, b.grad)
+        for g, r in zip(got, want):
+            assert torch.equal(g, r)
