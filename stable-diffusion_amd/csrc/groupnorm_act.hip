@@ -7,11 +7,12 @@
 // A (sample, group) slice that fits LDS is one workgroup's work: read once, normalised from LDS, one launch (the
 // weight gradients of several samples take a second one).  Larger slices take two launches over strips of pixels:
 // the first leaves per-strip sums, the second folds them in double and finishes the strip.  Every sum is taken in a
-// fixed order.  Statistics are taken about a value of the group (its first one), so that a common offset does not
-// cancel in E[x^2] - E[x]^2.
+// fixed order.  Statistics are taken about a value of the group, so that a common offset does not cancel in
+// E[x^2] - E[x]^2: about the middle one of three far apart, because an outlier a (feature maps have them, in corners too)
+// would make the sums' rounding a^2 times that of a variance that may be a^2 / n.
 //
-// Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 12 us (HBM: 8), apply 23, gradient
-// sums 23, gradient apply 25 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
+// Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 11 us (HBM: 8), apply 23, gradient
+// sums 23, gradient apply 26 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
 // (480) and the SiLU (its exponential and reciprocal at a quarter of the rate) of 512 elements, 20 us in all, where HBM
 // would take 16, 16 and 24.  3x37x53x480 fp32: 7, 9, 9 and 9 us, launches and the fold of the strips.  One workgroup per
 // slice: 2x8x8x1280 fp16 forward 5.6 us, 16x16x16x1280 bf16 12 forward, 23 backward.
@@ -21,7 +22,7 @@
 
 namespace {
 
-constexpr int GNA_MAX_C = 8192;               // channel sums of a strip fit LDS
+constexpr int GNA_MAX_C = 8192;               // a thread per eight channels, and their sums fit LDS
 
 struct GnaParams {
   const void* x0; const void* x1; const void* dy;
@@ -120,9 +121,15 @@ __device__ __forceinline__ void load_params(const float* p, int c, int C, float 
     for (int e = 0; e < 8; ++e) v[e] = p[c + e < C ? c + e : C - 1];
   }
 }
-template <typename T> __device__ __forceinline__ float first_of(const GnaParams& p, int b, int c) {
-  const int64_t row = (int64_t)b * p.HW;
+template <typename T> __device__ __forceinline__ float element(const GnaParams& p, int64_t row, int c) {
   return c < p.c0 ? to_f32<T>(((const T*)p.x0)[row * p.c0 + c]) : to_f32<T>(((const T*)p.x1)[row * p.c1 + (c - p.c0)]);
+}
+// the value that the sums of sample b's group g are taken about
+template <typename T> __device__ __forceinline__ float shift_of(const GnaParams& p, int b, int g) {
+  const int64_t row = (int64_t)b * p.HW;
+  const int c = g * p.cpg;
+  return __builtin_amdgcn_fmed3f(element<T>(p, row, c), element<T>(p, row + p.HW / 2, c + p.cpg / 2),
+                                 element<T>(p, row + p.HW - 1, c + p.cpg - 1));
 }
 
 // W columns from c on, that do not leave their group of eight
@@ -297,20 +304,18 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
 }
 
 // ---- strips ------------------------------------------------------------------------------------------
-// A thread owns one group of eight columns and walks every lanes-th pixel of its strip; tensors of more than 2048
-// channels make a thread take several column groups, one after the other.
+// A thread owns one group of eight columns (a block has at least as many threads) and walks every lanes-th pixel of its
+// strip.
 // pixels a thread has in flight while it works on as many: 64 bytes (32 of each tensor backward), what the registers hold
 template <typename T> struct Depth { static constexpr int FWD = 16 / (int)sizeof(T) / 2, BWD = 1; };
-struct Walk { int ncg, lanes, pl, cg0, count; int64_t row0; };      // count pixels from row row0 on
+struct Walk { int ncg, lanes, pl, cg, count; int64_t row0; bool live; };      // count pixels from row row0 on
 __device__ __forceinline__ Walk walk_of(const GnaParams& p, int strip, int b) {
   Walk w;
   w.ncg = (p.C + 7) >> 3;
-  const int threads = (int)blockDim.x;
-  const bool fits = w.ncg <= threads;
-  w.lanes = fits ? threads / w.ncg : 1;
-  w.pl = fits ? (int)threadIdx.x / w.ncg : 0;
-  w.cg0 = fits ? (int)threadIdx.x - w.pl * w.ncg : (int)threadIdx.x;
-  if (w.pl >= w.lanes) w.cg0 = w.ncg;                    // threads left over
+  w.lanes = (int)blockDim.x / w.ncg;
+  w.pl = (int)threadIdx.x / w.ncg;
+  w.cg = (int)threadIdx.x - w.pl * w.ncg;
+  w.live = w.pl < w.lanes;                               // the others are left over
   const int64_t pb = (int64_t)strip * p.px_per_strip, left = p.HW - pb;
   w.count = (int)(left < p.px_per_strip ? left : p.px_per_strip);
   w.row0 = (int64_t)b * p.HW + pb;
@@ -353,25 +358,28 @@ __global__ __launch_bounds__(1024) void gna_stats_kernel(GnaParams p) {
   const int width = w.ncg * 8;
   float* s1 = reinterpret_cast<float*>(smem);
   float* s2 = s1 + w.lanes * width;
-  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
-    const int c = cg * 8;
-    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
-    float sh[8], s[8], q[8];
+  const int c = w.cg * 8;
+  const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
+  typename C::Raw r[WALK];                     // the first pixels come while the groups' shifts go round
+  if (w.live) fetch(x, w, w.pl, r);
+  for (int g = threadIdx.x; g < p.G; g += (int)blockDim.x) s1[g] = shift_of<T>(p, b, g);
+  __syncthreads();
+  float sh[8], s[8], q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int ce = c + e < p.C ? c + e : p.C - 1;
-      sh[e] = first_of<T>(p, b, (int)div_by((unsigned)ce, p.div_cpg) * p.cpg);
-      s[e] = 0.f; q[e] = 0.f;
-    }
+  for (int e = 0; e < 8; ++e) {
+    sh[e] = s1[div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg)];
+    s[e] = 0.f; q[e] = 0.f;
+  }
+  __syncthreads();
+  if (w.live) {
     for (int px = w.pl; px < w.count; px += WALK * w.lanes) {
-      typename C::Raw r[WALK];
-      fetch(x, w, px, r);
 #pragma unroll
       for (int u = 0; u < WALK; ++u) {
         if (px + u * w.lanes >= w.count) break;
 #pragma unroll
         for (int e = 0; e < 8; ++e) { const float t = to_f32<T>(r[u][e]) - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
       }
+      if (px + WALK * w.lanes < w.count) fetch(x, w, px + WALK * w.lanes, r);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
@@ -426,12 +434,14 @@ __global__ __launch_bounds__(1024) void gna_apply_kernel(GnaParams p) {
   const Walk w = walk_of(p, strip, b);
   typedef Cols<T, WHOLE> C;
   typename C::Raw r[WALK];                     // the first pixels come while the strips' sums are folded
-  if (w.cg0 < w.ncg) fetch(C(p.x0, p.x1, p.c0, p.c1, w.cg0 * 8, w.row0), w, w.pl, r);
+  const int c = w.cg * 8;
+  const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
+  if (w.live) fetch(x, w, w.pl, r);
   fold_strips(p, b, [&](int g, double a, double q) {
     const double n = (double)p.HW * (double)p.cpg, m = a / n;
     double var = q / n - m * m;
     if (var < 0.0) var = 0.0;
-    const float mean = (float)((double)first_of<T>(p, b, g * p.cpg) + m), rstd = (float)(1.0 / sqrt(var + (double)p.eps));
+    const float mean = (float)((double)shift_of<T>(p, b, g) + m), rstd = (float)(1.0 / sqrt(var + (double)p.eps));
     s_mean[g] = mean; s_rstd[g] = rstd;
     if (strip == 0) {
       p.stats[((size_t)b * p.G + g) * 2] = mean;
@@ -441,10 +451,8 @@ __global__ __launch_bounds__(1024) void gna_apply_kernel(GnaParams p) {
   __syncthreads();
   unsigned k0 = 0, k1 = 0;
   if (DROP) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
-    const int c = cg * 8;
-    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), y(p.out0, p.out0, p.C, 0, c, w.row0);
-    if (cg != w.cg0) fetch(x, w, w.pl, r);
+  if (w.live) {
+    const C y(p.out0, p.out0, p.C, 0, c, w.row0);
     float mn[8], sc[8], bt[8];
     load_params(p.gamma, c, p.C, sc);
     load_params(p.beta, c, p.C, bt);
@@ -465,7 +473,7 @@ __global__ __launch_bounds__(1024) void gna_apply_kernel(GnaParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(to_f32<T>(now[u][e]) - mn[e], sc[e], bt[e]);
         act_n<T>(v, act);
-        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)(w.row0 + px + u * w.lanes), p.drop.offset), p.drop.thr, p.drop.scale);
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)w.cg, (uint64_t)(w.row0 + px + u * w.lanes), p.drop.offset), p.drop.thr, p.drop.scale);
         y.store(px + u * w.lanes, v);
       }
     }
@@ -486,8 +494,8 @@ __global__ __launch_bounds__(1024) void gna_grad_sums_kernel(GnaParams p) {
   float* s2 = s1 + w.lanes * width;
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
-    const int c = cg * 8;
+  if (w.live) {
+    const int c = w.cg * 8;
     const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0);
     typename C::Raw rx[WALK_BWD], rd[WALK_BWD];
     fetch(x, w, w.pl, rx);
@@ -523,7 +531,7 @@ __global__ __launch_bounds__(1024) void gna_grad_sums_kernel(GnaParams p) {
           d[e] = to_f32<T>(nx[u][e]) - mn[e];
           z[e] = fmaf(d[e], sc[e], bt[e]);
         }
-        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, 1.f);
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)w.cg, (uint64_t)row, p.drop.offset), p.drop.thr, 1.f);
         act_grad_n<T>(z, v, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e) { s[e] += v[e]; q[e] = fmaf(v[e], d[e], q[e]); }
@@ -597,9 +605,11 @@ __global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
   const Walk w = walk_of(p, strip, b);
   typedef Cols<T, WHOLE> C;
   typename C::Raw rx[WALK_BWD], rd[WALK_BWD];
-  if (w.cg0 < w.ncg) {
-    fetch(C(p.x0, p.x1, p.c0, p.c1, w.cg0 * 8, w.row0), w, w.pl, rx);
-    fetch(C(p.dy, p.dy, p.C, 0, w.cg0 * 8, w.row0), w, w.pl, rd);
+  const int c = w.cg * 8;
+  const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0);
+  if (w.live) {
+    fetch(x, w, w.pl, rx);
+    fetch(dy, w, w.pl, rd);
   }
   fold_strips(p, b, [&](int g, double a, double q) {
     const double n = (double)p.HW * (double)p.cpg;
@@ -608,13 +618,8 @@ __global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
   __syncthreads();
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
-  for (int cg = w.cg0; cg < w.ncg; cg += (int)blockDim.x) {
-    const int c = cg * 8;
-    const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0), dy(p.dy, p.dy, p.C, 0, c, w.row0), dx(p.out0, p.out1, p.c0, p.c1, c, w.row0);
-    if (cg != w.cg0) {
-      fetch(x, w, w.pl, rx);
-      fetch(dy, w, w.pl, rd);
-    }
+  if (w.live) {
+    const C dx(p.out0, p.out1, p.c0, p.c1, c, w.row0);
     // dx = rstd (h - a - xh q) = sc du - (rstd a + (x - mean) rstd^2 q)
     float mn[8], sc[8], bt[8], ka[8], kq[8];
     load_params(p.gamma, c, p.C, sc);
@@ -647,7 +652,7 @@ __global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
           d[e] = to_f32<T>(nx[u][e]) - mn[e];
           z[e] = fmaf(d[e], sc[e], bt[e]);
         }
-        if (DROP) drop8(v, philox8(k0, k1, (unsigned)cg, (uint64_t)row, p.drop.offset), p.drop.thr, ds);
+        if (DROP) drop8(v, philox8(k0, k1, (unsigned)w.cg, (uint64_t)row, p.drop.offset), p.drop.thr, ds);
         act_grad_n<T>(z, v, act);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = fmaf(sc[e], v[e], -fmaf(d[e], kq[e], ka[e]));
@@ -694,7 +699,7 @@ GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backwa
   int lanes;
   int64_t strips;
   for (pl.threads = 512;; pl.threads = 1024) {
-    lanes = ncg <= pl.threads ? pl.threads / ncg : 1;
+    lanes = ncg <= pl.threads ? pl.threads / ncg : 1;      // (a block of 512 is given up below if that is too few)
     const int64_t by_work = (HW + 4 * lanes - 1) / (4 * lanes);
     strips = ((1 << 18) / pl.threads + B - 1) / B;
     if (strips > by_work) strips = by_work;

@@ -675,7 +675,10 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
         if (p.dz_lo) {
           float lo[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lo[e] = v[u][e] - to_f32<T>(from_f32<T>(v[u][e]));
+          for (int e = 0; e < 8; ++e) {
+            const float hi = to_f32<T>(from_f32<T>(v[u][e]));
+            lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? v[u][e] - hi : 0.f;      // infinities stay infinite
+          }
           store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
         }
 #pragma unroll

@@ -145,9 +145,15 @@ def groupnorm_ref(x, x1, gamma, beta, dy, eps, name, groups, p, seed, offset, dt
     t = v - mean
     var = (t * t).mean((1, 3), keepdim=True)
     rstd = 1 / torch.sqrt(var + eps)
-    spread = (v - v[:, :1, :, :1]).abs().amax((1, 3), keepdim=True)       # sums are taken about the first value
-    emean = S * spread + U * mean.abs()
-    ers = 0.5 * rstd ** 2 * (S * 2 * spread ** 2) + 4 * U                 # relative
+    hw = v.shape[1]                                                       # sums are taken about the middle of three values
+    if hw:
+        about = torch.stack([v[:, 0, :, 0], v[:, hw // 2, :, cpg // 2], v[:, -1, :, -1]]).median(0).values[:, None, :, None]
+        off = (v - about).abs()
+    else:
+        off = t.abs()
+    emean = S * off.mean((1, 3), keepdim=True) + U * mean.abs()
+    evar = S * ((off * off).mean((1, 3), keepdim=True) + 2 * (mean - about if hw else mean).abs() * off.mean((1, 3), keepdim=True))
+    ers = 0.5 * rstd ** 2 * evar * (1 + evar * rstd ** 2) + 4 * U         # relative
     xh = t * rstd
     exh = rstd * (emean + U * v.abs()) + xh.abs() * (ers + 3 * U)
     ga, be = gamma.reshape(groups, cpg), beta.reshape(groups, cpg)

@@ -213,6 +213,22 @@ def test_infinite_and_nan_inputs_stay_where_they_are():
             assert (y[3].cpu()[torch.isneginf(z)] == 0).all()
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_infinite_gradients_stay_infinite(act, dt):
+    """An infinite entry of dy (or one that is infinite once scaled to the type) makes its row of dx and its column of
+    dw infinite, as the formula has it, and nothing else."""
+    dt = DT[dt]
+    x, w = (1 + rand(5, 64).abs()).to(dt).requires_grad_(), (1 + rand(24, 64, seed=1).abs()).to(dt).requires_grad_()
+    dy = rand(5, 24, seed=2).abs().to(dt)
+    dy[3, 7] = float("inf")
+    b = torch.zeros(24, device="cuda", requires_grad=True)
+    dx, dw, db = torch.autograd.grad(ops.linear_act(x, w, b, act=act), (x, w, b), dy)
+    assert torch.isposinf(dx[3]).all() and torch.isfinite(dx[[0, 1, 2, 4]]).all()
+    assert torch.isposinf(dw[7]).all() and torch.isfinite(dw[:7]).all() and torch.isfinite(dw[8:]).all()
+    assert torch.isposinf(db[7]) and torch.isfinite(db).sum() == 23
+
+
 # ---- group norm -----------------------------------------------------------------------------------------------
 
 GROUPNORM = [  # batch, spatial, c0, c1, groups, act, p
@@ -281,6 +297,26 @@ def test_groupnorm_act_far_from_zero_partial_gradients_and_strides(hw, dt):
     y = ops.groupnorm_act(e, gamma, beta, groups=8)
     ge, gg, gb = torch.autograd.grad(y, [e, gamma, beta], torch.empty_like(y))
     assert ge.shape == e.shape and not gg.any() and not gb.any()
+
+
+@dtypes
+@pytest.mark.parametrize("hot", ["first", "middle", "last"])
+@pytest.mark.parametrize("b,hw,c,groups", [(2, (8, 8), 64, 8), (1, (200, 201), 64, 4), (2, (64, 65), 30, 3)])
+def test_groupnorm_act_with_an_outlier(b, hw, c, groups, hot, dt):
+    """One pixel is a few hundred spreads away in every channel: it makes up most of the variance, and the statistics
+    may not be its rounding, whichever pixel it is."""
+    dt = DT[dt]
+    n = hw[0] * hw[1]
+    x = rand(b, n, c)
+    x[:, {"first": 0, "middle": n // 2, "last": n - 1}[hot]] += 700.0
+    x = x.reshape(b, *hw, c).to(dt).requires_grad_()
+    gamma, beta = rand(c, seed=2).requires_grad_(), rand(c, seed=3, grad=True)
+    dy = rand(b, *hw, c, dtype=dt, seed=4)
+    ref = R.groupnorm_ref(x, None, gamma, beta, dy, 1e-5, "silu", groups, 0.0, 0, 0, dt)
+    y = ops.groupnorm_act(x, gamma, beta, 1e-5, groups=groups)
+    R.check("y", y, *ref["y"])
+    for name, g in zip(("dx", "dgamma", "dbeta"), torch.autograd.grad(y, [x, gamma, beta], dy)):
+        R.check(name, g, *ref[name])
 
 
 def test_groupnorm_act_equals_the_inference_kernel_where_both_apply():
