@@ -706,24 +706,27 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // them, each costing `step` per K-tile of 128 bytes and its stores (a CU's share of HBM, 20 KB a microsecond); a split
 // contraction stores fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.8
 // with a column operand, not for two: their addresses do not fit the registers beside 160 accumulators), 256x256 1.55
-// (1.72 with column operands), 128x128 0.55 with two on a CU (0.8 alone), 64x64 0.26 (0.35 alone).  What the choice is
+// (1.72 with column operands), 128x128 0.55 with two on a CU, 64x64 0.27 with four; a workgroup that has a CU for itself
+// waits for its loads: 0.8 to 1.1 and 0.42 to 0.59, rows before columns, and twice that where the sizes keep the operands
+// from LDS-DMA.  twice: the contraction is done a second time, with the low parts of Q.  What the choice is
 // worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
 // round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
-// 64x64, 11 at 128x128 in 4 splits.  fp32 runs at a sixteenth of the matrix rate: 128x128
-// 2.3, 64x64 0.56.
+// 64x64, 11 at 128x128 in 4 splits, and its dx with the low parts 9 in 4 splits, 16 in one.  fp32 runs at a sixteenth of
+// the matrix rate: 128x128 2.3, 64x64 0.65 (alone 0.72).
 struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; double us; };
-constexpr double SPLIT_US = 10.0;      // see bwd_layout
+constexpr double SPLIT_US = 14.0;      // see bwd_layout
 
 enum Form { FORWARD, GRAD_X, GRAD_W };
 // sizes that are no whole 16-byte chunks stay off the large tiles
-Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
+Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form, bool twice) {
   const bool forward = form == FORWARD;
   const int kt = 128 / esize;
   const int64_t nkt = (K + kt - 1) / kt;
-  const bool whole = esize == 2 && N % 8 == 0 && (form == GRAD_W ? M : K) % 8 == 0;
+  const bool vec = N % 8 == 0 && (form == GRAD_W ? M : K) * esize % 16 == 0, whole = vec && esize == 2;
   struct Opt { int bm, bn; double step, alone; };
-  const Opt opts[4] = {{64, 64, esize == 2 ? 0.26 : 0.56, esize == 2 ? 0.35 : 0.56},
-                       {128, 128, esize == 2 ? 0.55 : 2.3, esize == 2 ? 0.8 : 2.3},
+  const double alone64[2][3] = {{0.8, 1.1, 1.25}, {0.42, 0.52, 0.59}}, alone128[2][3] = {{1.9, 2.4, 3.0}, {0.8, 0.95, 1.1}};
+  const Opt opts[4] = {{64, 64, esize == 2 ? (vec ? 0.27 : 0.45) : 0.65, esize == 2 ? alone64[vec][form] : vec ? 0.72 : 1.3},
+                       {128, 128, esize == 2 ? (vec ? 0.55 : 1.1) : 2.3, esize == 2 ? alone128[vec][form] : vec ? 2.2 : 3.3},
                        {256, 256, forward ? 1.55 : 1.72, 0.0},
                        {256, 320, forward ? 1.85 : 2.8, 0.0}};
   Plan best = {};
@@ -738,7 +741,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form) {
       const int64_t per = nkt > 0 ? (nkt + s - 1) / s : 1, used = nkt > 0 ? (nkt + per - 1) / per : 1;
       const double load = (double)((tiles * used + 255) / 256);
       double us = load * t.step > t.alone ? load * t.step : t.alone;
-      us = us * per + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
+      us = us * (twice ? 2 * per : per) + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
       if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 6.0;
       if (us < best_us) {
         best_us = us;
@@ -798,7 +801,7 @@ template <typename T, bool QC, bool PC>
 int product(const void* q, const void* q2, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e, float* partial,
             const DbFold& fold, hipStream_t stream) {
   const int sz = (int)sizeof(T);
-  Plan pl = plan_product(e.M, e.N, K, sz, QC ? GRAD_W : PC ? GRAD_X : FORWARD);
+  Plan pl = plan_product(e.M, e.N, K, sz, QC ? GRAD_W : PC ? GRAD_X : FORWARD, q2 != nullptr);
   const bool vec = chunked(q, ldq, QC ? e.M : K, sz) && ((uintptr_t)q2 & 15) == 0 && chunked(p, ldp, PC ? e.N : K, sz) && e.N % 8 == 0;
   if (!vec && pl.bm == 256) {      // pointers or strides that the sizes do not tell; the splits (and the workspace) stay
     pl.bm = pl.bn = 128;
@@ -834,8 +837,9 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   // large as the rounding of their own (error against 64 bits 1.41 times that of an unrounded dz, more where a few
   // entries dominate).  Products whose time is mostly their launch's multiply what the rounding lost as well; the larger
   // ones would take twice as long (4096x1280x5120 bf16 by about 130 us) and live with it.
-  const Plan px = plan_product(M, K, N, esize, GRAD_X), pw = plan_product(N, K, M, esize, GRAD_W);
+  Plan px = plan_product(M, K, N, esize, GRAD_X, false), pw = plan_product(N, K, M, esize, GRAD_W, false);
   w.split = w.need_dz && act != ACT_NONE && esize == 2 && px.us <= SPLIT_US && pw.us <= SPLIT_US;
+  if (w.split) { px = plan_product(M, K, N, esize, GRAD_X, true); pw = plan_product(N, K, M, esize, GRAD_W, true); }
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
   w.dz_lo = o; o += w.split ? up256((size_t)M * N * esize) : 0;
   // column groups a block takes (all, or an even share), and strips of rows: about 1024 blocks, every row lane at
@@ -937,7 +941,7 @@ int check_common(const LinearActArgs& a, const char* who) {
 
 int64_t linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype) {
   if (rows <= 0 || k <= 0 || n <= 0 || few_rows(rows, k, (int)sdmi_dtype_size(dtype))) return 0;
-  return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype), FORWARD), rows, n);
+  return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype), FORWARD, false), rows, n);
 }
 int64_t linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype) {
   if (rows <= 0 || k <= 0 || n <= 0) return 0;
