@@ -593,3 +593,49 @@ def test_recomputation_gives_the_same_gradients():
             got = (x.grad, w.grad, b.grad)
         for g, r in zip(got, want):
             assert torch.equal(g, r)
+
+
+def test_tensors_of_more_than_2_to_the_31_elements():
+    """Offsets beyond 32 bits: the last rows of a large call against the formula, and a batch's last image against a
+    call of its own."""
+    dt, m, k, n = torch.bfloat16, (1 << 21) + 4099, 64, 1032
+    x, w = torch.zeros(m, k, dtype=dt, device="cuda"), rand(n, k, dtype=dt)
+    x[-5:] = rand(5, k, seed=1).to(dt)
+    dy = torch.zeros(m, n, dtype=dt, device="cuda")
+    dy[-5:] = rand(5, n, seed=2).to(dt)
+    x.requires_grad_(), w.requires_grad_()
+    b = rand(n, seed=3, grad=True)
+    y = ops.linear_act(x, w, b, act="silu", p=0.3, seed=4, offset=1)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    s = R.keep_scale((5, n), 0.3, 4, 1, row0=m - 5)
+    xd, wd = R.d(x[-5:]), R.d(w)
+    z = xd @ wd.t() + R.d(b)
+    za = xd.abs() @ wd.abs().t() + R.d(b).abs()
+    ez = (k + 2) * R.U * za
+    ref = s * R.act(z, "silu")
+    R.check("y", y[-5:], ref, R.rounded(ref, s * (1.13 * ez + R.ACT_ERR * z.abs().clamp(min=1)) + 4 * R.U * ref.abs(), dt))
+    g = R.d(dy[-5:]) * s
+    dz = g * R.act_grad(z, "silu")
+    edz = R.rounded(dz, 4 * R.U * dz.abs() + g.abs() * (0.86 * ez + R.ACT_ERR * z.abs().clamp(min=1)), dt)
+    for name, got, want, e, rows in (("dx", dx[-5:], dz @ wd, edz @ wd.abs(), n), ("dw", dw, dz.t() @ xd, edz.t() @ xd.abs(), 5)):
+        R.check(name, got, want, R.rounded(want, e + (rows + 2) * R.U * (e + want.abs() + dz.abs().sum()), dt))
+    R.check("db", db, dz.sum(0), edz.sum(0) + 8 * R.U * dz.abs().sum(0))
+    assert not dx[:-5].any()
+    del x, w, dy, y, dx, dw
+
+    hw, c = (1 << 21) + 77, 640
+    x = torch.empty(2, hw, c, dtype=dt, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    gamma, beta = rand(c, seed=2), rand(c, seed=3)
+    x.requires_grad_()
+    y = ops.groupnorm_act(x, gamma, beta, groups=32)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    one = x.detach()[1:].clone().requires_grad_()
+    y1 = ops.groupnorm_act(one, gamma, beta, groups=32)
+    dx1, = torch.autograd.grad(y1, one, y.detach()[1:])
+    # the strips differ, so the statistics may differ by a few 2^-24 of their size, and a value by one step of bf16
+    for a, r in ((y[1:], y1), (dx[1:], dx1)):
+        for lo in range(0, hw, 1 << 18):
+            p, q = a[:, lo:lo + (1 << 18)].detach().float(), r[:, lo:lo + (1 << 18)].detach().float()
+            assert bool(((p - q).abs() <= 2.0 ** -7 * q.abs() + 1e-5).all())
+    del x, y, dx, one, y1, dx1
+    torch.cuda.empty_cache()
