@@ -22,6 +22,7 @@
 
 namespace {
 
+constexpr unsigned SLICES_X = 1u << 20;      // slices of a row of the grid: a launch has less than 2^32 threads that way
 constexpr int GNA_MAX_C = 8192;               // a thread per eight channels, and their sums fit LDS
 
 struct GnaParams {
@@ -155,11 +156,13 @@ __device__ __forceinline__ float block_sum(float v, float* red) {       // red: 
   for (unsigned w = 0; w < blockDim.x >> 6; ++w) t += red[w];
   return t;
 }
-__device__ __forceinline__ void slice_of_block(const GnaParams& p, int& b, int& g) {
+__device__ __forceinline__ bool slice_of_block(const GnaParams& p, int& b, int& g) {
   // neighbouring groups of a sample share 128-byte lines: a contiguous run of slices per XCD
-  const unsigned total = (unsigned)p.B * (unsigned)p.G, xcd = blockIdx.x & 7, q8 = total >> 3, r8 = total & 7;
-  const unsigned id = xcd * q8 + (xcd < r8 ? xcd : r8) + (blockIdx.x >> 3);
+  const unsigned block = blockIdx.y * SLICES_X + blockIdx.x;
+  const unsigned total = (unsigned)p.B * (unsigned)p.G, xcd = block & 7, q8 = total >> 3, r8 = total & 7;
+  const unsigned id = xcd * q8 + (xcd < r8 ? xcd : r8) + (block >> 3);
   b = (int)(id / (unsigned)p.G); g = (int)(id - (unsigned)b * (unsigned)p.G);
+  return block < total;
 }
 
 template <typename T, int W>
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(1024) void gna_slice_fwd_kernel(GnaParams p) {
   __shared__ float red[16];
   T* xs = reinterpret_cast<T*>(smem);
   int b, g;
-  slice_of_block(p, b, g);
+  if (!slice_of_block(p, b, g)) return;
   const int cbase = g * p.cpg, vpp = p.cpg / W, nv = (int)p.HW * vpp;
   float s = 0.f;
   for (int i = threadIdx.x; i < nv; i += blockDim.x) {
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
   extern __shared__ __align__(16) char smem[];
   __shared__ float red[16];
   int b, g;
-  slice_of_block(p, b, g);
+  if (!slice_of_block(p, b, g)) return;
   const int cbase = g * p.cpg, vpp = p.cpg / W, nv = (int)p.HW * vpp;
   float* dus = reinterpret_cast<float*>(smem);                     // [HW][cpg] fp32
   T* xs = reinterpret_cast<T*>(smem + (size_t)p.HW * p.cpg * 4);   // [HW][cpg]
@@ -750,6 +753,11 @@ int slice_threads(const GnaPlan& pl, const GnaParams& p) {
   return t;
 }
 
+dim3 slice_grid(const GnaParams& p) {
+  const unsigned total = (unsigned)p.B * (unsigned)p.G;
+  return total <= SLICES_X ? dim3(total) : dim3(SLICES_X, (total + SLICES_X - 1) / SLICES_X);
+}
+
 // the kernels over strips with SiLU (others by a branch), dropout and whole column groups compiled in
 #define GNA_LAUNCH(K, A, D, W, GRID, LDS) hipLaunchKernelGGL((K<T, A, D, W>), GRID, dim3(pl.threads), LDS, s, p)
 #define GNA_VARIANTS_W(K, W, GRID, LDS)                                   \
@@ -780,7 +788,7 @@ int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
   snprintf(label, sizeof(label), "gn_act B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
   ProfScope prof(PROF_GROUPNORM, s, 0.0, 2.0 * p.B * (double)p.HW * p.C * sizeof(T), label);
   if (pl.slice) {
-    const dim3 grid((unsigned)p.B * (unsigned)p.G), block(slice_threads(pl, p));
+    const dim3 grid = slice_grid(p), block(slice_threads(pl, p));
     if (pl.w == 8) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 8>), grid, block, pl.lds, s, p);
     else if (pl.w == 4) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 4>), grid, block, pl.lds, s, p);
     else if (pl.w == 2) hipLaunchKernelGGL((gna_slice_fwd_kernel<T, 2>), grid, block, pl.lds, s, p);
@@ -806,7 +814,7 @@ int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
   const bool weights = p.dgamma || p.dbeta;
   const unsigned fold_blocks = weights ? (unsigned)(p.C + 15) / 16 : 0;
   if (pl.slice) {
-    const dim3 grid((unsigned)p.B * (unsigned)p.G), block(slice_threads(pl, p));
+    const dim3 grid = slice_grid(p), block(slice_threads(pl, p));
     if (pl.w == 8) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 8>), grid, block, pl.lds, s, p);
     else if (pl.w == 4) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 4>), grid, block, pl.lds, s, p);
     else if (pl.w == 2) hipLaunchKernelGGL((gna_slice_bwd_kernel<T, 2>), grid, block, pl.lds, s, p);

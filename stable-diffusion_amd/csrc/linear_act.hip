@@ -573,7 +573,9 @@ __global__ __launch_bounds__(512) void linear_few_kernel(GemmParams p) {
 }
 // where it beats the tiles (us, replayed, few / tiles): fp16 32x1280x1280 5.8 / 9.0, 16x2560x640 6.8 / 6.8,
 // 8x5120x1280 9.6 / 8.0; fp32 2x1280x1280 5.8 / 8.6, 16x2560x640 11.3 / 9.3
-bool few_rows(int64_t rows, int64_t k, int esize) { return rows <= 32 && k * esize * (8 + rows) <= (128 << 10); }
+bool few_rows(int64_t rows, int64_t k, int n, int esize) {
+  return rows <= 32 && k * esize * (8 + rows) <= (128 << 10) && n <= (1 << 26);      // (a launch has less than 2^32 threads)
+}
 
 // ---- joins -----------------------------------------------------------------------------------------
 // Sum of the splits in a fixed order, then the epilogue.  A group of eight columns is summed by LANES threads, each over
@@ -812,6 +814,7 @@ int launch_join(const float* partial, unsigned splits, const Epilogue& e, hipStr
 }
 
 // out[m][n] = epilogue(sum_k (Q + Q2)(m, k) P(n, k)); Q2 may be null
+constexpr uint64_t MAX_BLOCKS = (1ull << 32) / 512;      // a launch has less than 2^32 threads: 512 a block, or 256 for two products
 struct Product { GemmParams g; Plan pl; bool vec; };
 template <typename T, bool QC, bool PC>
 int plan_launch(Product* pr, const void* q, const void* q2, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e,
@@ -827,7 +830,8 @@ int plan_launch(Product* pr, const void* q, const void* q2, int64_t ldq, const v
   g.q = (const char*)q; g.q2 = (const char*)q2; g.p = (const char*)p; g.fold = fold; g.ldq = ldq; g.ldp = ldp; g.K = K;
   g.k_per_split = pl.k_per_split; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.e = e;
   const uint64_t total = (uint64_t)pl.tiles_m * pl.tiles_n * pl.splits;
-  SDMI_REQUIRE(pl.bm && total < (1ull << 30), "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
+  const uint64_t folds = fold.db ? (uint64_t)(fold.n + DB_COLS - 1) / DB_COLS : 0;
+  SDMI_REQUIRE(pl.bm && total + folds < MAX_BLOCKS, "linear_act: %lld x %d outputs are too many", (long long)e.M, e.N);
   g.tiles = pl.tiles_m * pl.tiles_n;
   g.partial = pl.splits > 1 ? partial : nullptr;
   pr->pl = pl;
@@ -990,7 +994,7 @@ int check_common(const LinearActArgs& a, const char* who) {
 }  // namespace
 
 int64_t linear_act_workspace_bytes(int64_t rows, int k, int n, int dtype) {
-  if (rows <= 0 || k <= 0 || n <= 0 || few_rows(rows, k, (int)sdmi_dtype_size(dtype))) return 0;
+  if (rows <= 0 || k <= 0 || n <= 0 || few_rows(rows, k, n, (int)sdmi_dtype_size(dtype))) return 0;
   return (int64_t)partial_bytes(plan_product(rows, n, k, (int)sdmi_dtype_size(dtype), FORWARD, false), rows, n);
 }
 int64_t linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype) {
@@ -1008,7 +1012,7 @@ int linear_act(const LinearActArgs& a, hipStream_t stream) {
   SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %lld bytes", (long long)need);
   e.bias = a.bias; e.resid = a.resid; e.ldr = a.ldr; e.out = a.out; e.ldo = a.n;
   e.alpha = 1.f; e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
-  if (few_rows(a.rows, a.k, (int)sdmi_dtype_size(a.dtype))) { SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_few<T>(a, e, stream)); }
+  if (few_rows(a.rows, a.k, a.n, (int)sdmi_dtype_size(a.dtype))) { SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_few<T>(a, e, stream)); }
   Product pr;
   SDMI_DISPATCH_DTYPE(a.dtype, T, {
     SDMI_TRY((plan_launch<T, false, false>(&pr, a.x, nullptr, a.ldx, a.w, a.ldw, a.k, e, (float*)a.workspace, DbFold())));

@@ -63,6 +63,7 @@ def test_library_refuses_bad_calls():
     assert "size" in _refused("sdmi_linear_act", *lin(rows=-1))
     assert "too many" in _refused("sdmi_linear_act", *lin(n=(1 << 30) + 1))
     assert "too many" in _refused("sdmi_linear_act", *lin(rows=1 << 50))
+    assert "too many" in _refused("sdmi_linear_act", *lin(rows=1 << 31))              # more threads than a launch has
     assert "activation" in _refused("sdmi_linear_act", *lin(act=4))
     assert "dtype" in _refused("sdmi_linear_act", *lin(dt=-1))
     assert "null" in _refused("sdmi_linear_act", *lin(w=None))

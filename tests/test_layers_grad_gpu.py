@@ -639,3 +639,20 @@ def test_tensors_of_more_than_2_to_the_31_elements():
             assert bool(((p - q).abs() <= 2.0 ** -7 * q.abs() + 1e-5).all())
     del x, y, dx, one, y1, dx1
     torch.cuda.empty_cache()
+
+
+def test_groupnorm_act_of_more_slices_than_a_launch_has_blocks_in_a_row():
+    """A group per channel and many samples: 2^27 slices, whose threads are more than 2^32."""
+    b, c = 65535, 2048
+    x = torch.empty(b, 2, c, dtype=torch.float16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    gamma, beta = rand(c, seed=2).requires_grad_(), rand(c, seed=3, grad=True)
+    x.requires_grad_()
+    y = ops.groupnorm_act(x, gamma, beta, groups=c)
+    dx, dg, db = torch.autograd.grad(y, (x, gamma, beta), torch.ones_like(y))
+    for i in (0, 1023, 30000, b - 1):
+        ref = R.groupnorm_ref(x[i:i + 1], None, gamma, beta, torch.ones(1, 2, c), 1e-5, "silu", c, 0.0, 0, 0, torch.float16)
+        R.check("y", y[i:i + 1], *ref["y"])
+        R.check("dx", dx[i:i + 1], *ref["dx"])
+    assert torch.isfinite(dg).all() and torch.isfinite(db).all()
+    del x, y, dx
+    torch.cuda.empty_cache()
