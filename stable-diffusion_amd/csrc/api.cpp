@@ -41,6 +41,7 @@ void prof_begin(int cls, hipStream_t stream, double flops, double bytes, const c
   g_prof_entries.push_back(e);
   g_prof_flops[cls] += flops; g_prof_bytes[cls] += bytes; g_prof_launches[cls] += 1;
 }
+bool prof_on() { return g_prof_on; }
 void prof_end(int cls, hipStream_t stream) {
   if (!g_prof_on) return;
   for (size_t i = g_prof_entries.size(); i-- > 0;)

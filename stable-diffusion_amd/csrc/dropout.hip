@@ -56,8 +56,8 @@ int launch_dropout(const DropoutArgs& a, const DropArgs& drop, hipStream_t strea
   const int64_t ny = (a.rows + p.rows_per_y - 1) / p.rows_per_y;
   SDMI_REQUIRE(ny <= 65535, "dropout: %lld rows of %d columns are too many", (long long)a.rows, a.cols);
   const unsigned blocks = (unsigned)(((uint64_t)p.rows_per_y * groups + 255) / 256);
-  char label[64];
-  snprintf(label, sizeof(label), "dropout %lldx%d", (long long)a.rows, a.cols);
+  char label[64] = "";
+  if (prof_on()) snprintf(label, sizeof(label), "dropout %lldx%d", (long long)a.rows, a.cols);
   ProfScope prof(PROF_OTHER, stream, 0.0, (a.resid ? 3.0 : 2.0) * a.rows * (double)a.cols * sizeof(T), label);
   const dim3 grid(blocks, (unsigned)ny);
   if (a.resid) hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(256), 0, stream, p);

@@ -784,8 +784,8 @@ template <typename T>
 int gna_fwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
   GnaParams p = gna_params(a, pl, drop);
   p.out0 = a.out;
-  char label[64];
-  snprintf(label, sizeof(label), "gn_act B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
+  char label[64] = "";
+  if (prof_on()) snprintf(label, sizeof(label), "gn_act B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
   ProfScope prof(PROF_GROUPNORM, s, 0.0, 2.0 * p.B * (double)p.HW * p.C * sizeof(T), label);
   if (pl.slice) {
     const dim3 grid = slice_grid(p), block(slice_threads(pl, p));
@@ -808,8 +808,8 @@ template <typename T>
 int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, hipStream_t s) {
   GnaParams p = gna_params(a, pl, drop);
   p.out0 = a.dx0; p.out1 = a.dx1;
-  char label[64];
-  snprintf(label, sizeof(label), "gn_act bwd B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
+  char label[64] = "";
+  if (prof_on()) snprintf(label, sizeof(label), "gn_act bwd B%d HW%lld C%d", p.B, (long long)p.HW, p.C);
   ProfScope prof(PROF_GROUPNORM, s, 0.0, 3.0 * p.B * (double)p.HW * p.C * sizeof(T), label);
   const bool weights = p.dgamma || p.dbeta;
   const unsigned fold_blocks = weights ? (unsigned)(p.C + 15) / 16 : 0;

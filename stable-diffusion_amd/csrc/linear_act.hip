@@ -817,10 +817,9 @@ int launch_join(const float* partial, unsigned splits, const Epilogue& e, hipStr
 constexpr uint64_t MAX_BLOCKS = (1ull << 32) / 512;      // a launch has less than 2^32 threads: 512 a block, or 256 for two products
 struct Product { GemmParams g; Plan pl; bool vec; };
 template <typename T, bool QC, bool PC>
-int plan_launch(Product* pr, const void* q, const void* q2, int64_t ldq, const void* p, int64_t ldp, int64_t K, const Epilogue& e,
-                float* partial, const DbFold& fold) {
+int plan_launch(Product* pr, Plan pl, const void* q, const void* q2, int64_t ldq, const void* p, int64_t ldp, int64_t K,
+                const Epilogue& e, float* partial, const DbFold& fold) {
   const int sz = (int)sizeof(T);
-  Plan pl = plan_product(e.M, e.N, K, sz, QC ? GRAD_W : PC ? GRAD_X : FORWARD, q2 != nullptr);
   pr->vec = chunked(q, ldq, QC ? e.M : K, sz) && ((uintptr_t)q2 & 15) == 0 && chunked(p, ldp, PC ? e.N : K, sz) && e.N % 8 == 0;
   if (!pr->vec && pl.bm == 256) {  // pointers or strides that the sizes do not tell; the splits (and the workspace) stay
     pl.bm = pl.bn = 128;
@@ -842,10 +841,10 @@ template <typename T> int join_splits(const Product& pr, hipStream_t stream) {
   return SDMI_OK;
 }
 void product_label(char (&label)[96], const GemmParams& g) {
-  snprintf(label, sizeof(label), "linear M%lld N%d K%lld", (long long)g.e.M, g.e.N, (long long)g.K);
+  if (prof_on()) snprintf(label, sizeof(label), "linear M%lld N%d K%lld", (long long)g.e.M, g.e.N, (long long)g.K);
 }
 template <typename T, bool QC, bool PC> int run_product(const Product& pr, hipStream_t stream) {
-  char label[96];
+  char label[96] = "";
   product_label(label, pr.g);
   {
     ProfScope prof(PROF_OTHER, stream, 2.0 * pr.g.e.M * (double)pr.g.e.N * pr.g.K, 0.0, label);
@@ -865,7 +864,7 @@ template <typename T, bool VEC> void launch_grads(const Product& w, const Produc
   else hipLaunchKernelGGL((linear_grads_kernel<T, 2, 2, VEC>), grid, dim3(256), 0, stream, w.g, x.g);
 }
 template <typename T> int run_grads(const Product& w, const Product& x, hipStream_t stream) {
-  char label[96];
+  char label[96] = "";
   product_label(label, w.g);
   {
     ProfScope prof(PROF_OTHER, stream, 4.0 * w.g.e.M * (double)w.g.e.N * w.g.K, 0.0, label);
@@ -877,7 +876,7 @@ template <typename T> int run_grads(const Product& w, const Product& x, hipStrea
   return join_splits<T>(x, stream);
 }
 
-struct BwdLayout { size_t dz, dz_lo, dbp, px, pw, total; int strips, col_blocks, groups; int64_t rows_per_strip; bool need_dz, split; };
+struct BwdLayout { Plan plan_x, plan_w; size_t dz, dz_lo, dbp, px, pw, total; int strips, col_blocks, groups; int64_t rows_per_strip; bool need_dz, split; };
 BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int esize) {
   BwdLayout w;
   size_t o = 0;
@@ -886,7 +885,9 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   // large as the rounding of their own (error against 64 bits 1.41 times that of an unrounded dz, more where a few
   // entries dominate).  Products whose time is mostly their launch's multiply what the rounding lost as well; the larger
   // ones would take twice as long (4096x1280x5120 bf16 by about 130 us) and live with it.
-  Plan px = plan_product(M, K, N, esize, GRAD_X, false), pw = plan_product(N, K, M, esize, GRAD_W, false);
+  Plan &px = w.plan_x, &pw = w.plan_w;
+  px = plan_product(M, K, N, esize, GRAD_X, false);
+  pw = plan_product(N, K, M, esize, GRAD_W, false);
   w.split = w.need_dz && act != ACT_NONE && esize == 2 && px.us <= SPLIT_US && pw.us <= SPLIT_US;
   if (w.split) { px = plan_product(M, K, N, esize, GRAD_X, true); pw = plan_product(N, K, M, esize, GRAD_W, true); }
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
@@ -918,9 +919,7 @@ Epilogue plain_out(void* out, int64_t M, int N, float alpha) {
 }
 
 template <typename T>
-int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
-  const int want = (a.dx ? 1 : 0) | (a.dw ? 2 : 0) | (a.db ? 4 : 0);
-  const BwdLayout w = bwd_layout(a.rows, a.k, a.n, a.act, drop.thr != 0, want, (int)sizeof(T));
+int linear_bwd(const LinearActArgs& a, const BwdLayout& w, const DropArgs& drop, hipStream_t s) {
   char* ws = (char*)a.workspace;
   const void* dz = a.dy;
   int64_t lddz = a.lddy;
@@ -936,8 +935,8 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
     d.M = a.rows; d.rows_per_strip = w.rows_per_strip; d.N = a.n; d.act = a.act; d.drop = drop; d.groups = w.groups;
     if (a.act == ACT_NONE) d.drop.scale = 1.f;
     d.db_scale = alpha;
-    char label[64];
-    snprintf(label, sizeof(label), "linear dz %lldx%d", (long long)a.rows, a.n);
+    char label[64] = "";
+    if (prof_on()) snprintf(label, sizeof(label), "linear dz %lldx%d", (long long)a.rows, a.n);
     ProfScope prof(PROF_OTHER, s, 0.0, 2.0 * a.rows * (double)a.n * sizeof(T), label);
     hipLaunchKernelGGL(linear_dz_kernel<T>, dim3(w.col_blocks, w.strips), dim3(256), 0, s, d);
     SDMI_CHECK_HIP(hipGetLastError());
@@ -948,10 +947,10 @@ int linear_bwd(const LinearActArgs& a, const DropArgs& drop, hipStream_t s) {
   const bool want_x = a.dx && a.rows > 0;
   Product w_, x_;
   if (a.dw)
-    SDMI_TRY((plan_launch<T, true, true>(&w_, dz, dz_lo, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha),
+    SDMI_TRY((plan_launch<T, true, true>(&w_, w.plan_w, dz, dz_lo, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha),
                                          (float*)(ws + w.pw), want_x ? DbFold() : fold)));
   if (want_x)
-    SDMI_TRY((plan_launch<T, false, true>(&x_, dz, dz_lo, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha),
+    SDMI_TRY((plan_launch<T, false, true>(&x_, w.plan_x, dz, dz_lo, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha),
                                           (float*)(ws + w.px), fold)));
   if (a.dw && want_x && grads_together(w_, x_)) {
     SDMI_TRY(run_grads<T>(w_, x_, s));
@@ -971,8 +970,8 @@ template <typename T>
 int linear_few(const LinearActArgs& a, const Epilogue& e, hipStream_t s) {
   GemmParams g = {};
   g.q = (const char*)a.x; g.p = (const char*)a.w; g.ldq = a.ldx; g.ldp = a.ldw; g.K = a.k; g.e = e;
-  char label[96];
-  snprintf(label, sizeof(label), "linear M%lld N%d K%d", (long long)a.rows, a.n, a.k);
+  char label[96] = "";
+  if (prof_on()) snprintf(label, sizeof(label), "linear M%lld N%d K%d", (long long)a.rows, a.n, a.k);
   ProfScope prof(PROF_OTHER, s, 2.0 * a.rows * (double)a.n * a.k, (double)a.n * a.k * sizeof(T), label);
   const dim3 grid((unsigned)(a.n + 15) / 16);
   if (a.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, dim3(512), 0, s, g);
@@ -1008,14 +1007,16 @@ int linear_act(const LinearActArgs& a, hipStream_t stream) {
   SDMI_TRY(drop_args(&e.drop, a.p, a.seed, a.seed_dev, a.offset, "linear_act"));
   if (a.rows == 0) return SDMI_OK;
   SDMI_REQUIRE(a.x && a.w && a.out, "linear_act: null pointer");
-  const int64_t need = linear_act_workspace_bytes(a.rows, a.k, a.n, a.dtype);
-  SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %lld bytes", (long long)need);
+  const int esize = (int)sdmi_dtype_size(a.dtype);
   e.bias = a.bias; e.resid = a.resid; e.ldr = a.ldr; e.out = a.out; e.ldo = a.n;
   e.alpha = 1.f; e.preact = a.act != ACT_NONE ? a.preact : nullptr; e.act = a.act; e.M = a.rows; e.N = a.n;
-  if (few_rows(a.rows, a.k, a.n, (int)sdmi_dtype_size(a.dtype))) { SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_few<T>(a, e, stream)); }
+  if (few_rows(a.rows, a.k, a.n, esize)) { SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_few<T>(a, e, stream)); }
+  const Plan pl = plan_product(a.rows, a.n, a.k, esize, FORWARD, false);
+  const size_t need = partial_bytes(pl, a.rows, a.n);
+  SDMI_REQUIRE(need == 0 || a.workspace, "linear_act: this size needs a workspace of %zu bytes", need);
   Product pr;
   SDMI_DISPATCH_DTYPE(a.dtype, T, {
-    SDMI_TRY((plan_launch<T, false, false>(&pr, a.x, nullptr, a.ldx, a.w, a.ldw, a.k, e, (float*)a.workspace, DbFold())));
+    SDMI_TRY((plan_launch<T, false, false>(&pr, pl, a.x, nullptr, a.ldx, a.w, a.ldw, a.k, e, (float*)a.workspace, DbFold())));
     return run_product<T, false, false>(pr, stream);
   });
   return SDMI_OK;
@@ -1030,9 +1031,10 @@ int linear_act_backward(const LinearActArgs& a, hipStream_t stream) {
   if (a.rows > 0) {
     SDMI_REQUIRE(a.dy && (a.x || !a.dw) && (a.w || !a.dx), "linear_act_backward: null pointer");
     SDMI_REQUIRE(a.preact || a.act == ACT_NONE, "linear_act_backward: the activation's gradient needs preact");
-    const int64_t need = linear_act_backward_workspace_bytes(a.rows, a.k, a.n, a.act, a.p, want, a.dtype);
-    SDMI_REQUIRE(need == 0 || a.workspace, "linear_act_backward: this size needs a workspace of %lld bytes", (long long)need);
   }
-  SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_bwd<T>(a, drop, stream));
+  const BwdLayout w = bwd_layout(a.rows, a.k, a.n, a.act, drop.thr != 0, want, (int)sdmi_dtype_size(a.dtype));
+  SDMI_REQUIRE(a.rows == 0 || w.total == 0 || a.workspace, "linear_act_backward: this size needs a workspace of %zu bytes",
+               w.total);
+  SDMI_DISPATCH_DTYPE(a.dtype, T, return linear_bwd<T>(a, w, drop, stream));
   return SDMI_OK;
 }

@@ -7,6 +7,7 @@
 enum { PROF_CONV_GEMM = 0, PROF_ATTENTION = 1, PROF_GROUPNORM = 2, PROF_LAYERNORM = 3, PROF_OTHER = 4, PROF_NCLS = 5 };
 void prof_begin(int cls, hipStream_t stream, double flops, double bytes, const char* label = nullptr);
 void prof_end(int cls, hipStream_t stream);
+bool prof_on();                   // whether labels are read at all
 struct ProfScope {
   int cls; hipStream_t s;
   ProfScope(int c, hipStream_t st, double flops, double bytes, const char* label = nullptr) : cls(c), s(st) {

@@ -656,3 +656,34 @@ def test_groupnorm_act_of_more_slices_than_a_launch_has_blocks_in_a_row():
     assert torch.isfinite(dg).all() and torch.isfinite(db).all()
     del x, y, dx
     torch.cuda.empty_cache()
+
+
+def test_two_threads_at_once():
+    """Two threads with a stream each, forward and backward, give what they give one after the other."""
+    import threading
+
+    def work(i):
+        x, w, b = rand(300 + i, 256, seed=i, grad=True), rand(384, 256, seed=i, grad=True), rand(384, seed=i, grad=True)
+        g, h = rand(384, seed=i + 5).requires_grad_(), rand(384, seed=i + 6, grad=True)
+        u = ops.linear_act(x, w, b, act="gelu", p=0.2, seed=i, offset=0)
+        u = ops.groupnorm_act(u.view(1, -1, 384), g, h, groups=12, p=0.2, seed=i, offset=1)
+        u = ops.dropout(u, 0.2, i, offset=2)
+        return [u] + list(torch.autograd.grad(u.square().sum(), (x, w, b, g, h)))
+    want = [[t.detach().cpu() for t in work(i)] for i in range(2)]
+    wrong = []
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = [t.detach().cpu() for t in work(i)]
+                    if not all(torch.equal(a, r) for a, r in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as e:                      # noqa: BLE001  (a thread's failure must reach the test)
+            wrong.append(repr(e))
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
