@@ -720,18 +720,19 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 
 // ---- host ------------------------------------------------------------------------------------------
 // Tile and split of a product: the least of an estimate in microseconds.  A CU works through ceil(workgroups / 256) of
-// them, each costing `step` per K-tile of 128 bytes and its stores (a CU's share of HBM, 20 KB a microsecond); a split
-// contraction stores fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.8
+// them, `together` at a time and then the rest, each costing `step` per K-tile of 128 bytes (`alone`, if it is the only
+// one, and in between for a few) and its stores (a CU's share of HBM, 20 KB a microsecond); a split contraction stores
+// fp32 and pays a join.  Steps measured on MI355X in fp16 with long contractions: 256x320 1.85 (2.8
 // with a column operand, not for two: their addresses do not fit the registers beside 160 accumulators), 256x256 1.55
 // (1.72 with column operands), 128x128 0.55 with two on a CU, 64x64 0.27 with four; a workgroup that has a CU for itself
-// waits for its loads: 0.8 to 1.1 and 0.42 to 0.59, rows before columns, and twice that where the sizes keep the operands
+// waits for its loads: 0.8 to 1.1 and 0.45 to 0.62, rows before columns, and twice that where the sizes keep the operands
 // from LDS-DMA.  twice: the contraction is done a second time, with the low parts of Q.  What the choice is
 // worth (us): 8192x4096x4096 217 at 256x256, 284 at 128x128, 546 at 64x64; 4096x5120x1280 54 at 256x320 (256 tiles, one
 // round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
 // 64x64, 11 at 128x128 in 4 splits, and its dx with the low parts 9 in 4 splits, 16 in one.  fp32 runs at a sixteenth of
 // the matrix rate: 128x128 2.3, 64x64 0.65 (alone 0.72).
 struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; double us; };
-constexpr double SPLIT_US = 14.0;      // see bwd_layout
+constexpr double SPLIT_US = 15.0;      // see bwd_layout
 
 enum Form { FORWARD, GRAD_X, GRAD_W };
 // sizes that are no whole 16-byte chunks stay off the large tiles
@@ -740,12 +741,13 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form, bool twice)
   const int kt = 128 / esize;
   const int64_t nkt = (K + kt - 1) / kt;
   const bool vec = N % 8 == 0 && (form == GRAD_W ? M : K) * esize % 16 == 0, whole = vec && esize == 2;
-  struct Opt { int bm, bn; double step, alone; };
-  const double alone64[2][3] = {{0.8, 1.1, 1.25}, {0.42, 0.52, 0.59}}, alone128[2][3] = {{1.9, 2.4, 3.0}, {0.8, 0.95, 1.1}};
-  const Opt opts[4] = {{64, 64, esize == 2 ? (vec ? 0.27 : 0.45) : 0.65, esize == 2 ? alone64[vec][form] : vec ? 0.72 : 1.3},
-                       {128, 128, esize == 2 ? (vec ? 0.55 : 1.1) : 2.3, esize == 2 ? alone128[vec][form] : vec ? 2.2 : 3.3},
-                       {256, 256, forward ? 1.55 : 1.72, 0.0},
-                       {256, 320, forward ? 1.85 : 2.8, 0.0}};
+  struct Opt { int bm, bn, together; double step, alone; };      // workgroups a CU takes together
+  const double step64[3] = {0.40, 0.47, 0.54}, step128[3] = {1.1, 1.25, 1.5};      // not staged by DMA
+  const double alone64[2][3] = {{0.8, 1.1, 1.25}, {0.45, 0.58, 0.62}}, alone128[2][3] = {{1.9, 2.4, 3.0}, {0.8, 0.95, 1.1}};
+  const Opt opts[4] = {{64, 64, 4, esize == 2 ? (vec ? 0.27 : step64[form]) : 0.65, esize == 2 ? alone64[vec][form] : vec ? 0.72 : 1.3},
+                       {128, 128, 2, esize == 2 ? (vec ? 0.55 : step128[form]) : 2.3, esize == 2 ? alone128[vec][form] : vec ? 2.2 : 3.3},
+                       {256, 256, 1, forward ? 1.55 : 1.72, 0.0},
+                       {256, 320, 1, forward ? 1.85 : 2.8, 0.0}};
   Plan best = {};
   double best_us = 1e30;
   const double out = (double)M * N;
@@ -756,8 +758,9 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form, bool twice)
     for (int64_t s = 1; s <= 64 && s * 2 <= (nkt > 2 ? nkt : 2); s += s < 4 ? 1 : s < 16 ? 2 : 8) {
       if (s > 1 && tiles * s > 1536) break;
       const int64_t per = nkt > 0 ? (nkt + s - 1) / s : 1, used = nkt > 0 ? (nkt + per - 1) / per : 1;
-      const double load = (double)((tiles * used + 255) / 256);
-      double us = load * t.step > t.alone ? load * t.step : t.alone;
+      const int64_t load = (tiles * used + 255) / 256, rest = load % t.together;
+      double us = (load - rest) * t.step;
+      if (rest) us += t.alone + (rest - 1) * (t.together * t.step - t.alone) / (t.together > 1 ? t.together - 1 : 1);
       us = us * (twice ? 2 * per : per) + load * t.bm * t.bn * (used > 1 ? 4 : esize) / 20e3;
       if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 6.0;
       if (us < best_us) {
