@@ -642,8 +642,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
 }
 
 // ---- dz = drop(dy) act'(z), and the strips' column sums ----------------------------------------------
-// HBM without an activation (65536x320 bf16 21 us, 4 TB/s), the vector ALU with one (generator and GELU's derivative, about
-// 1700 cycles a wave for 512 elements: 4096x5120 bf16 41 us, 32 of them at least for 168 MB).
+// HBM (65536x320 bf16 without an activation 19 us, 4.4 TB/s; 4096x5120 bf16 with GELU and dropout 34 us, 4.9 TB/s, in spite of
+// about 1700 cycles a wave for 512 elements).  One row at a time and many waves: with two rows in flight and two thirds of
+// the waves these were 22 and 40 us.
 struct DzParams {
   const void* dy; int64_t lddy;
   const float* preact;          // [M][N], null without an activation
@@ -672,35 +673,24 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
   unsigned k0 = 0, k1 = 0;
   if (p.drop.thr) drop_key(p.drop, k0, k1);
   if (cnt > 0 && rl < lanes) {
-    // U rows at a time, their loads ahead of the arithmetic; rows beyond the strip repeat its last one and count nothing
-    constexpr int U = 2;
-    for (int64_t m0 = rb + rl; m0 < re; m0 += U * lanes) {
-      float v[U][8], z[U][8];
+    for (int64_t m = rb + rl; m < re; m += lanes) {
+      float v[8], z[8];
+      load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v);
+      if (p.act != ACT_NONE) load8<float>(p.preact + m * p.N + n, cnt, z);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
+      act_grad_n<T>(z, v, p.act);
+      if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v);
+      if (p.dz_lo) {
+        float lo[8];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t m = m0 + u * lanes < re ? m0 + u * lanes : re - 1;
-        load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v[u]);
-        if (p.act != ACT_NONE) load8<float>(p.preact + m * p.N + n, cnt, z[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t m = m0 + u * lanes;
-        if (m >= re) break;
-        if (p.drop.thr) drop8(v[u], philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
-        act_grad_n<T>(z[u], v[u], p.act);
-        if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v[u]);
-        if (p.dz_lo) {
-          float lo[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float hi = to_f32<T>(from_f32<T>(v[u][e]));
-            lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? v[u][e] - hi : 0.f;      // infinities stay infinite
-          }
-          store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
+        for (int e = 0; e < 8; ++e) {
+          const float hi = to_f32<T>(from_f32<T>(v[e]));
+          lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? v[e] - hi : 0.f;      // infinities stay infinite
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += v[u][e];
+        store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += v[e];
     }
   }
   if (!p.db_partial) return;
@@ -895,16 +885,17 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   if (w.split) { px = plan_product(M, K, N, esize, GRAD_X, true); pw = plan_product(N, K, M, esize, GRAD_W, true); }
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
   w.dz_lo = o; o += w.split ? up256((size_t)M * N * esize) : 0;
-  // column groups a block takes (all, or an even share), and strips of rows: about 1024 blocks, every row lane at
-  // least four rows where there are that many
+  // column groups a block takes (all, or an even share), and strips of rows: about 1536 blocks, every row lane at least
+  // four rows where there are that many, or fewer if that leaves most of the CUs without a block (308x768 with SiLU 6.9 us
+  // in 64 strips, 5.3 in 154)
   const int ncg = (N + 7) / 8;
   w.col_blocks = (ncg + 255) / 256;
   w.groups = (ncg + w.col_blocks - 1) / w.col_blocks;
   const int lanes = 256 / w.groups;
-  int64_t strips = 1024 / w.col_blocks;
+  int64_t strips = 1536 / w.col_blocks;
   if (strips < 1) strips = 1;
   const int64_t by_work = (M + 4 * lanes - 1) / (4 * lanes), by_lane = (M + lanes - 1) / lanes;
-  if (strips > by_work) strips = by_work < 64 ? (by_lane < 64 ? by_lane : 64) : by_work;
+  if (strips > by_work) strips = by_work < 256 ? (by_lane < 256 ? by_lane : 256) : by_work;
   if (strips < 1) strips = 1;
   w.rows_per_strip = (M + strips - 1) / strips;
   w.strips = w.rows_per_strip ? (int)((M + w.rows_per_strip - 1) / w.rows_per_strip) : 0;
