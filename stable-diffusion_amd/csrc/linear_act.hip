@@ -8,7 +8,7 @@
 //   dW       Q = dz columns,  P = x  columns   (contraction over the tokens, split over workgroups)
 // Bounds, MI355X: the matrix rate where the contraction is long (8192x4096x4096 fp16: forward 217 us = 1269 TFLOP/s, dx 238,
 // dW 233; a plain library product 212), HBM where it is short (65536x320x320 bf16: forward with bias, dropout and residual
-// 38 us for 126 MB, dx 28 and dW 28 + 6 us), latency where there is little of anything (308x768x768 bf16 forward 8 us).
+// 38 us for 126 MB, dx 27 and dW 28 + 6 us), latency where there is little of anything (308x768x768 bf16 forward 8 us).
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
@@ -88,10 +88,11 @@ __device__ __forceinline__ void fold_bias_gradient(const DbFold& f, int block, f
   if (n < f.n && rl < 16) {
     const float* src = f.partial + n;
     int i = rl;
-    for (; i + 48 < f.strips; i += 64) {
-      const float a = src[(size_t)i * f.n], b = src[(size_t)(i + 16) * f.n], c = src[(size_t)(i + 32) * f.n],
-                  d = src[(size_t)(i + 48) * f.n];
-      s += (a + b) + (c + d);
+    for (; i + 112 < f.strips; i += 128) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(i + 16 * u) * f.n];
+      s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     }
     for (; i < f.strips; i += 16) s += src[(size_t)i * f.n];
   }
@@ -942,13 +943,15 @@ int linear_bwd(const LinearActArgs& a, const BwdLayout& w, const DropArgs& drop,
   Product w_, x_;
   if (a.dw)
     SDMI_TRY((plan_launch<T, true, true>(&w_, w.plan_w, dz, dz_lo, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha),
-                                         (float*)(ws + w.pw), want_x ? DbFold() : fold)));
+                                         (float*)(ws + w.pw), fold)));
   if (want_x)
     SDMI_TRY((plan_launch<T, false, true>(&x_, w.plan_x, dz, dz_lo, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha),
                                           (float*)(ws + w.px), fold)));
   if (a.dw && want_x && grads_together(w_, x_)) {
+    w_.g.fold = DbFold();
     SDMI_TRY(run_grads<T>(w_, x_, s));
   } else {
+    if (a.dw && want_x) x_.g.fold = DbFold();      // dW's tiles are the smaller ones, which leave a CU room for the fold
     if (a.dw) SDMI_TRY((run_product<T, true, true>(w_, s)));
     if (want_x) SDMI_TRY((run_product<T, false, true>(x_, s)));
   }
