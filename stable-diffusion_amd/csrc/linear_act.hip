@@ -722,8 +722,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 // round), 72 at 256x256 (two rounds); 320x320x65536 34 at 64x64 in 32 splits, 45 at 256x256 in 64; 308x768x768 6.6 at
 // 64x64, 11 at 128x128 in 4 splits, and its dx with the low parts 9 in 4 splits, 16 in one.  fp32 runs at a sixteenth of
 // the matrix rate: 128x128 2.3, 64x64 0.65 (alone 0.72).
-struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; double us; };
-constexpr double SPLIT_US = 15.0;      // see bwd_layout
+struct Plan { int bm, bn; unsigned tiles_m, tiles_n, splits; int64_t k_per_split; };
 
 enum Form { FORWARD, GRAD_X, GRAD_W };
 // sizes that are no whole 16-byte chunks stay off the large tiles
@@ -756,7 +755,7 @@ Plan plan_product(int64_t M, int N, int64_t K, int esize, Form form, bool twice)
       if (used > 1) us += out * (4.0 * used + esize) / 5.2e6 + 6.0;
       if (us < best_us) {
         best_us = us;
-        best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt, us};
+        best = Plan{t.bm, t.bn, (unsigned)tm, (unsigned)tn, (unsigned)used, per * kt};
       }
     }
   }
@@ -877,13 +876,13 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   w.need_dz = (act != ACT_NONE || drop) && (want & 3);
   // With an activation dz = dy act'(z) does not fit the tensors' type, and rounded to it adds an error to dx and dw as
   // large as the rounding of their own (error against 64 bits 1.41 times that of an unrounded dz, more where a few
-  // entries dominate).  Products whose time is mostly their launch's multiply what the rounding lost as well; the larger
-  // ones would take twice as long (4096x1280x5120 bf16 by about 130 us) and live with it.
-  Plan &px = w.plan_x, &pw = w.plan_w;
-  px = plan_product(M, K, N, esize, GRAD_X, false);
-  pw = plan_product(N, K, M, esize, GRAD_W, false);
-  w.split = w.need_dz && act != ACT_NONE && esize == 2 && px.us <= SPLIT_US && pw.us <= SPLIT_US;
-  if (w.split) { px = plan_product(M, K, N, esize, GRAD_X, true); pw = plan_product(N, K, M, esize, GRAD_W, true); }
+  // entries dominate; 43 % of the entries of 4096x1280x5120 bf16 then are not the ones that 64 bits round to, 0.2 % so).
+  // The products therefore take dz in two parts of the type, at any size: how exact a sample's gradient is may not depend
+  // on how many others come with it.  The second part costs the products' time again (4096x1280x5120 bf16: 364 us a training pass, 266 with dz rounded).
+  w.split = w.need_dz && act != ACT_NONE && esize == 2;
+  w.plan_x = plan_product(M, K, N, esize, GRAD_X, w.split);
+  w.plan_w = plan_product(N, K, M, esize, GRAD_W, w.split);
+  const Plan &px = w.plan_x, &pw = w.plan_w;
   w.dz = o; o += w.need_dz ? up256((size_t)M * N * esize) : 0;
   w.dz_lo = o; o += w.split ? up256((size_t)M * N * esize) : 0;
   // column groups a block takes (all, or an even share), and strips of rows: about 1536 blocks, every row lane at least
