@@ -112,7 +112,8 @@ __global__ __launch_bounds__(256) void linear_db_kernel(DbFold f) {
 
 struct GemmParams {
   const char* q; const char* p;      // operands
-  const char* q2;                    // not null: a second Q, multiplied with the same P and added (low parts of Q)
+  const char* q2; float q_scale;     // q2 not null: a second Q, multiplied with the same P and added to the first one's sums times
+                                     // q_scale (the first are then the second's low parts, held larger by 1 / q_scale)
   int64_t ldq, ldp;                  // elements from one stored row to the next
   int64_t K, k_per_split;            // contraction; a split's share is a multiple of the K-tile
   unsigned tiles_n, tiles, splits;
@@ -334,6 +335,16 @@ __device__ __forceinline__ void gemm_block(const GemmParams& p, const unsigned b
   for (int i = 0; i < FP; ++i)
 #pragma unroll
     for (int j = 0; j < FQ; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  auto begin_tile = [&](int t) {     // before the products of K-tile t: behind the first Q its sums are scaled
+    if constexpr (PC) {              // (a forward product has one Q)
+      if (t == nk1) {
+#pragma unroll
+        for (int i = 0; i < FP; ++i)
+#pragma unroll
+          for (int j = 0; j < FQ; ++j) acc[i][j] *= p.q_scale;
+      }
+    }
+  };
 
   constexpr int PH = PAIR ? PAIR : 1, FPH = FP / PH;
   static_assert(FPH * PH == FP, "segments share the column fragments evenly");
@@ -378,6 +389,7 @@ __device__ __forceinline__ void gemm_block(const GemmParams& p, const unsigned b
     barrier();
     if (wp == 1) barrier();
     for (int t = 0; t < nk; ++t) {
+      begin_tile(t);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -404,6 +416,7 @@ __device__ __forceinline__ void gemm_block(const GemmParams& p, const unsigned b
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       if (t + 1 < nk) stage_in(t + 1);
+      begin_tile(t);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) { read_frags(t, kk, 0); multiply(0); }
     }
@@ -412,6 +425,7 @@ __device__ __forceinline__ void gemm_block(const GemmParams& p, const unsigned b
     for (int t = 0; t < nk; ++t) {
       __syncthreads();
       if (t + 1 < nk) stage_in(t + 1);
+      begin_tile(t);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk) { read_frags(t, kk, 0); multiply(0); }
       if (t + 1 < nk) regs_to_lds(t + 1);      // last read in iteration t - 1, before this iteration's barrier
@@ -646,6 +660,14 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
 // HBM (65536x320 bf16 without an activation 19 us, 4.4 TB/s; 4096x5120 bf16 with GELU and dropout 34 us, 4.9 TB/s, in spite of
 // about 1700 cycles a wave for 512 elements).  One row at a time and many waves: with two rows in flight and two thirds of
 // the waves these were 22 and 40 us.
+// With an activation dz is held halved, before the mask's scale, which wait for the products' epilogue (and the sums'): |act'|
+// is at most 1.13, so a finite dy gives a finite dz in its own type.  Its low part is held larger by LO_SCALE: fp16 has no
+// numbers below 2^-24, where the low parts of everything below 2^-13 lie; the first part of at most 2^15.2 leaves at most
+// 32, 2^15 then.  bf16 has the exponents of fp32.
+constexpr float DZ_HELD = 0.5f;
+template <typename T> constexpr float LO_SCALE = 1.f;
+template <> constexpr float LO_SCALE<half_t> = 1024.f;
+
 struct DzParams {
   const void* dy; int64_t lddy;
   const float* preact;          // [M][N], null without an activation
@@ -654,8 +676,8 @@ struct DzParams {
   float* db_partial;            // [strips][N] or null
   int64_t M, rows_per_strip;
   int N, act, groups;
-  float db_scale;
-  DropArgs drop;
+  float held, db_scale;         // held: what dy is multiplied by
+  DropArgs drop;                // (its scale unused)
 };
 
 // A block takes `groups` column groups of eight (256 at most) x as many row lanes as its threads give, of one strip:
@@ -678,7 +700,11 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
       float v[8], z[8];
       load8<T>((const T*)p.dy + m * p.lddy + n, cnt, v);
       if (p.act != ACT_NONE) load8<float>(p.preact + m * p.N + n, cnt, z);
-      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.drop.scale);
+      if (p.drop.thr) drop8(v, philox8(k0, k1, (unsigned)cgg, (uint64_t)m, p.drop.offset), p.drop.thr, p.held);
+      else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= p.held;
+      }
       act_grad_n<T>(z, v, p.act);
       if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v);
       if (p.dz_lo) {
@@ -686,7 +712,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float hi = to_f32<T>(from_f32<T>(v[e]));
-          lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? v[e] - hi : 0.f;      // infinities stay infinite
+          lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? (v[e] - hi) * LO_SCALE<T> : 0.f;      // infinities stay infinite
         }
         store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
       }
@@ -806,7 +832,7 @@ int launch_join(const float* partial, unsigned splits, const Epilogue& e, hipStr
   return SDMI_OK;
 }
 
-// out[m][n] = epilogue(sum_k (Q + Q2)(m, k) P(n, k)); Q2 may be null
+// out[m][n] = epilogue(sum_k Q(m, k) P(n, k)), or with a Q2 sum_k (Q / LO_SCALE + Q2)(m, k) P(n, k)
 constexpr uint64_t MAX_BLOCKS = (1ull << 32) / 512;      // a launch has less than 2^32 threads: 512 a block, or 256 for two products
 struct Product { GemmParams g; Plan pl; bool vec; };
 template <typename T, bool QC, bool PC>
@@ -819,7 +845,7 @@ int plan_launch(Product* pr, Plan pl, const void* q, const void* q2, int64_t ldq
     pl.tiles_m = (unsigned)((e.M + 127) / 128); pl.tiles_n = (unsigned)((e.N + 127) / 128);
   }
   GemmParams& g = pr->g;
-  g.q = (const char*)q; g.q2 = (const char*)q2; g.p = (const char*)p; g.fold = fold; g.ldq = ldq; g.ldp = ldp; g.K = K;
+  g.q = (const char*)q; g.q2 = (const char*)q2; g.q_scale = 1.f / LO_SCALE<T>; g.p = (const char*)p; g.fold = fold; g.ldq = ldq; g.ldp = ldp; g.K = K;
   g.k_per_split = pl.k_per_split; g.tiles_n = pl.tiles_n; g.splits = pl.splits; g.e = e;
   const uint64_t total = (uint64_t)pl.tiles_m * pl.tiles_n * pl.splits;
   const uint64_t folds = fold.db ? (uint64_t)(fold.n + DB_COLS - 1) / DB_COLS : 0;
@@ -917,8 +943,8 @@ int linear_bwd(const LinearActArgs& a, const BwdLayout& w, const DropArgs& drop,
   char* ws = (char*)a.workspace;
   const void* dz = a.dy;
   int64_t lddz = a.lddy;
-  // without an activation dz is dy, masked: its scale waits for the products' epilogue, so that nothing is rounded here
-  const float alpha = a.act == ACT_NONE && drop.thr ? drop.scale : 1.f;
+  // the mask's scale waits for the products' epilogue: without an activation dz is dy, masked, and nothing is rounded here
+  const float held = a.act != ACT_NONE ? DZ_HELD : 1.f, alpha = (drop.thr ? drop.scale : 1.f) / held;
   DbFold fold;
   if (a.rows > 0 && (w.need_dz || a.db)) {
     DzParams d;
@@ -927,8 +953,7 @@ int linear_bwd(const LinearActArgs& a, const BwdLayout& w, const DropArgs& drop,
     d.dz_lo = w.split ? ws + w.dz_lo : nullptr;
     d.db_partial = a.db ? (float*)(ws + w.dbp) : nullptr;
     d.M = a.rows; d.rows_per_strip = w.rows_per_strip; d.N = a.n; d.act = a.act; d.drop = drop; d.groups = w.groups;
-    if (a.act == ACT_NONE) d.drop.scale = 1.f;
-    d.db_scale = alpha;
+    d.held = held; d.db_scale = alpha;
     char label[64] = "";
     if (prof_on()) snprintf(label, sizeof(label), "linear dz %lldx%d", (long long)a.rows, a.n);
     ProfScope prof(PROF_OTHER, s, 0.0, 2.0 * a.rows * (double)a.n * sizeof(T), label);
@@ -937,14 +962,16 @@ int linear_bwd(const LinearActArgs& a, const BwdLayout& w, const DropArgs& drop,
     if (w.need_dz) { dz = d.dz; lddz = a.n; }
   }
   if (a.db) { fold.partial = (const float*)(ws + w.dbp); fold.strips = a.rows > 0 ? w.strips : 0; fold.n = a.n; fold.db = a.db; }
-  const void* dz_lo = a.rows > 0 && w.split ? ws + w.dz_lo : nullptr;
+  // the products' operands: dz, or its low part and then dz
+  const void* q = a.rows > 0 && w.split ? ws + w.dz_lo : dz;
+  const void* q2 = q != dz ? dz : nullptr;
   const bool want_x = a.dx && a.rows > 0;
   Product w_, x_;
   if (a.dw)
-    SDMI_TRY((plan_launch<T, true, true>(&w_, w.plan_w, dz, dz_lo, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha),
+    SDMI_TRY((plan_launch<T, true, true>(&w_, w.plan_w, q, q2, lddz, a.x, a.ldx, a.rows, plain_out(a.dw, a.n, a.k, alpha),
                                          (float*)(ws + w.pw), fold)));
   if (want_x)
-    SDMI_TRY((plan_launch<T, false, true>(&x_, w.plan_x, dz, dz_lo, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha),
+    SDMI_TRY((plan_launch<T, false, true>(&x_, w.plan_x, q, q2, lddz, a.w, a.ldw, a.n, plain_out(a.dx, a.rows, a.k, alpha),
                                           (float*)(ws + w.px), fold)));
   if (a.dw && want_x && grads_together(w_, x_)) {
     w_.g.fold = DbFold();

@@ -34,7 +34,75 @@ def exact_linear(x, w, bias, dy, act, p, seed, offset):
     return z, dz, dz @ w, dz.t().contiguous() @ x, dz.sum(0)
 
 
+def gradient_bounds(x, w, z, dz, dt):
+    """Bounds of dx and dw whose only rounding to 16 bits is their own: the two parts of dz hold it to eps^2 / 2 (the first
+    is within eps of it, the second within eps / 2 of what is left), its derivative is off by ACT_ERR per unit of |z| and
+    by 0.86 times z's error of (k + 2) u, and n products sum to within (n + 2) u of their magnitudes."""
+    eps, half = torch.finfo(dt).eps, R.half(dt)
+    x, w = x.detach().double().abs(), w.detach().double().abs()
+    k, n = w.shape[1], w.shape[0]
+    ez = (k + 2) * R.U * (x @ w.t())
+    # |dz| / |act'| is |dy| times the mask; its largest value bounds it where the derivative is near 0
+    top = dz.abs().amax()
+    edz = (eps * eps / 2 + 8 * R.U) * dz.abs() + 2 * top * (0.86 * ez + R.ACT_ERR * z.abs().clamp(min=1))
+    out = []
+    for terms, err, m in ((dz.abs() @ w, edz @ w, n), (dz.abs().t().contiguous() @ x, edz.t().contiguous() @ x, x.shape[0])):
+        out.append(err + (m + 2) * R.U * (terms + err))
+    return out
+
+
+def check(name, got, want, err, dt):
+    """Entries that the type does not hold are infinite, those within an error of its end may be."""
+    top, got = torch.finfo(dt).max, got.detach().clone()
+    assert torch.equal(got[want.abs() > top + 2 * err + R.half(dt) * top].double(),
+                       want[want.abs() > top + 2 * err + R.half(dt) * top].sign() * math.inf), name
+    near = (want.abs() > top - err) & torch.isinf(got) & (got.sign() == want.sign())
+    got = torch.where(near, want.clamp(-top, top).to(dt), got)
+    want = torch.where(near, got.double(), want)
+    R.check(name, got, want.cpu(), R.rounded(want, err, dt).cpu())
+
+
 # ---- gradients at the ends of the types' range ----------------------------------------------------------------
+
+@halves
+@pytest.mark.parametrize("act", ["silu", "gelu", "quick_gelu"])
+@pytest.mark.parametrize("m,n", [(5, 24), (300, 136)])
+def test_finite_gradients_stay_finite(act, dt, m, n):
+    """dy near the type's largest value, doubled by the dropout's scale and times a slope of up to 1.13, leaves the type;
+    dx and (but for a few sums over many rows) dw, its products with small numbers, do not."""
+    dt = DT[dt]
+    k = 64
+    x, w = rand(m, k, dtype=dt, scale=2.0 ** -6, grad=True), rand(n, k, dtype=dt, seed=1, scale=2.0 ** -7, grad=True)
+    b = (3.0 * rand(n, seed=2)).detach().requires_grad_()      # slopes on both sides of 1
+    g = torch.Generator().manual_seed(3)
+    dy = torch.finfo(dt).max * (0.6 + 0.35 * torch.rand(m, n, generator=g)) * torch.randn(m, n, generator=g).sign()
+    dy = dy.to(dt).cuda()
+    dx, dw = torch.autograd.grad(ops.linear_act(x, w, b, act=act, p=0.5, seed=9), (x, w), dy)
+    z, dz, wx, ww, _ = exact_linear(x, w, b, dy, act, 0.5, 9, 0)
+    assert float(dz.abs().max()) > torch.finfo(dt).max and float(wx.abs().max()) < torch.finfo(dt).max
+    assert float((ww.abs() < torch.finfo(dt).max).double().mean()) > 0.9
+    ex, ew = gradient_bounds(x, w, z, dz, dt)
+    check("dx", dx, wx, ex, dt)
+    check("dw", dw, ww, ew, dt)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "quick_gelu"])
+def test_small_fp16_gradients_add_up(act):
+    """Entries of dz below half of fp16's smallest number still count: thousands of them make a dw that fp16 holds."""
+    dt, m, k, n = torch.float16, 20000, 64, 40
+    x, w = (1 + rand(m, k).abs()).to(dt).requires_grad_(), rand(n, k, dtype=dt, seed=1, scale=0.02, grad=True)
+    b = torch.full((n,), -2.5, device="cuda", requires_grad=True)
+    dy = torch.full((m, n), 2.0 ** -24, dtype=dt, device="cuda")
+    dx, dw = torch.autograd.grad(ops.linear_act(x, w, b, act=act), (x, w), dy)
+    z, dz, wx, ww, _ = exact_linear(x, w, b, dy, act, 0.0, 0, 0)
+    assert float(dz.abs().max()) < 2.0 ** -24
+    ex, ew = gradient_bounds(x, w, z, dz, dt)
+    floor = 2.0 ** -34           # half of the second part's smallest step 2^-24, which is held 1024 times larger, dz being halved
+    ex += floor * w.detach().double().abs().sum(0)
+    ew += floor * x.detach().double().abs().sum(0)
+    check("dx", dx, wx, ex, dt)
+    check("dw", dw, ww, ew, dt)
+
 
 @halves
 @pytest.mark.parametrize("m,k,n,act,p", [(616, 768, 2000, "quick_gelu", 0.0), (2048, 320, 1280, "gelu", 0.1),
