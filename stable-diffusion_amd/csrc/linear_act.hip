@@ -668,6 +668,21 @@ constexpr float DZ_HELD = 0.5f;
 template <typename T> constexpr float LO_SCALE = 1.f;
 template <> constexpr float LO_SCALE<half_t> = 1024.f;
 
+// v = hi + lo / LO_SCALE.  Both parts have v's sign and neither is 0 unless v is (or is below the type's smallest number): an
+// infinite x or W then gives the infinity of v's sign in both products, where a low part of 0 or of the other sign would
+// make it a NaN.  hi is the next number of the type towards 0, so lo is at most one of its steps and rounds to a 2^-15th
+// (bf16; fp16 a 2^-21st) of v.  An infinite or NaN v is both.
+template <typename T> __device__ __forceinline__ void split_in_two(float v, float& hi, float& lo) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  hi = lo = v;
+  if ((u & 0x7FFFFFFFu) - 1u < 0x7F7FFFFFu) {             // finite, not 0
+    const float below = __builtin_bit_cast(float, u - 1u);
+    if constexpr (__is_same(T, half_t)) hi = (float)__builtin_amdgcn_cvt_pkrtz(below, below)[0];
+    else hi = __builtin_bit_cast(float, (u - 1u) & 0xFFFF0000u);
+    lo = (v - hi) * LO_SCALE<T>;
+  }
+}
+
 struct DzParams {
   const void* dy; int64_t lddy;
   const float* preact;          // [M][N], null without an activation
@@ -706,18 +721,15 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(DzParams p) {
         for (int e = 0; e < 8; ++e) v[e] *= p.held;
       }
       act_grad_n<T>(z, v, p.act);
-      if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += v[e];
       if (p.dz_lo) {
         float lo[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float hi = to_f32<T>(from_f32<T>(v[e]));
-          lo[e] = __builtin_fabsf(hi) < __builtin_inff() ? (v[e] - hi) * LO_SCALE<T> : 0.f;      // infinities stay infinite
-        }
+        for (int e = 0; e < 8; ++e) split_in_two<T>(v[e], v[e], lo[e]);
         store8<T>((T*)p.dz_lo + m * p.N + n, cnt, lo);
       }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += v[e];
+      if (p.dz) store8<T>((T*)p.dz + m * p.N + n, cnt, v);
     }
   }
   if (!p.db_partial) return;

@@ -105,6 +105,34 @@ def test_small_fp16_gradients_add_up(act):
 
 
 @halves
+@pytest.mark.parametrize("act", ["silu", "gelu", "quick_gelu"])
+def test_infinite_inputs_and_weights_make_infinite_gradients(act, dt):
+    """dx = dz W and dw = dz^T x of an infinite W or x are infinite with the sign of the products, not NaN, whatever dz is
+    (numbers that 16 bits hold among them)."""
+    dt = DT[dt]
+    m, k, n = 70, 24, 40
+    x, w = rand(m, k, dtype=dt), rand(n, k, dtype=dt, seed=1, scale=0.3)
+    b = torch.zeros(n, device="cuda")
+    dy = (1 + rand(m, n, seed=2).abs()).to(dt)
+    dy[:, ::2] = 1.0
+    w[:, 5] = 0.25
+    xi = x.clone()
+    xi[3, 5] = float("inf")                           # z = inf in row 3, where the slope is 1 and dz = dy
+    wl = w.clone().requires_grad_()
+    dw, = torch.autograd.grad(ops.linear_act(xi, wl, b, act=act), wl, dy)
+    assert torch.isposinf(dw[:, 5]).all()
+    finite = torch.ones(k, dtype=torch.bool)
+    finite[5] = False
+    assert torch.isfinite(dw[:, finite.cuda()]).all()
+    xs = x.abs()                                      # W[7][0] = inf, x > 0: z = inf in column 7, dx[:, 0] = inf
+    wi = w.clone()
+    wi[7, 0] = float("inf")
+    xs.requires_grad_()
+    dx, = torch.autograd.grad(ops.linear_act(xs, wi, b, act=act), xs, dy)
+    assert torch.isposinf(dx[:, 0]).all() and torch.isfinite(dx[:, 1:]).all()
+
+
+@halves
 @pytest.mark.parametrize("m,k,n,act,p", [(616, 768, 2000, "quick_gelu", 0.0), (2048, 320, 1280, "gelu", 0.1),
                                          (2056, 1992, 2568, "silu", 0.1), (4096, 1280, 5120, "gelu", 0.1)])
 def test_large_products_lose_nothing_but_their_own_rounding(m, k, n, act, p, dt):
