@@ -76,9 +76,11 @@ __device__ __forceinline__ void drop8(float (&v)[8], const Keep8& k, unsigned th
 }
 
 // ---- activations ---------------------------------------------------------------------------------
-// fp32 tensors take the library functions, or (sigmoid) as good as those; 16-bit ones the hardware exponential (relative error a few 2^-23, times
-// the exponent's size) and, for the normal distribution function of GELU, Abramowitz & Stegun 7.1.26
-// (|error| <= 1.5e-7), whose exponential also gives the density that the derivative needs.
+// fp32 tensors take the library functions, or (sigmoid) as good as those; 16-bit ones the hardware exponential (relative
+// error a few 2^-23, times the exponent's size) and, for the normal distribution function of GELU, e^{-x^2} t P(t) with
+// t = 1 / (1 + 0.43 x) and P of degree 7: a fit of erfc(x) e^{x^2} / 2 on 0 <= x <= 10 by Lawson's reweighted least squares,
+// whose error is relative (1e-7, 4e-7 as evaluated), so that the tail that GELU shows below -3 keeps all the digits of 16
+// bits; one exponential gives the density for the derivative too.
 // e^-x reaches infinity below x = -88, where the reciprocal is 0
 template <typename T> __device__ __forceinline__ float sigmoid_for(float x) {
   if constexpr (sizeof(T) == 4) {
@@ -102,12 +104,15 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float z, float
     const float x = fabsf(z) * 0.70710678118654752440f;
     const float ex = __expf(-x * x);
     if (pdf) *pdf = 0.39894228040143267794f * ex;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-    float q = fmaf(1.061405429f, t, -1.453152027f);
-    q = fmaf(q, t, 1.421413741f);
-    q = fmaf(q, t, -0.284496736f);
-    q = fmaf(q, t, 0.254829592f);
-    q = 0.5f * q * t * ex;                       // upper tail beyond |z|
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.43f, x, 1.f));
+    float q = fmaf(0.0365728475f, t, -0.154047564f);
+    q = fmaf(q, t, 0.189943194f);
+    q = fmaf(q, t, -0.0411517546f);
+    q = fmaf(q, t, 0.122540131f);
+    q = fmaf(q, t, 0.102736309f);
+    q = fmaf(q, t, 0.122146904f);
+    q = fmaf(q, t, 0.121259913f);
+    q = q * t * ex;                              // upper tail beyond |z|
     return z < 0.f ? q : 1.f - q;
   }
 }

@@ -147,3 +147,23 @@ def test_large_products_lose_nothing_but_their_own_rounding(m, k, n, act, p, dt)
     for name, got, want in (("dx", grads[0], dx), ("dw", grads[1], dw)):
         own = float((want.to(dt).double() - want).norm())
         assert float((got.double() - want).norm()) < 1.01 * own, name
+
+
+# ---- activations --------------------------------------------------------------------------------------------------
+
+@halves
+def test_gelu_holds_its_lower_tail(dt):
+    """Relative to the value, where GELU approaches zero: the exponential's argument z^2 / 2 <= 41 is off by 2 u of itself
+    and the base's change by as much again, the fit by 3e-7: 2e-5 in all.  The derivative is Phi + z phi, each so exact."""
+    dt = DT[dt]
+    z = torch.linspace(-9, 0, 4001)[:-1] if dt == torch.bfloat16 else torch.linspace(-5.5, 0, 4001)[:-1]
+    x = z.to(dt).cuda().view(-1, 1).requires_grad_()
+    y = ops.linear_act(x, torch.ones(1, 1, dtype=dt, device="cuda"), act="gelu")
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    zr = R.d(x)
+    phi, pdf = 0.5 * torch.special.erfc(-zr / math.sqrt(2.0)), torch.exp(-zr * zr / 2) / math.sqrt(2 * math.pi)
+    R.check("y", y, zr * phi, R.rounded(zr * phi, 2e-5 * (zr * phi).abs(), dt))
+    want, err = phi + zr * pdf, 2e-5 * (phi + (zr * pdf).abs())
+    # dx = dz * 1 in two parts: eps^2 / 2 and half of the second one's smallest step
+    err = err + torch.finfo(dt).eps ** 2 / 2 * want.abs() + 2.0 ** -34
+    R.check("dx", dx, want, R.rounded(want, err, dt))
