@@ -7,9 +7,10 @@
 // A (sample, group) slice that fits LDS is one workgroup's work: read once, normalised from LDS, one launch (the
 // weight gradients of several samples take a second one).  Larger slices take two launches over strips of pixels:
 // the first leaves per-strip sums, the second folds them in double and finishes the strip.  Every sum is taken in a
-// fixed order.  Statistics are taken about a value of the group, so that a common offset does not cancel in
-// E[x^2] - E[x]^2: about the middle one of three far apart, because an outlier a (feature maps have them, in corners too)
-// would make the sums' rounding a^2 times that of a variance that may be a^2 / n.
+// fixed order.  Statistics never go through E[x^2] - E[x]^2, where a common offset or an outlier a (feature maps have them, in
+// corners too) leaves the rounding of a^2 in a variance that may be a^2 / n.  A slice takes two passes over LDS.  A thread
+// of a strip updates its columns' running means and squares about them (Welford 1962); a group's threads and columns, and
+// then the strips, are joined by the squares of their means' distances from the joint mean (Chan, Golub, LeVeque 1979).
 //
 // Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 11 us (HBM: 8), apply 23, gradient
 // sums 23, gradient apply 26 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
@@ -37,7 +38,7 @@ struct GnaParams {
   DropArgs drop;
   float* stats;                               // [B][G][2]: mean, rstd
   int strips; int64_t px_per_strip;
-  float* part;                                // [B][strips][G][2] sums of a strip's groups
+  float* part;                                // [B][strips][G][2] of a strip's groups: mean and squares about it; backward sums
   float* cpart;                               // backward: [B][strips][2][C] sums of a strip's channels
   float* dgamma; float* dbeta;
   int apply_blocks;                           // backward: blockIdx.x beyond fold dgamma / dbeta
@@ -122,17 +123,6 @@ __device__ __forceinline__ void load_params(const float* p, int c, int C, float 
     for (int e = 0; e < 8; ++e) v[e] = p[c + e < C ? c + e : C - 1];
   }
 }
-template <typename T> __device__ __forceinline__ float element(const GnaParams& p, int64_t row, int c) {
-  return c < p.c0 ? to_f32<T>(((const T*)p.x0)[row * p.c0 + c]) : to_f32<T>(((const T*)p.x1)[row * p.c1 + (c - p.c0)]);
-}
-// the value that the sums of sample b's group g are taken about
-template <typename T> __device__ __forceinline__ float shift_of(const GnaParams& p, int b, int g) {
-  const int64_t row = (int64_t)b * p.HW;
-  const int c = g * p.cpg;
-  return __builtin_amdgcn_fmed3f(element<T>(p, row, c), element<T>(p, row + p.HW / 2, c + p.cpg / 2),
-                                 element<T>(p, row + p.HW - 1, c + p.cpg - 1));
-}
-
 // W columns from c on, that do not leave their group of eight
 template <int W>
 __device__ __forceinline__ void drop_n(const DropArgs& d, unsigned k0, unsigned k1, int64_t row, int c, float (&v)[W]) {
@@ -359,70 +349,96 @@ __global__ __launch_bounds__(1024) void gna_stats_kernel(GnaParams p) {
   const Walk w = walk_of(p, strip, b);
   typedef Cols<T, WHOLE> C;
   const int width = w.ncg * 8;
-  float* s1 = reinterpret_cast<float*>(smem);
-  float* s2 = s1 + w.lanes * width;
+  float* s_mean = reinterpret_cast<float*>(smem);      // [lanes][width] each
+  float* s_sq = s_mean + w.lanes * width;
   const int c = w.cg * 8;
   const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
-  typename C::Raw r[WALK];                     // the first pixels come while the groups' shifts go round
-  if (w.live) fetch(x, w, w.pl, r);
-  for (int g = threadIdx.x; g < p.G; g += (int)blockDim.x) s1[g] = shift_of<T>(p, b, g);
-  __syncthreads();
-  float sh[8], s[8], q[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    sh[e] = s1[div_by((unsigned)(c + e < p.C ? c + e : p.C - 1), p.div_cpg)];
-    s[e] = 0.f; q[e] = 0.f;
-  }
-  __syncthreads();
+  typename C::Raw r[WALK];
   if (w.live) {
+    fetch(x, w, w.pl, r);
+    float mean[8], sq[8], n = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { mean[e] = 0.f; sq[e] = 0.f; }
     for (int px = w.pl; px < w.count; px += WALK * w.lanes) {
 #pragma unroll
       for (int u = 0; u < WALK; ++u) {
         if (px + u * w.lanes >= w.count) break;
+        n += 1.f;
+        const float inv = __builtin_amdgcn_rcpf(n);    // within an ulp, a rounding like the others (and 1 / 1 is 1)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) { const float t = to_f32<T>(r[u][e]) - sh[e]; s[e] += t; q[e] = fmaf(t, t, q[e]); }
+        for (int e = 0; e < 8; ++e) {
+          const float v = to_f32<T>(r[u][e]), d = v - mean[e];
+          mean[e] = fmaf(d, inv, mean[e]);
+          sq[e] = fmaf(d, v - mean[e], sq[e]);
+        }
       }
       if (px + WALK * w.lanes < w.count) fetch(x, w, px + WALK * w.lanes, r);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) { s1[w.pl * width + c + e] = s[e]; s2[w.pl * width + c + e] = q[e]; }
+    for (int e = 0; e < 8; ++e) { s_mean[w.pl * width + c + e] = mean[e]; s_sq[w.pl * width + c + e] = sq[e]; }
   }
-  fold_pixel_lanes(s1, s2, w.lanes, width);
+  __syncthreads();
+  // a group's lanes and columns: the joint mean about the first of them, then all squares about that
   const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
+  const int lanes = min(w.lanes, w.count), every = w.count / w.lanes, more = w.count - every * w.lanes;    // pixels: every, or one more
+  const int l0 = j / p.cpg, dl = tpg / p.cpg, k0 = j - l0 * p.cpg, dk = tpg - dl * p.cpg;
+  const float inv_n = 1.f / ((float)w.count * (float)p.cpg);
   for (int g0 = 0; g0 < p.G; g0 += (int)blockDim.x / tpg) {                // every lane goes round equally often (shuffles)
     const int g = g0 + (int)threadIdx.x / tpg;
-    float a = 0.f, q = 0.f;
+    auto each = [&](auto fn) {       // fn(pixels, mean, squares about it) of this thread's share of lanes x columns
+      for (int l = l0, k = k0; l < lanes;) {
+        const int i = l * width + g * p.cpg + k;
+        fn((float)(every + (l < more ? 1 : 0)), s_mean[i], s_sq[i]);
+        l += dl; k += dk;
+        if (k >= p.cpg) { k -= p.cpg; ++l; }
+      }
+    };
+    float at = 0.f, a = 0.f;
+    if (g < p.G) {
+      at = s_mean[g * p.cpg];
+      each([&](float n, float m, float) { a = fmaf(n, m - at, a); });
+    }
+    at = fmaf(fold_lanes(a, tpg), inv_n, at);
+    float d = 0.f, q = 0.f;
     if (g < p.G)
-      for (int c = j; c < p.cpg; c += tpg) { a += s1[g * p.cpg + c]; q += s2[g * p.cpg + c]; }
-    a = fold_lanes(a, tpg);
+      each([&](float n, float m, float sq) {
+        const float t = m - at;
+        d = fmaf(n, t, d);                             // what the first sum's rounding left over
+        q += fmaf(n * t, t, sq);
+      });
+    d = fold_lanes(d, tpg) * inv_n;
     q = fold_lanes(q, tpg);
     if (g < p.G && j == 0) {
       float* dst = p.part + (((size_t)b * p.strips + strip) * p.G + g) * 2;
-      dst[0] = a; dst[1] = q;
+      dst[0] = at + d;
+      q -= d * d * (float)w.count * (float)p.cpg;
+      dst[1] = q < 0.f ? 0.f : q;                      // (a NaN stays)
     }
   }
 }
 
-// sums over the strips of sample b, per group, in double: fin(g, first sum, second sum) on one thread per group
-template <typename Fn> __device__ __forceinline__ void fold_strips(const GnaParams& p, int b, Fn fin) {
+// sums over the strips of sample b, per group, in double, of add's two terms of a strip's pair (and of the first strip's first
+// number): fin(g, that number, first sum, second sum) on one thread per group
+template <typename Add, typename Fn> __device__ __forceinline__ void fold_strips(const GnaParams& p, int b, Add add, Fn fin) {
   const int tpg = threads_per_group(p.G), j = threadIdx.x & (tpg - 1);
   for (int g0 = 0; g0 < p.G; g0 += (int)blockDim.x / tpg) {
     const int g = g0 + (int)threadIdx.x / tpg;
-    double a = 0.0, q = 0.0;
+    double a = 0.0, q = 0.0, at = 0.0;
     if (g < p.G) {
       const float2* src = reinterpret_cast<const float2*>(p.part) + (size_t)b * p.strips * p.G + g;
+      at = (double)src[0].x;
       for (int s0 = j; s0 < p.strips; s0 += 8 * tpg) {       // eight loads in flight, the ones beyond the end count nothing
         float2 v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = src[(size_t)min(s0 + u * tpg, p.strips - 1) * p.G];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-          if (s0 + u * tpg < p.strips) { a += (double)v[u].x; q += (double)v[u].y; }
+          if (s0 + u * tpg < p.strips) add(s0 + u * tpg, at, v[u], a, q);
       }
     }
     a = fold_lanes(a, tpg);
     q = fold_lanes(q, tpg);
-    if (g < p.G && j == 0) fin(g, a, q);
+    if (g < p.G && j == 0) fin(g, at, a, q);
   }
 }
 
@@ -440,11 +456,16 @@ __global__ __launch_bounds__(1024) void gna_apply_kernel(GnaParams p) {
   const int c = w.cg * 8;
   const C x(p.x0, p.x1, p.c0, p.c1, c, w.row0);
   if (w.live) fetch(x, w, w.pl, r);
-  fold_strips(p, b, [&](int g, double a, double q) {
-    const double n = (double)p.HW * (double)p.cpg, m = a / n;
+  const double n_strip = (double)p.px_per_strip * (double)p.cpg, n = (double)p.HW * (double)p.cpg;
+  fold_strips(p, b, [&](int s, double at, float2 v, double& a, double& q) {
+    const double w = s < p.strips - 1 ? n_strip : n - n_strip * (double)(p.strips - 1), d = (double)v.x - at;
+    a += w * d;
+    q += (double)v.y + w * d * d;
+  }, [&](int g, double at, double a, double q) {
+    const double m = a / n;
     double var = q / n - m * m;
     if (var < 0.0) var = 0.0;
-    const float mean = (float)((double)shift_of<T>(p, b, g) + m), rstd = (float)(1.0 / sqrt(var + (double)p.eps));
+    const float mean = (float)(at + m), rstd = (float)(1.0 / sqrt(var + (double)p.eps));
     s_mean[g] = mean; s_rstd[g] = rstd;
     if (strip == 0) {
       p.stats[((size_t)b * p.G + g) * 2] = mean;
@@ -614,7 +635,8 @@ __global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
     fetch(x, w, w.pl, rx);
     fetch(dy, w, w.pl, rd);
   }
-  fold_strips(p, b, [&](int g, double a, double q) {
+  fold_strips(p, b, [](int, double, float2 v, double& a, double& q) { a += (double)v.x; q += (double)v.y; },
+              [&](int g, double, double a, double q) {
     const double n = (double)p.HW * (double)p.cpg;
     s_a[g] = (float)(a / n); s_q[g] = (float)(q / n);
   });

@@ -167,3 +167,60 @@ def test_gelu_holds_its_lower_tail(dt):
     # dx = dz * 1 in two parts: eps^2 / 2 and half of the second one's smallest step
     err = err + torch.finfo(dt).eps ** 2 / 2 * want.abs() + 2.0 ** -34
     R.check("dx", dx, want, R.rounded(want, err, dt))
+
+
+# ---- statistics and sums ----------------------------------------------------------------------------------------
+
+def two_pass(x, groups, eps):
+    """mean and 1 / sqrt(var + eps) per (sample, group) in 64 bits, and bounds: every value is off by at most u |mean| + 100 u
+    of the group's spread about its mean, as updates of a running mean and folds of a few dozen terms leave it, and the
+    spread's square by 200 u of itself (each square and each running sum's step, 100 values at most one after another)."""
+    b, c = x.shape[0], x.shape[-1]
+    v = x.reshape(b, -1, groups, c // groups)
+    mean = v.mean((1, 3), keepdim=True)
+    t = v - mean
+    var = (t * t).mean((1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    return v, mean, rstd, R.U * mean.abs() + 100 * R.U * t.abs().mean((1, 3), keepdim=True), 100 * R.U * var * rstd ** 2 + 4 * R.U
+
+
+@pytest.mark.parametrize("hot", [("first", "last"), ("first", "middle"), ("middle", "last"), ("first", "middle", "last"),
+                                 ("second", "last")])
+@pytest.mark.parametrize("far", [100.0, 700.0, 1e5])
+@pytest.mark.parametrize("b,hw,c,groups", [(2, (8, 8), 64, 8), (1, (200, 201), 64, 4), (2, (64, 65), 30, 3), (1, (256, 256), 8, 1)])
+def test_groupnorm_act_with_several_outliers(b, hw, c, groups, far, hot):
+    """Pixels far from the others, wherever they are and however many: the statistics may not be their rounding."""
+    n = hw[0] * hw[1]
+    x = rand(b, n, c)
+    at = {"first": 0, "second": 1, "middle": n // 2, "last": n - 1}
+    for h in hot:
+        x[:, at[h]] += far
+    x = x.reshape(b, *hw, c).requires_grad_()
+    gamma, beta = torch.ones(c, device="cuda", requires_grad=True), torch.zeros(c, device="cuda", requires_grad=True)
+    dy = rand(b, *hw, c, seed=4)
+    y = ops.groupnorm_act(x, gamma, beta, 1e-5, act=None, groups=groups)
+    grads = torch.autograd.grad(y, [x, gamma, beta], dy)
+    v, mean, rstd, emean, ers = two_pass(R.d(x), groups, 1e-5)
+    xh = (v - mean) * rstd
+    exh = rstd * (emean + R.U * v.abs()) + xh.abs() * (ers + 4 * R.U)
+    R.check("y", y, xh.reshape(x.shape), R.rounded(xh, exh, torch.float32).reshape(x.shape))
+    h = R.d(dy).reshape(v.shape)
+    a, q = h.mean((1, 3), keepdim=True), (h * xh).mean((1, 3), keepdim=True)
+    S = 200 * R.U
+    ea = S * h.abs().mean((1, 3), keepdim=True)
+    eq = (h.abs() * exh + S * (h * xh).abs()).mean((1, 3), keepdim=True)
+    dx = rstd * (h - a - xh * q)
+    edx = rstd * (ea + xh.abs() * eq + exh * q.abs()) + (ers + 8 * R.U) * rstd * (h.abs() + a.abs() + (xh * q).abs())
+    R.check("dx", grads[0], dx.reshape(x.shape), R.rounded(dx, edx, torch.float32).reshape(x.shape))
+    dg, edg = (h * xh).sum((0, 1)).reshape(c), (h.abs() * exh + 400 * R.U * (h * xh).abs()).sum((0, 1)).reshape(c)
+    R.check("dgamma", grads[1], dg, R.rounded(dg, edg, torch.float32))
+
+
+def test_groupnorm_act_far_from_zero_over_strips():
+    """A common offset of 20000 spreads: each value is off by its own rounding, the statistics by no more."""
+    x = (rand(1, 200, 201, 64, scale=0.05) + 1000.0)
+    v, mean, rstd, emean, ers = two_pass(R.d(x), 4, 1e-5)
+    y = ops.groupnorm_act(x, torch.ones(64, device="cuda"), torch.zeros(64, device="cuda"), 1e-5, act=None, groups=4)
+    xh = (v - mean) * rstd
+    exh = rstd * (emean + R.U * mean.abs()) + xh.abs() * (ers + 4 * R.U)
+    R.check("y", y, xh.reshape(x.shape), R.rounded(xh, exh, torch.float32).reshape(x.shape))
