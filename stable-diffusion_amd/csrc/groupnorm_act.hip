@@ -591,24 +591,26 @@ __global__ __launch_bounds__(1024) void gna_grad_sums_kernel(GnaParams p) {
   }
 }
 
-// dgamma / dbeta: sum of `rows` rows [2][C] of channel sums; a block takes 16 channels x 16 row lanes
-__device__ __forceinline__ void fold_channels(const GnaParams& p, int block, int64_t rows, float* red) {
+// dgamma / dbeta: sum of `rows` rows [2][C] of channel sums; a block takes 16 channels x 16 row lanes.  In double: a lane adds
+// up to 4096 rows one after the other (65535 samples of a slice each; in fp32 their rounding was 9 steps of dbeta).
+constexpr int FOLD_LDS = 2 * 256 * 8;
+__device__ __forceinline__ void fold_channels(const GnaParams& p, int block, int64_t rows, double* red) {
   const int cl = threadIdx.x & 15, rl = (threadIdx.x >> 4) & 15, c = block * 16 + cl;
-  float a = 0.f, q = 0.f;
+  double a = 0.0, q = 0.0;
   if (threadIdx.x < 256 && c < p.C)
-    for (int64_t r = rl; r < rows; r += 16) { a += p.cpart[r * 2 * p.C + c]; q += p.cpart[r * 2 * p.C + p.C + c]; }
+    for (int64_t r = rl; r < rows; r += 16) { a += (double)p.cpart[r * 2 * p.C + c]; q += (double)p.cpart[r * 2 * p.C + p.C + c]; }
   if (threadIdx.x < 256) { red[rl * 16 + cl] = a; red[256 + rl * 16 + cl] = q; }
   __syncthreads();
   if (threadIdx.x < 16 && c < p.C) {
-    a = 0.f; q = 0.f;
+    a = 0.0; q = 0.0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) { a += red[r * 16 + cl]; q += red[256 + r * 16 + cl]; }
-    if (p.dbeta) p.dbeta[c] = a;
-    if (p.dgamma) p.dgamma[c] = q;
+    if (p.dbeta) p.dbeta[c] = (float)a;
+    if (p.dgamma) p.dgamma[c] = (float)q;
   }
 }
 __global__ __launch_bounds__(256) void gna_fold_channels_kernel(GnaParams p, int64_t rows) {
-  __shared__ float red[512];
+  __shared__ double red[FOLD_LDS / 8];
   fold_channels(p, (int)blockIdx.x, rows, red);
 }
 
@@ -620,7 +622,7 @@ __global__ __launch_bounds__(1024) void gna_grad_apply_kernel(GnaParams p) {
   extern __shared__ __align__(16) char smem[];
   if ((int)blockIdx.x >= p.apply_blocks) {
     if (blockIdx.y == 0)
-      fold_channels(p, (int)blockIdx.x - p.apply_blocks, (int64_t)p.B * p.strips, reinterpret_cast<float*>(smem));
+      fold_channels(p, (int)blockIdx.x - p.apply_blocks, (int64_t)p.B * p.strips, reinterpret_cast<double*>(smem));
     return;
   }
   float* s_a = reinterpret_cast<float*>(smem);
@@ -846,7 +848,7 @@ int gna_bwd(const GroupNormActArgs& a, const GnaPlan& pl, const DropArgs& drop, 
     const bool whole = gna_whole(p);
     GNA_VARIANTS(gna_grad_sums_kernel, dim3(pl.strips, p.B), pl.lds)
     p.apply_blocks = (a.dx0 || a.dx1) ? pl.strips : 0;
-    const int lds = 2 * p.G * 4 > 2048 ? 2 * p.G * 4 : 2048;
+    const int lds = 2 * p.G * 4 > FOLD_LDS ? 2 * p.G * 4 : FOLD_LDS;
     if (p.apply_blocks + fold_blocks) GNA_VARIANTS(gna_grad_apply_kernel, dim3(p.apply_blocks + fold_blocks, p.B), lds)
   }
   SDMI_CHECK_HIP(hipGetLastError());

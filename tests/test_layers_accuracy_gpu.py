@@ -224,3 +224,24 @@ def test_groupnorm_act_far_from_zero_over_strips():
     xh = (v - mean) * rstd
     exh = rstd * (emean + R.U * mean.abs()) + xh.abs() * (ers + 4 * R.U)
     R.check("y", y, xh.reshape(x.shape), R.rounded(xh, exh, torch.float32).reshape(x.shape))
+
+
+def test_weight_gradients_over_many_samples():
+    """dgamma and dbeta over 65535 samples of one slice each, whose sums the last launch folds: as exact as the terms.  A
+    slice's sums of two terms and their factors are within 12 u, the fold in double loses nothing, the result is fp32."""
+    b, c = 65535, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(b, 2, c, device="cuda").normal_(generator=g)
+    dy = torch.empty(b, 2, c, device="cuda").uniform_(0.5, 1.5, generator=g)
+    gamma, beta = torch.ones(c, device="cuda", requires_grad=True), torch.zeros(c, device="cuda", requires_grad=True)
+    y = ops.groupnorm_act(x, gamma, beta, 1e-5, act=None, groups=4)
+    dg, db = torch.autograd.grad(y, (gamma, beta), dy)
+    v = x.double().view(b, 2, 4, c // 4)
+    t = v - v.mean((1, 3), keepdim=True)
+    xh = (t / torch.sqrt((t * t).mean((1, 3), keepdim=True) + 1e-5)).view(b, 2, c)
+    # xh: 32 terms of the statistics, 3 roundings of its own and one of x against the mean
+    want, size = (dy.double() * xh).sum((0, 1)), (dy.double() * (2 * xh.abs() + 1)).sum((0, 1))
+    err = 16 * R.U * size / math.sqrt(2 * b) * 8              # independent from slice to slice: eight deviations
+    R.check("dgamma", dg, want.cpu(), (err + R.U * want.abs()).cpu())
+    want = dy.double().sum((0, 1))
+    R.check("dbeta", db, want.cpu(), (2 * R.U * want.abs()).cpu())
