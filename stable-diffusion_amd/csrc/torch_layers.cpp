@@ -7,12 +7,15 @@
 // sides of the package use one copy of it.  A call's kernels are launched without the interpreter lock.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/sdmi.h"
@@ -82,6 +85,15 @@ int dtype_code(const Tensor& x) {
 void check_like(const char* what, const Tensor& t, const Tensor& x, at::ScalarType dtype) {
   TORCH_CHECK_VALUE(t.device() == x.device(), what, " is on ", t.device(), ", expected ", x.device());
   TORCH_CHECK_VALUE(t.scalar_type() == dtype, what, " is ", dtype_name(t.scalar_type()), ", expected ", dtype_name(dtype));
+}
+// What records torch's operators (torch.jit.trace, make_fx, export) would record the allocation of a result and not the launch
+// that fills it, and give back whatever is in that memory when it runs.
+void check_not_traced() {
+  using c10::impl::TorchDispatchModeTLS;
+  const bool traced = torch::jit::tracer::isTracing() ||
+                      TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+                      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the layers with dropout cannot be traced: their launches are no operators of torch");
 }
 // forward-mode tangents would be lost without a word
 template <typename... T> void check_no_tangent(const T&... t) {
@@ -207,6 +219,7 @@ struct DropoutNode : Node {
 };
 
 Tensor dropout(const Tensor& x, double p, py::handle seed, int64_t offset, const OptTensor& resid_) {
+  check_not_traced();
   const Drop d = drop_state(p, seed, offset, x);
   const py::gil_scoped_release no_gil;
   check_columns(x.dim() ? x.size(-1) : 1);
@@ -276,6 +289,7 @@ struct LinearNode : Node {
 
 Tensor linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias_, const std::optional<std::string>& act_,
                   const OptTensor& resid_, double p, py::handle seed, int64_t offset) {
+  check_not_traced();
   const Drop d = drop_state(p, seed, offset, x);
   const py::gil_scoped_release no_gil;
   const int act = act_code(act_);
@@ -370,6 +384,7 @@ struct GroupNormNode : Node {
 Tensor groupnorm_act(const Tensor& x_, const Tensor& gamma_, const Tensor& beta_, double eps,
                      const std::optional<std::string>& act_, const OptTensor& x1_, int64_t groups, double p, py::handle seed,
                      int64_t offset) {
+  check_not_traced();
   const Drop d = drop_state(p, seed, offset, x_);
   const py::gil_scoped_release no_gil;
   const int act = act_code(act_), dt = dtype_code(x_);

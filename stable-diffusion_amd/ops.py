@@ -292,6 +292,8 @@ def inpaint_composite(image, mask, predicted):
 # any device, launch on that device's current stream and allocate with torch, so they can be captured into a graph;
 # there a `seed` in device memory makes every replay draw anew.  Capture a backward pass together with its forward
 # pass, and with no eager graph of the same leaves alive (torch joins the streams of a leaf's graphs).
+# They are no operators of torch's dispatcher: torch.jit.trace, make_fx and torch.export are refused (torch.compile breaks its
+# graph around them).
 
 def dropout(x, p, seed, offset=0, resid=None):
     """Dropout with a counter-based mask that is never stored: ``[resid +] keep * x / (1 - p)``, differentiable.
