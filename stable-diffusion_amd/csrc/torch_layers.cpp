@@ -95,6 +95,13 @@ void check_not_traced() {
                       c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, "the layers with dropout cannot be traced: their launches are no operators of torch");
 }
+// A wrapper subclass (DTensor, a fake tensor) has no memory of its own: its address is null, and an optional one would count as
+// missing.
+void check_memory(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t.unsafeGetTensorImpl()->is_python_dispatch(),
+                              "the layers with dropout need tensors each with memory of its own, no subclasses that hand their operators to Python");
+}
+void check_memory(const OptTensor& t) { if (t) check_memory(*t); }
 // forward-mode tangents would be lost without a word
 template <typename... T> void check_no_tangent(const T&... t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(t) || ...),
@@ -124,6 +131,7 @@ Drop drop_state(double p, py::handle seed, int64_t offset, const Tensor& x) {
   d.offset = offset;
   if (THPVariable_Check(seed.ptr())) {
     d.seed_t = THPVariable_Unpack(seed.ptr());
+    check_memory(d.seed_t);
     check_like("seed", d.seed_t, x, at::kLong);
     TORCH_CHECK_VALUE(d.seed_t.numel() == 1, "seed holds ", d.seed_t.numel(), " numbers, expected one");
     return d;
@@ -220,6 +228,7 @@ struct DropoutNode : Node {
 
 Tensor dropout(const Tensor& x, double p, py::handle seed, int64_t offset, const OptTensor& resid_) {
   check_not_traced();
+  check_memory(x); check_memory(resid_);
   const Drop d = drop_state(p, seed, offset, x);
   const py::gil_scoped_release no_gil;
   check_columns(x.dim() ? x.size(-1) : 1);
@@ -290,6 +299,7 @@ struct LinearNode : Node {
 Tensor linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias_, const std::optional<std::string>& act_,
                   const OptTensor& resid_, double p, py::handle seed, int64_t offset) {
   check_not_traced();
+  check_memory(x); check_memory(w); check_memory(bias_); check_memory(resid_);
   const Drop d = drop_state(p, seed, offset, x);
   const py::gil_scoped_release no_gil;
   const int act = act_code(act_);
@@ -385,6 +395,7 @@ Tensor groupnorm_act(const Tensor& x_, const Tensor& gamma_, const Tensor& beta_
                      const std::optional<std::string>& act_, const OptTensor& x1_, int64_t groups, double p, py::handle seed,
                      int64_t offset) {
   check_not_traced();
+  check_memory(x_); check_memory(gamma_); check_memory(beta_); check_memory(x1_);
   const Drop d = drop_state(p, seed, offset, x_);
   const py::gil_scoped_release no_gil;
   const int act = act_code(act_), dt = dtype_code(x_);
