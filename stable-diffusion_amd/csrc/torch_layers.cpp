@@ -114,6 +114,14 @@ void check_columns(int64_t n) {
   TORCH_CHECK_VALUE(n <= (int64_t)1 << 30, "rows of ", n, " columns are too long: at most 2^30");
 }
 
+// a tensor whose memory holds its values: not a view that torch negates lazily (the imaginary part of a conjugate), nor zeros
+// that it keeps without memory
+Tensor in_memory(const Tensor& t) {
+  if (C10_UNLIKELY(t.is_neg())) return t.resolve_neg();
+  if (C10_UNLIKELY(t._is_zerotensor())) return t.clone();
+  return t;
+}
+
 struct Drop {
   double p = 0.0;
   int64_t seed = 0, offset = 0;
@@ -134,6 +142,7 @@ Drop drop_state(double p, py::handle seed, int64_t offset, const Tensor& x) {
     check_memory(d.seed_t);
     check_like("seed", d.seed_t, x, at::kLong);
     TORCH_CHECK_VALUE(d.seed_t.numel() == 1, "seed holds ", d.seed_t.numel(), " numbers, expected one");
+    d.seed_t = in_memory(d.seed_t);
     return d;
   }
   const py::object i = py::reinterpret_steal<py::object>(PyNumber_Index(seed.ptr()));
@@ -158,7 +167,8 @@ int act_code(const std::optional<std::string>& act) {
 
 // a tensor as (rows, cols) with unit column stride: a view where the strides allow it
 struct Rows { Tensor t; int64_t ld = 0, rows = 0; };
-Rows rows_of(const Tensor& t, int64_t cols) {
+Rows rows_of(const Tensor& given, int64_t cols) {
+  const Tensor t = in_memory(given);
   Rows r{t, cols, cols ? t.numel() / cols : 0};
   if (t.is_contiguous()) return r;
   r.t = t.reshape({r.rows, cols});
@@ -316,7 +326,7 @@ Tensor linear_act(const Tensor& x, const Tensor& w, const OptTensor& bias_, cons
   if (bias.defined()) {
     check_like("bias", bias, x, at::kFloat);
     check_shape("bias", bias, {n});
-    bias = bias.contiguous();
+    bias = in_memory(bias).contiguous();
   }
   if (resid.defined()) {
     check_like("resid", resid, x, x.scalar_type());
@@ -365,7 +375,7 @@ struct GroupNormNode : Node {
     if (!grads[0].defined()) return g;
     {
       at::NoGradGuard no_grad;
-      const Tensor dy = grads[0].contiguous(), tx = x.unpack(), tx1 = c1 ? x1.unpack() : Tensor(), tg = gamma.unpack(),
+      const Tensor dy = in_memory(grads[0]).contiguous(), tx = x.unpack(), tx1 = c1 ? x1.unpack() : Tensor(), tg = gamma.unpack(),
                    tb = beta.unpack(), ts = stats.unpack(), seed_t = seeded ? seed.unpack() : Tensor();
       const bool need_x = task_should_compute_output(0), need_x1 = task_should_compute_output(1);
       Tensor dx, dx1;
@@ -417,8 +427,8 @@ Tensor groupnorm_act(const Tensor& x_, const Tensor& gamma_, const Tensor& beta_
   check_like("beta", beta_, x_, at::kFloat);
   check_shape("beta", beta_, {c});
   for (int64_t i = 1; i + 1 < x_.dim(); ++i) hw *= x_.size(i);
-  const Tensor x = x_.contiguous(), x1 = c1 ? x1_->contiguous() : Tensor(), gamma = gamma_.contiguous(),
-               beta = beta_.contiguous();
+  const Tensor x = in_memory(x_).contiguous(), x1 = c1 ? in_memory(*x1_).contiguous() : Tensor(),
+               gamma = in_memory(gamma_).contiguous(), beta = in_memory(beta_).contiguous();
   const Tensor y = at::empty(with_last(x, c), x.options()), stats = at::empty({b, groups, 2}, gamma.options());
   {
     at::NoGradGuard no_grad;

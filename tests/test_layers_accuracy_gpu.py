@@ -245,3 +245,32 @@ def test_weight_gradients_over_many_samples():
     R.check("dgamma", dg, want.cpu(), (err + R.U * want.abs()).cpu())
     want = dy.double().sum((0, 1))
     R.check("dbeta", db, want.cpu(), (2 * R.U * want.abs()).cpu())
+
+
+# ---- views ----------------------------------------------------------------------------------------------------------
+
+def test_views_with_the_negative_bit_and_zeros_without_memory():
+    """torch negates the imaginary part of a conjugate lazily, by a bit on the view and nothing in the memory, and keeps
+    some zeros as no memory at all: a layer sees the values."""
+    column = torch.complex(rand(70, 1), rand(70, 1, seed=1)).conj().imag
+    assert column.is_neg() and column.clone().is_neg() is False
+    assert torch.equal(ops.dropout(column, 0.3, 5, resid=column), ops.dropout(column.clone(), 0.3, 5, resid=column.clone()))
+    x, x1, r, w, b, g, h = (rand(*s, seed=i) for i, s in enumerate(((70, 64), (70, 64), (70, 32), (32, 64), (32,), (128,), (128,))))
+    calls = [(lambda t, u: ops.dropout(t, 0.3, 5, resid=u), (x, x1)),
+             (lambda t, a, c, u: ops.linear_act(t, a, c, act="silu", resid=u, p=0.2, seed=1), (x, w, b, r)),
+             (lambda t, u, a, c: ops.groupnorm_act(t.view(2, 35, 64), a, c, groups=8, x1=u.view(2, 35, 64)), (x, x1, g, h))]
+    for call, args in calls:
+        for odd, same in ((torch._neg_view, torch.neg), (lambda t: torch._efficientzerotensor(t.shape, device="cuda"), torch.zeros_like)):
+            for i in range(len(args)):
+                leaves = [a.detach().requires_grad_() for a in args]
+                ys = [call(*(f(a) if j == i else a for j, a in enumerate(leaves))) for f in (odd, same)]
+                assert torch.equal(*ys), i
+                dy = rand(*ys[0].shape, seed=8)
+                others = [a for j, a in enumerate(leaves) if j != i]
+                for a, c in zip(*(torch.autograd.grad(y, others, dy) for y in ys)):
+                    assert torch.equal(a, c), i
+            leaves = [a.detach().requires_grad_() for a in args]
+            for a, c in zip(*(torch.autograd.grad(call(*leaves), leaves, f(rand(*ys[0].shape, seed=8))) for f in (odd, same))):
+                assert torch.equal(a, c)
+    seed = torch.tensor([7], device="cuda")
+    assert torch.equal(ops.dropout(x, 0.3, torch._neg_view(seed)), ops.dropout(x, 0.3, -7))
