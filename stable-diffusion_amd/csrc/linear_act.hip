@@ -871,12 +871,16 @@ template <typename T> int join_splits(const Product& pr, hipStream_t stream) {
   if (pr.g.partial) SDMI_TRY(launch_join<T>(pr.g.partial, pr.g.splits, pr.g.e, stream));
   return SDMI_OK;
 }
-void product_label(char (&label)[96], const GemmParams& g) {
-  if (prof_on()) snprintf(label, sizeof(label), "linear M%lld N%d K%lld", (long long)g.e.M, g.e.N, (long long)g.K);
+// sizes, tile and splits, for the profiler's records
+void product_label(char (&label)[96], const Product& pr, unsigned more_splits = 0) {
+  if (!prof_on()) return;
+  const int n = snprintf(label, sizeof(label), "linear M%lld N%d K%lld %dx%d%s/%u", (long long)pr.g.e.M, pr.g.e.N, (long long)pr.g.K,
+                         pr.pl.bm, pr.pl.bn, pr.vec ? "" : "u", pr.g.splits);
+  if (more_splits) snprintf(label + n, sizeof(label) - n, "+%u", more_splits);      // dx beside dW
 }
 template <typename T, bool QC, bool PC> int run_product(const Product& pr, hipStream_t stream) {
   char label[96] = "";
-  product_label(label, pr.g);
+  product_label(label, pr);
   {
     ProfScope prof(PROF_OTHER, stream, 2.0 * pr.g.e.M * (double)pr.g.e.N * pr.g.K, 0.0, label);
     if (pr.vec) launch_tiles<T, QC, PC, true>(pr.g, pr.pl, stream);
@@ -896,7 +900,7 @@ template <typename T, bool VEC> void launch_grads(const Product& w, const Produc
 }
 template <typename T> int run_grads(const Product& w, const Product& x, hipStream_t stream) {
   char label[96] = "";
-  product_label(label, w.g);
+  product_label(label, w, x.g.splits);
   {
     ProfScope prof(PROF_OTHER, stream, 4.0 * w.g.e.M * (double)w.g.e.N * w.g.K, 0.0, label);
     if (w.vec) launch_grads<T, true>(w, x, stream);
@@ -1006,7 +1010,7 @@ int linear_few(const LinearActArgs& a, const Epilogue& e, hipStream_t s) {
   GemmParams g = {};
   g.q = (const char*)a.x; g.p = (const char*)a.w; g.ldq = a.ldx; g.ldp = a.ldw; g.K = a.k; g.e = e;
   char label[96] = "";
-  if (prof_on()) snprintf(label, sizeof(label), "linear M%lld N%d K%d", (long long)a.rows, a.n, a.k);
+  if (prof_on()) snprintf(label, sizeof(label), "linear M%lld N%d K%d few", (long long)a.rows, a.n, a.k);
   ProfScope prof(PROF_OTHER, s, 2.0 * a.rows * (double)a.n * a.k, (double)a.n * a.k * sizeof(T), label);
   const dim3 grid((unsigned)(a.n + 15) / 16);
   if (a.rows <= 16) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, dim3(512), 0, s, g);
