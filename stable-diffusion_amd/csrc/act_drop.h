@@ -180,7 +180,7 @@ template <typename T> __device__ __forceinline__ void store8(T* p, int n, const 
 
 #endif
 
-// n / d for 0 <= n < 2^31 by one multiply-high (d >= 1)
+// n / d for 0 <= n < 2^31 by one multiply-high (d >= 1): division by an invariant, Granlund and Montgomery 1994
 struct FastDiv { unsigned mul, shift, d; };
 static inline FastDiv fast_div(unsigned d) {
   FastDiv f{0, 0, d};

@@ -71,8 +71,8 @@ __device__ __forceinline__ void store_n(T* p, const float (&v)[W]) {
   }
 }
 // Eight columns of a two-source tensor that a thread walks down, from row `row0` on.  WHOLE: all groups of eight lie in one
-// source, 16-byte pieces (32 in fp32) that stay packed until they are used; otherwise a row's short last group and one
-// that straddles the sources go element by element.
+// source, 16-byte pieces (32 in fp32) that stay packed until they are used; otherwise every group goes element by element, as a
+// row's short last group and one that straddles the sources must.
 template <typename T, bool WHOLE> struct Cols;
 template <typename T> struct Cols<T, true> {
   typedef T Raw __attribute__((ext_vector_type(8)));
@@ -220,8 +220,7 @@ __device__ __forceinline__ void grad_u(const GnaParams& p, unsigned k0, unsigned
   act_grad_n<T>(u, du, p.act);
 }
 
-// Backward of a slice: x and du in LDS.  Channel sums: a thread keeps one vector column (blockDim is a multiple of
-// the vectors per pixel, or the channels are walked one after the other), folded over the pixel lanes in LDS.
+// Backward of a slice: x and du stay in LDS from the group's sums to dx and the channels' sums.
 template <typename T, int W>
 __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
   extern __shared__ __align__(16) char smem[];
@@ -272,8 +271,7 @@ __global__ __launch_bounds__(1024) void gna_slice_bwd_kernel(GnaParams p) {
     }
   }
   if (!p.dgamma && !p.dbeta) return;
-  // channel sums over the pixels: the block's threads as pl pixel lanes x channels, a lane's sums folded by shuffles
-  // where a group of lanes is whole, else through red: one wave per channel
+  // channel sums over the pixels: a wave per channel, its lanes' sums folded by shuffles
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nw = blockDim.x >> 6;
   for (int c = wave; c < p.cpg; c += nw) {
     float s1 = 0.f, s2 = 0.f;
