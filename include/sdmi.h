@@ -340,7 +340,7 @@ int sdmi_linear_act(const void* x, int64_t ldx, const void* w, int64_t ldw, cons
                     int64_t ldr, void* out, float* preact, int64_t rows, int k, int n, int act, double p, int64_t seed,
                     const int64_t* seed_dev, int64_t offset, void* workspace, int dtype, void* stream);
 /* dz = dropout(dy) act'(z); dx = dz W [rows][k], dw = dz^T x [n][k] in dtype, db = column sums of dz, fp32; each may
- * be NULL.  want of the workspace: 1 dx + 2 dw + 4 db.  preact is needed with an activation only.  resid's gradient
+ * be NULL.  With an activation 16-bit products take dz in two parts: dx and dw are as exact as their own rounding.  want of the workspace: 1 dx + 2 dw + 4 db.  preact is needed with an activation only.  resid's gradient
  * is dy. */
 int64_t sdmi_linear_act_backward_workspace_bytes(int64_t rows, int k, int n, int act, double p, int want, int dtype);
 int sdmi_linear_act_backward(const void* dy, int64_t lddy, const float* preact, const void* x, int64_t ldx, const void* w,
@@ -348,7 +348,7 @@ int sdmi_linear_act_backward(const void* dy, int64_t lddy, const float* preact, 
                              int64_t seed, const int64_t* seed_dev, int64_t offset, void* workspace, int dtype,
                              void* stream);
 /* out = dropout(act(GroupNorm(x0 | x1))), channels last; x1 NULL with c1 = 0.  Any channel count up to 8192 that
- * `groups` divides, any hw.  stats: fp32 [batch][groups][2], receives (mean, 1 / sqrt(var + eps)). */
+ * `groups` divides, a batch of up to 65535, any hw.  stats: fp32 [batch][groups][2], receives (mean, 1 / sqrt(var + eps)). */
 int64_t sdmi_groupnorm_act_workspace_bytes(int batch, int64_t hw, int c0, int c1, int groups, int dtype, int backward);
 int sdmi_groupnorm_act(const void* x0, int c0, const void* x1, int c1, int batch, int64_t hw, int groups, float eps,
                        const float* gamma, const float* beta, int act, double p, int64_t seed, const int64_t* seed_dev,

@@ -12,11 +12,12 @@
 // of a strip updates its columns' running means and squares about them (Welford 1962); a group's threads and columns, and
 // then the strips, are joined by the squares of their means' distances from the joint mean (Chan, Golub, LeVeque 1979).
 //
-// Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 11 us (HBM: 8), apply 23, gradient
-// sums 23, gradient apply 26 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
+// Bounds, MI355X, 16x64x64x320 bf16 (42 MB a tensor) with SiLU and dropout: statistics 13 us (HBM: 8), apply 22, gradient
+// sums 22, gradient apply 24 us.  The last three are the vector ALU's: a wave spends about 1100 cycles on the generator
 // (480) and the SiLU (its exponential and reciprocal at a quarter of the rate) of 512 elements, 20 us in all, where HBM
-// would take 16, 16 and 24.  3x37x53x480 fp32: 7, 9, 9 and 9 us, launches and the fold of the strips.  One workgroup per
-// slice: 2x8x8x1280 fp16 forward 5.6 us, 16x16x16x1280 bf16 12 forward, 23 backward.
+// would take 16, 16 and 24.  3x37x53x480 fp32: 8, 10, 9 and 10 us, launches and the fold of the strips.  One workgroup per
+// slice: 2x8x8x1280 fp16 forward 5.8 us, a launch; 16x16x16x1280 bf16 12 forward, 19 + 4 backward (HBM: 4 and 6): 512 workgroups,
+// one round of two per CU, whose load, three sums over the workgroup and store wait for one another.
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
@@ -706,8 +707,8 @@ GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backwa
   for (int w = 8; w > 1; w >>= 1)
     if (cpg % w == 0 && c0 % w == 0) { pl.w = w; break; }
   // beyond 8192 accesses a slice keeps its workgroup longer than two launches over strips take (bf16, us forward:
-  // 3x37x53x480, 15 channels a group one by one, 37 against 15; 16x32x32x960 in pairs 37 against 28; but 16x32x32x640 in
-  // fours 18 against 21)
+  // 3x37x53x480, 15 channels a group one by one, 23 against 14; 16x32x32x960 in pairs 27 against 25; but 16x32x32x640 in
+  // fours 17 against 23)
   if (HW * (cpg / pl.w) <= 8192 && (size_t)HW * cpg * per <= 60 * 1024) {
     pl.slice = 1;
     pl.lds = (int)((size_t)HW * cpg * per);
@@ -718,8 +719,8 @@ GnaPlan gna_plan(int B, int64_t HW, int c0, int c1, int G, int dtype, int backwa
   // About 1024 waves' worth of threads on the chip at a time (128 registers each): 512 blocks of 512, every pixel lane at
   // least four pixels.  Every block of the second launch folds its sample's strips, so where few samples would get more
   // than 128 strips each, and where a row alone takes half a block, it is 256 blocks of 1024.  Forward + backward, bf16,
-  // us: 16x64x64x320 84 (92 with the large blocks), 2x64x64x320 34 (44), 1x256x256x256 75 (93 with the small ones),
-  // 1x40x30x2560 45 (58).  A lane adds at most 512 values one after the other.
+  // us: 16x64x64x320 80 (84 with the large blocks), 2x64x64x320 32 (42), 1x256x256x256 73 (90 with the small ones),
+  // 1x40x30x2560 45 (56).  A lane adds at most 512 values one after the other.
   const int ncg = (C + 7) / 8;
   int lanes;
   int64_t strips;

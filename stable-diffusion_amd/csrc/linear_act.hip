@@ -6,9 +6,11 @@
 //   forward  Q = x  rows,     P = W  rows
 //   dx       Q = dz rows,     P = W  columns   (contraction over the layer's outputs)
 //   dW       Q = dz columns,  P = x  columns   (contraction over the tokens, split over workgroups)
-// Bounds, MI355X: the matrix rate where the contraction is long (8192x4096x4096 fp16: forward 217 us = 1269 TFLOP/s, dx 238,
-// dW 233; a plain library product 212), HBM where it is short (65536x320x320 bf16: forward with bias, dropout and residual
-// 38 us for 126 MB, dx 27 and dW 28 + 6 us), latency where there is little of anything (308x768x768 bf16 forward 8 us).
+// Bounds, MI355X: the matrix rate where the contraction is long (8192x4096x4096 fp16: forward 220 us = 1249 TFLOP/s, dx 233,
+// dW 227; a plain library product 212), HBM where it is short (65536x320x320 bf16: forward with bias, dropout and residual
+// 38 us for 126 MB, dx 25 and dW 31 + 6 us), latency where there is little of anything (308x768x768 bf16 forward 8 us).
+// With an activation 16-bit dx and dW take dz in two parts and twice the products' time (4096x1280x5120 bf16: 103 + 13 and
+// 114 + 12 us, joins of the splits behind the plus).
 #include "act_drop.h"
 #include "ops.h"
 #include <stdio.h>
@@ -513,8 +515,8 @@ __global__ __launch_bounds__(64 * WQ * WP) void linear_gemm_kernel(GemmParams p)
   gemm_block<T, WQ, WP, FQ, FP, QC, PC, VEC, PAIR>(p, blockIdx.x, smem);
 }
 // dW and dx in one launch: products that leave CUs idle one after the other share them.  us, replayed, apart / together:
-// 308x768x768 bf16 16.2 / 9.8, 406x256x384 fp16 11.1 / 6.1, 1003x517x259 fp32 23.6 / 19.7, 22932x128x2112 fp16 with its dz 153 / 154;
-// over 400 sizes 1.29 times faster at the mean, 0.92 at worst
+// 308x768x768 bf16 13.4 / 9.2 (with an activation's dz in two parts 22.6 / 16.5), 406x256x384 fp16 11.2 / 6.4, 1003x517x259 fp32
+// 28.1 / 23.6, 22932x128x2112 fp16 63 / 62 (218 / 211); over 300 sizes 1.33 times faster at the mean, 0.93 at worst
 template <typename T, int FQ, int FP, bool VEC>
 __global__ __launch_bounds__(256) void linear_grads_kernel(GemmParams w, GemmParams x) {
   __shared__ __align__(16) char smem[lds_bytes<2, 2, FQ, FP>()];
@@ -657,9 +659,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinParams p) {
 }
 
 // ---- dz = drop(dy) act'(z), and the strips' column sums ----------------------------------------------
-// HBM (65536x320 bf16 without an activation 19 us, 4.4 TB/s; 4096x5120 bf16 with GELU and dropout 34 us, 4.9 TB/s, in spite of
-// about 1700 cycles a wave for 512 elements).  One row at a time and many waves: with two rows in flight and two thirds of
-// the waves these were 22 and 40 us.
+// HBM (65536x320 bf16 without an activation 19 us, 4.4 TB/s; 4096x5120 bf16 with GELU and dropout 43 us for 210 MB, 4.9 TB/s,
+// in spite of about 1700 cycles a wave for 512 elements).  One row at a time and many waves: with two rows in flight and
+// two thirds of the waves the first was 22 us, and the second, then without dz's low part, 40 instead of 34.
 // With an activation dz is held halved, before the mask's scale, which wait for the products' epilogue (and the sums'): |act'|
 // is at most 1.13, so a finite dy gives a finite dz in its own type.  Its low part is held larger by LO_SCALE: fp16 has no
 // numbers below 2^-24, where the low parts of everything below 2^-13 lie; the first part of at most 2^15.2 leaves at most
@@ -918,9 +920,9 @@ BwdLayout bwd_layout(int64_t M, int K, int N, int act, bool drop, int want, int 
   w.need_dz = (act != ACT_NONE || drop) && (want & 3);
   // With an activation dz = dy act'(z) does not fit the tensors' type, and rounded to it adds an error to dx and dw as
   // large as the rounding of their own (error against 64 bits 1.41 times that of an unrounded dz, more where a few
-  // entries dominate; 43 % of the entries of 4096x1280x5120 bf16 then are not the ones that 64 bits round to, 0.2 % so).
+  // entries dominate; 43 % of the entries of 4096x1280x5120 bf16 then are not the ones that 64 bits round to, 0.5 % so).
   // The products therefore take dz in two parts of the type, at any size: how exact a sample's gradient is may not depend
-  // on how many others come with it.  The second part costs the products' time again (4096x1280x5120 bf16: 364 us a training pass, 266 with dz rounded).
+  // on how many others come with it.  The second part costs the products' time again (4096x1280x5120 bf16: 367 us a training pass, 266 with dz rounded).
   w.split = w.need_dz && act != ACT_NONE && esize == 2;
   w.plan_x = plan_product(M, K, N, esize, GRAD_X, w.split);
   w.plan_w = plan_product(N, K, M, esize, GRAD_W, w.split);

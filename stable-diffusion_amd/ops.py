@@ -319,7 +319,9 @@ def linear_act(x, w, bias=None, act=None, resid=None, p=0.0, seed=None, offset=0
 
     x (..., K), w (N, K) and resid (..., N) in one dtype (fp32, fp16, bf16), bias fp32 (N,).  act: None, "silu",
     "gelu" (erf) or "quick_gelu" (z sigmoid(1.702 z)); p, seed, offset as in ``dropout``.  With an activation a
-    training call keeps x w^T + bias in fp32.  Any sizes from one on; rows of whole 16-byte pieces are fastest."""
+    training call keeps x w^T + bias in fp32, and in 16 bits the gradients of x and w take z's gradient in two parts of the
+    type (twice the products' time), so that they are as exact as their own rounding at every size.  Any sizes from one
+    on; rows of whole 16-byte pieces are fastest."""
     return _lib.layers().linear_act(x, w, bias, act, resid, p, seed, offset)
 
 
@@ -328,5 +330,5 @@ def groupnorm_act(x, gamma, beta, eps=1e-5, act="silu", x1=None, groups=32, p=0.
 
     x (B, ..., C0) [and x1 (B, ..., C1), concatenated behind it] -> (B, ..., C0 + C1); gamma, beta fp32 (C0 + C1,).
     act as in ``linear_act``, p / seed / offset as in ``dropout`` (a pixel is a row).  Any number of channels per
-    group (8192 channels in all at most) and any image size; ``groupnorm`` is the inference path's own kernel."""
+    group (8192 channels in all and 65535 samples at most) and any image size; ``groupnorm`` is the inference path's own kernel."""
     return _lib.layers().groupnorm_act(x, gamma, beta, eps, act, x1, groups, p, seed, offset)
